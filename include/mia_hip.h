@@ -458,6 +458,136 @@ int mhip_sample(mhip_ctx *c, mhip_sampler *s, const float *d_logits, void *d_scr
 #define MHIP_CHAIN_GT 2
 int mhip_chain_f32(mhip_ctx *c, const float *d_v, int n, int mode, float thr, int *d_out);
 
+/* ---- a key/value cache in pages, for a batch of sequences -----------------
+ * No counterpart in the reference, which keeps one contiguous cache for one
+ * sequence. Tokens are kept in pages of a fixed number of tokens; a
+ * sequence is a slot: a row of the table (its pages in token order) and a
+ * length. Sequences that begin with the same tokens share the pages that
+ * those tokens fill; a page that is not full belongs to one sequence.
+ *
+ * Every call is queued on the context's stream and allocates nothing; the
+ * state it works on (table, lengths, counts) is device memory, so calls can
+ * be captured into a graph and replayed. Calls on one cache must be ordered
+ * by the caller when made from several contexts. Which pages a call takes
+ * is fixed: the free pages of lowest index, in the order of the call's list.
+ * An invalid call that the host sees returns -1; what only the device sees
+ * (an index out of range, a slot twice in one list, no page left) sets bits
+ * of mhip_pages_status and leaves memory outside the cache alone.
+ */
+#define MHIP_F32 0 /* element types of the cache, and of rows in and out */
+#define MHIP_F16 1
+#define MHIP_BF16 2
+typedef struct {
+    int type;                           /* MHIP_F32, MHIP_F16, MHIP_BF16 */
+    int n_layers, n_kv_heads, head_dim; /* head_dim a multiple of 16, <= 256; heads <= 256 */
+    int page;                           /* tokens of a page: 16, 32, 64, 128 or 256 */
+    int n_pages;                        /* <= 2^20 */
+    int max_seqs;                       /* slots, <= 65536 */
+    int max_blocks;                     /* pages of one slot; max_blocks * page <= 2^30 */
+} mhip_page_dims;
+typedef struct {
+    void *k, *v; /* [n_layers][n_pages][n_kv_heads][page][head_dim], 16-byte aligned */
+    int *table;  /* [max_seqs][max_blocks] page, or -1 */
+    int *len;    /* [max_seqs] tokens */
+    int *refs;   /* [n_pages] slots that hold the page, 0: free */
+    int *state;  /* [16], zero at first: error bits, then words of the library */
+    int *plan;   /* mhip_pages_plan_bytes(): workspace of one call at a time */
+} mhip_pages;
+/* Bytes of a whole cache (0 for invalid dimensions), and its arrays carved
+ * out of d_base (256-byte aligned); mhip_pages_clear empties every slot. */
+size_t mhip_pages_bytes(const mhip_page_dims *s);
+size_t mhip_pages_plan_bytes(const mhip_page_dims *s);
+int mhip_pages_carve(const mhip_page_dims *s, void *d_base, mhip_pages *out);
+int mhip_pages_clear(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p);
+/* Slot d_seqs[i] (n different ones) grows by d_count[i] >= 0 tokens (NULL:
+ * one each) and gets the pages it needs: all slots, or (error bits) none. */
+int mhip_pages_extend(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
+                      const int *d_seqs, const int *d_count, int n);
+/* The keys and values of one layer for the last d_count[i] tokens of each
+ * slot (NULL: max_count each): token j < d_count[i] of entry i is row
+ * i * max_count + j of d_k and d_v (rows of n_kv_heads * head_dim values, ld
+ * values apart, 16-byte aligned as the rows' step is; rows past d_count[i] are
+ * not read). */
+int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,
+                     const int *d_seqs, const int *d_count, int n, int max_count,
+                     const void *d_k, const void *d_v, int ld);
+/* The empty slot d_dst[i] becomes a copy of slot d_src[i] (which may repeat,
+ * and be no d_dst): full pages are shared, the tokens of a page that is
+ * not full are copied to a page of its own, in every layer. MHIP_PAGES_DEEP
+ * copies every page instead. All n, or (error bits) none. */
+#define MHIP_PAGES_DEEP 1
+int mhip_pages_fork(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, const int *d_src,
+                    const int *d_dst, int n, int flags);
+/* Empties the slots; pages that no slot holds any more are free. An empty
+ * slot, or one twice in the list, is no error. */
+int mhip_pages_free(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, const int *d_seqs,
+                    int n);
+/* Moves pages so that the n pages in use are pages 0 .. n - 1: the i-th free
+ * page below n receives the i-th page in use from n on. Pages moved from keep
+ * their bytes. */
+int mhip_pages_compact(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p);
+/* Waits for the stream: status[0] the error bits since the last call (then
+ * cleared; a call that failed changed nothing, except that entries which
+ * are in order are still done by _write, _free and attention), status[1] the
+ * free pages. */
+#define MHIP_PAGES_NO_SPACE 1 /* too few free pages, or a slot longer than max_blocks */
+#define MHIP_PAGES_BAD 2      /* an index out of range, a slot twice, a d_dst in use */
+int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int status[2]);
+
+/*
+ * Attention over the cache for a batch of n slots with up to max_count
+ * tokens each (1: a decode step; more: drafted tokens, prompt chunks), whose
+ * rows are in the cache already (mhip_pages_extend and _write come first).
+ * Row i * max_count + j of d_q ([n_heads][head_dim] values of the cache's
+ * type, rows ldq values apart) is token j of slot d_seqs[i], at position
+ * t = len - d_count[i] + j (d_count NULL: max_count each); it attends to its
+ * slot's positions 0 .. t: softmax(scale q.k) v per query head, n_heads a
+ * multiple of n_kv_heads. Rows past d_count[i], and rows of an empty slot, are
+ * zeros in d_out (rows ldo values apart).
+ *
+ * The slots may share their first `prefix` tokens (0: they do not): those
+ * are read from slot prefix_seq's pages, once for the whole batch instead of
+ * once per slot, so slots that are a fork of prefix_seq or hold the same
+ * tokens give the same result as without. A slot shorter than the prefix
+ * sees the part that it has. max_len: no slot of the list is longer (the
+ * work is sized for it; a longer slot is an error bit and its row is NaN).
+ * d_q and d_out are 16-byte aligned as their rows' steps are. d_ws:
+ * mhip_attention_shared_ws_bytes() bytes, 256-byte aligned, of one call at a
+ * time (0 for invalid arguments). Scores, softmax and sums are fp32; with a
+ * 16-bit cache the softmax's weights are rounded to that type for the
+ * product with v. Where a page of the table is out of range its tokens
+ * count as zeros, with an error bit. */
+size_t mhip_attention_shared_ws_bytes(const mhip_page_dims *s, int n_heads, int n, int max_count,
+                                      int prefix, int max_len);
+int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,
+                          int n_heads, const void *d_q, int ldq, void *d_out, int ldo,
+                          const int *d_seqs, const int *d_count, int n, int max_count,
+                          int prefix_seq, int prefix, int max_len, float scale, void *d_ws);
+
+/* ---- weights in 4 bits ------------------------------------------------------
+ * No counterpart in the reference (Q8_0 and fp32 weights). A row of cols
+ * weights in groups of `group` (32, 64 or 128, dividing cols): weight =
+ * scale * code, code -8 .. 7 in two's complement. d_codes[rows][cols/2]: the
+ * even column in the low four bits (16-byte aligned); d_scales
+ * [rows][cols/group] in fp16. */
+/* Codes and scales of fp32 weights: scale = max|w| / 7 rounded to fp16 (at
+ * most 65504), code = the nearest integer of w / scale, kept in [-8, 7] (0 where
+ * the scale rounds to 0). */
+int mhip_quantize_q4(mhip_ctx *c, const float *d_w, int rows, int cols, int group, void *d_codes,
+                     void *d_scales);
+int mhip_dequantize_q4(mhip_ctx *c, const void *d_codes, const void *d_scales, int rows, int cols,
+                       int group, float *d_w);
+/* out[t][r] = sum over c of w[r][c] x[t][c] for n tokens: x and out of `type`
+ * (MHIP_F32, ...), rows ldx and ldo values apart (x 16-byte aligned as its
+ * rows' step is), sums in fp32. fp32 x enters the products with 22 bits or
+ * more of each value's (values 2^29 below the largest of 1024 columns lose
+ * further bits); 16-bit x enters whole. d_ws: mhip_matvec_q4_ws_bytes() bytes, 256-byte
+ * aligned, of one call at a time (0 for invalid arguments). */
+size_t mhip_matvec_q4_ws_bytes(int type, int cols, int n);
+int mhip_matvec_q4(mhip_ctx *c, int type, void *d_out, int ldo, const void *d_codes,
+                   const void *d_scales, int group, const void *d_x, int ldx, int rows, int cols,
+                   int n, void *d_ws);
+
 /* ---- reference tensor ops on device pointers ---------------------------- */
 /* Q8_0 blocks in the reference's 36-byte format. */
 int mhip_quantize_q8(mhip_ctx *c, const float *d_x, void *d_blocks, int n);

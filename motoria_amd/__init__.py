@@ -31,6 +31,9 @@ MHIP_DECODE_CHAINS_FIRST = 32
 MHIP_ATTN_FORCE_ABORT = 64
 MHIP_CHAIN_SUM, MHIP_CHAIN_GE, MHIP_CHAIN_GT = 0, 1, 2
 MHIP_MODEL_PER_LAYER = 128
+MHIP_F32, MHIP_F16, MHIP_BF16 = 0, 1, 2
+MHIP_PAGES_DEEP = 1
+MHIP_PAGES_NO_SPACE, MHIP_PAGES_BAD = 1, 2
 MHIP_DECODE_CERTIFIED = 256
 MHIP_FAST_DOWN = 512
 MHIP_MODEL_STACK_MAX_SEQ = 8192  # longest context of the model stack (mia_hip.h)
@@ -66,6 +69,17 @@ class Scratch(ctypes.Structure):
 class AttnDims(ctypes.Structure):
     _fields_ = [("dim", _i), ("n_heads", _i), ("n_kv_heads", _i), ("head_dim", _i),
                 ("norm_eps", _f)]
+
+
+class PageDims(ctypes.Structure):
+    """mhip_page_dims (include/mia_hip.h)."""
+    _fields_ = [(n, _i) for n in ("type", "n_layers", "n_kv_heads", "head_dim", "page", "n_pages",
+                                  "max_seqs", "max_blocks")]
+
+
+class PageArrays(ctypes.Structure):
+    """mhip_pages (include/mia_hip.h)."""
+    _fields_ = [(n, _p) for n in ("k", "v", "table", "len", "refs", "state", "plan")]
 
 
 class Sampler(ctypes.Structure):
@@ -175,6 +189,27 @@ SIGNATURES = {
     "mhip_model_stack_supported": (_i, [_p, _p, _p, _i]),
     "mhip_model_stack": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _p, _i, _p,
                               _p, _i]),
+    "mhip_pages_bytes": (_sz, [ctypes.POINTER(PageDims)]),
+    "mhip_pages_plan_bytes": (_sz, [ctypes.POINTER(PageDims)]),
+    "mhip_pages_carve": (_i, [ctypes.POINTER(PageDims), _p, ctypes.POINTER(PageArrays)]),
+    "mhip_pages_clear": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays)]),
+    "mhip_pages_extend": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _p, _p,
+                               _i]),
+    "mhip_pages_write": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _i, _p, _p,
+                              _i, _i, _p, _p, _i]),
+    "mhip_pages_fork": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _p, _p, _i,
+                             _i]),
+    "mhip_pages_free": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _p, _i]),
+    "mhip_pages_compact": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays)]),
+    "mhip_pages_status": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays),
+                               ctypes.POINTER(_i)]),
+    "mhip_attention_shared_ws_bytes": (_sz, [ctypes.POINTER(PageDims), _i, _i, _i, _i, _i]),
+    "mhip_attention_shared": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _i,
+                                   _i, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i, _f, _p]),
+    "mhip_quantize_q4": (_i, [_p, _p, _i, _i, _i, _p, _p]),
+    "mhip_dequantize_q4": (_i, [_p, _p, _p, _i, _i, _i, _p]),
+    "mhip_matvec_q4_ws_bytes": (_sz, [_i, _i, _i]),
+    "mhip_matvec_q4": (_i, [_p, _i, _p, _i, _p, _p, _i, _p, _i, _i, _i, _i, _p]),
     "mhip_quantize_q8": (_i, [_p, _p, _p, _i]),
     "mhip_dequantize_q8": (_i, [_p, _p, _p, _i]),
     "mhip_matvec": (_i, [_p, _p, _p, _i, _p, _p, _i, _i]),
@@ -523,6 +558,86 @@ class Gpu:
         out = np.zeros(shape, dtype=dtype)
         self.check(lib().mhip_d2h(self.h, _ptr(out), p, out.nbytes), "d2h")
         return out
+
+
+def pages_plan_bytes(dims):
+    """mhip_pages_plan_bytes (0 for invalid dimensions)."""
+    return lib().mhip_pages_plan_bytes(ctypes.byref(dims))
+
+
+class Pages:
+    """A paged key/value cache (mhip_pages) on a Gpu context. Its arrays are
+    device pointers given by name (k, v, table, len, refs, state, plan), or,
+    without any, one allocation of its own, emptied. Lists of slots and counts are
+    device pointers to ints; calls are queued on the context's stream."""
+
+    def __init__(self, gpu, dims, **arrays):
+        self.gpu, self.dims, self.mem = gpu, dims, None
+        self.arrays = PageArrays(**arrays)
+        self._d, self._a = ctypes.byref(self.dims), ctypes.byref(self.arrays)
+        if not arrays:
+            nbytes = lib().mhip_pages_bytes(self._d)
+            if not nbytes:
+                raise ValueError("not a cache this library runs")
+            self.mem = gpu.malloc(nbytes)
+            if lib().mhip_pages_carve(self._d, self.mem, self._a) != 0:
+                raise RuntimeError("mhip_pages_carve")
+            self.clear()
+
+    def close(self):
+        if self.mem:
+            self.gpu.free(self.mem)
+            self.mem = None
+
+    def clear(self):
+        self.gpu.check(lib().mhip_pages_clear(self.gpu.h, self._d, self._a), "mhip_pages_clear")
+
+    def extend(self, d_seqs, d_count, n):
+        self.gpu.check(lib().mhip_pages_extend(self.gpu.h, self._d, self._a, d_seqs, d_count, n),
+                       "mhip_pages_extend")
+
+    def write(self, layer, d_seqs, d_count, n, max_count, d_k, d_v, ld):
+        self.gpu.check(lib().mhip_pages_write(self.gpu.h, self._d, self._a, layer, d_seqs, d_count,
+                                              n, max_count, d_k, d_v, ld), "mhip_pages_write")
+
+    def fork(self, d_src, d_dst, n, flags=0):
+        self.gpu.check(lib().mhip_pages_fork(self.gpu.h, self._d, self._a, d_src, d_dst, n, flags),
+                       "mhip_pages_fork")
+
+    def free(self, d_seqs, n):
+        self.gpu.check(lib().mhip_pages_free(self.gpu.h, self._d, self._a, d_seqs, n),
+                       "mhip_pages_free")
+
+    def compact(self):
+        self.gpu.check(lib().mhip_pages_compact(self.gpu.h, self._d, self._a),
+                       "mhip_pages_compact")
+
+    def status(self):
+        """(error bits since the last call, free pages); waits for the stream."""
+        st = (_i * 2)()
+        self.gpu.check(lib().mhip_pages_status(self.gpu.h, self._d, self._a, st),
+                       "mhip_pages_status")
+        return st[0], st[1]
+
+    def attention_ws_bytes(self, n_heads, n, max_count, prefix, max_len):
+        return lib().mhip_attention_shared_ws_bytes(self._d, n_heads, n, max_count, prefix,
+                                                    max_len)
+
+    def attention(self, layer, n_heads, d_q, ldq, d_out, ldo, d_seqs, d_count, n, max_count,
+                  prefix_seq, prefix, max_len, scale, d_ws):
+        self.gpu.check(lib().mhip_attention_shared(
+            self.gpu.h, self._d, self._a, layer, n_heads, d_q, ldq, d_out, ldo, d_seqs, d_count, n,
+            max_count, prefix_seq, prefix, max_len, scale, d_ws), "mhip_attention_shared")
+
+
+def matvec_q4_ws_bytes(type, cols, n):
+    return lib().mhip_matvec_q4_ws_bytes(type, cols, n)
+
+
+def matvec_q4(gpu, type, d_out, ldo, d_codes, d_scales, group, d_x, ldx, rows, cols, n, d_ws):
+    """mhip_matvec_q4 on a Gpu context (queued)."""
+    gpu.check(lib().mhip_matvec_q4(gpu.h, type, d_out, ldo, d_codes, d_scales, group, d_x, ldx, rows,
+                                   cols, n, d_ws), "mhip_matvec_q4")
 
 
 class GpuModel:

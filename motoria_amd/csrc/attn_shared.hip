@@ -1,0 +1,118 @@
+// The entry points of the attention over a paged cache (include/mia_hip.h):
+// arguments, workspace and how a call is cut; its kernels are in
+// attn_shared.inc.
+#include "attn_shared.h"
+
+namespace {
+
+using mhip_shared::Cut;
+using mhip_shared::Job;
+using mhip_shared::PART_MAX;
+using mhip_shared::TILE;
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// How a call is cut. Every workgroup of the prefix reads its part for up to 128 rows, and
+// there should be one for every CU; a part of a slot is at least 256
+// positions while there are two workgroups per CU.
+Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int max_len) {
+    Cut k;
+    const int group = n_heads / s->n_kv_heads;
+    const long long rows = (long long)n * mc * group;
+    k.wr = rows > 32 ? 4 : rows > 16 ? 2 : 1;
+    k.rt = rows > 64 && s->head_dim <= 128 ? 2 : 1;
+    const int tile = k.wr * k.rt * 16;
+    k.ptiles = prefix > 0 ? (int)((rows + tile - 1) / tile) : 0;
+    k.sp = 0;
+    k.plen = 0;
+    if (prefix > 0) {
+        long long parts = 256 / ((long long)k.ptiles * s->n_kv_heads);
+        const int most = (prefix + 127) / 128, least = (prefix + PART_MAX - 1) / PART_MAX;
+        if (parts > most) parts = most;
+        if (parts < least) parts = least;
+        k.plen = (int)((prefix + parts - 1) / parts + TILE - 1) / TILE * TILE;
+        k.sp = (prefix + k.plen - 1) / k.plen;
+    }
+    const int rest = max_len - prefix;
+    k.stiles = (mc * group + 15) / 16;
+    long long parts = 512 / ((long long)n * s->n_kv_heads * k.stiles) + 1;
+    const int most = (rest + 255) / 256, least = (rest + PART_MAX - 1) / PART_MAX;
+    if (parts > most) parts = most;
+    if (parts < least) parts = least;
+    k.ss = parts < 1 ? 1 : (int)parts;
+    return k;
+}
+
+bool shape_ok(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int max_len) {
+    return n_heads >= 1 && n_heads <= 65536 && n_heads % s->n_kv_heads == 0 && n >= 1 &&
+           n <= s->max_seqs && mc >= 1 && (long long)n * mc * n_heads < 1 << 30 && prefix >= 0 &&
+           max_len >= prefix && max_len <= (long long)s->max_blocks * s->page;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mhip_attention_shared_ws_bytes(const mhip_page_dims *s, int n_heads, int n, int max_count,
+                                      int prefix, int max_len) {
+    if (!mhip_pages_plan_bytes(s) || !shape_ok(s, n_heads, n, max_count, prefix, max_len)) return 0;
+    const Cut k = cut_of(s, n_heads, n, max_count, prefix, max_len);
+    const size_t rows = (size_t)n * max_count * n_heads, parts = (size_t)k.sp + k.ss;
+    return align256(parts * rows * s->head_dim * 4) + align256(parts * rows * 8);
+}
+
+int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,
+                          int n_heads, const void *d_q, int ldq, void *d_out, int ldo,
+                          const int *d_seqs, const int *d_count, int n, int max_count,
+                          int prefix_seq, int prefix, int max_len, float scale, void *d_ws) {
+    const char *what = "attention shared";
+    if (mhip::check_pages(c, s, p, what)) return -1;
+    if (layer < 0 || layer >= s->n_layers) return mhip::fail(c, "%s: layer %d of %d", what, layer, s->n_layers);
+    if (n == 0 || max_count == 0) return 0;
+    if (!shape_ok(s, n_heads, n, max_count, prefix, max_len))
+        return mhip::fail(c, "%s: %d heads over %d, %d x %d tokens, prefix %d of %d positions", what,
+                          n_heads, s->n_kv_heads, n, max_count, prefix, max_len);
+    if (prefix > 0 && (prefix_seq < 0 || prefix_seq >= s->max_seqs))
+        return mhip::fail(c, "%s: prefix of slot %d of %d", what, prefix_seq, s->max_seqs);
+    const int esz = mhip::type_bytes(s->type);
+    if (ldq < n_heads * s->head_dim || ldo < n_heads * s->head_dim)
+        return mhip::fail(c, "%s: rows %d and %d apart (width %d)", what, ldq, ldo, n_heads * s->head_dim);
+    if (!d_q || !d_out || !d_seqs || !d_ws) return mhip::fail(c, "%s: a null argument", what);
+    if (((uintptr_t)d_q | (uintptr_t)d_out) % 16 || (size_t)ldq * esz % 16 || (size_t)ldo * esz % 16 ||
+        (uintptr_t)d_ws % 256)
+        return mhip::fail(c, "%s: rows must start on 16 bytes, the workspace on 256", what);
+    if (mhip::use_device(c)) return -1;
+    const Cut k = cut_of(s, n_heads, n, max_count, prefix, max_len);
+    Job a;
+    a.s = *s;
+    a.p = *p;
+    a.layer = layer;
+    a.nh = n_heads;
+    a.group = n_heads / s->n_kv_heads;
+    a.q = d_q;
+    a.ldq = ldq;
+    a.out = d_out;
+    a.ldo = ldo;
+    a.seqs = d_seqs;
+    a.count = d_count;
+    a.n = n;
+    a.mc = max_count;
+    a.prefix_seq = prefix_seq;
+    a.prefix = prefix;
+    a.max_len = max_len;
+    a.c = scale * 1.44269504088896341f;
+    a.lp = __builtin_ctz(s->page);
+    a.sp = k.sp;
+    a.plen = k.plen;
+    a.ptiles = k.ptiles;
+    a.ss = k.ss;
+    a.stiles = k.stiles;
+    const size_t rows = (size_t)n * max_count * n_heads, parts = (size_t)k.sp + k.ss;
+    a.o = (float *)d_ws;
+    a.ml = (float *)((uint8_t *)d_ws + align256(parts * rows * s->head_dim * 4));
+    if (s->type == MHIP_F32) return mhip_shared::launch_f32(c, a, k);
+    if (s->type == MHIP_F16) return mhip_shared::launch_f16(c, a, k);
+    return mhip_shared::launch_bf16(c, a, k);
+}
+
+}  // extern "C"

@@ -90,6 +90,10 @@ int launch_gateup_mfma(hipStream_t st, const mhip_dims *s, const mhip_layout *la
 int launch_down_mfma(hipStream_t st, const mhip_dims *s, const mhip_layout *lay,
                      const void *d_table_layer, const mhip_scratch *sc, int A, bool exact);
 
+// Arguments of the paged cache (pages.hip): 0 or fail().
+int check_pages(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, const char *what);
+inline int type_bytes(int type) { return type == MHIP_F32 ? 4 : 2; }
+
 }  // namespace mhip
 
 // ---- device helpers --------------------------------------------------------

@@ -1,0 +1,476 @@
+// Products with 4-bit weights in groups (include/mia_hip.h):
+//   out[t][r] = sum over groups g of scale[r][g] * (sum over c in g of code[r][c] x[t][c]).
+//
+// What bounds it: up to about 16 tokens the weights' bytes (4.5 bits each with
+// groups of 32), so the codes have to become matrix operands in few
+// instructions. A code is exact in fp16: nibble k and k + 4 of a word, masked
+// together and merged with the exponent of 1024, are the fp16 values 1024 + (code
+// + 8) (or 1024 + 16 (code + 8)), and one packed subtraction (or fused
+// multiply-add) leaves the two codes: 9 instructions for 8 weights. The inner
+// sums then run on the matrix cores, 16 rows x 16 tokens x 32 columns an
+// instruction with fp32 accumulators; with one token 15 of 16 of its columns are idle,
+// which still is faster than the vector units (2.25 instructions a weight).
+//
+// x as fp16 operands: k_q4_tokens scales each token's segment of 1024 columns by
+// a power of two that brings its largest value to [2^14, 2^15). A bf16 value
+// then is an fp16 value (8 bits; exact down to 2^-32 of the largest). An
+// fp32 value is split: hi = fp16(x'), lo = fp16((x' - hi) 2^11), together
+// within 2^-23 of x (a step of fp32's own rounding) down to 2^-29 of the
+// segment's largest value, as lo carries its own exponent; their products
+// are accumulated apart and joined in fp32. fp16 x is taken as it is.
+#include "mhip_internal.h"
+
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+
+constexpr int SEG = 1024;  // columns that share a token's power of two
+constexpr int TG = 64;     // tokens of one workgroup, at most
+
+// The workspace: per group of TG tokens (nt of them) the operands
+// [cols/32][pieces][nt][32] fp16, in each 32 the order of pair(), then
+// [cols/SEG][TG] the factors back.
+struct Tokens {
+    size_t operands, factors, group;  // bytes of each, and of a group
+};
+__host__ __device__ inline Tokens tokens_of(int type, int cols, int n) {
+    Tokens t;
+    const size_t nt = n < TG ? n : TG, pieces = type == MHIP_F32 ? 2 : 1;
+    t.operands = ((size_t)cols * pieces * nt * 2 + 255) & ~(size_t)255;
+    t.factors = ((size_t)((cols + SEG - 1) / SEG) * TG * 4 + 255) & ~(size_t)255;
+    t.group = t.operands + t.factors;
+    return t;
+}
+
+__device__ inline float value(float x) { return x; }
+__device__ inline float value(_Float16 x) { return (float)x; }
+__device__ inline float value(__bf16 x) { return (float)x; }
+
+// One workgroup a token and segment, four columns a thread.
+template <class T>
+__global__ __launch_bounds__(256) void k_q4_tokens(const T *x, int ldx, int cols, int n, int type,
+                                                   uint8_t *ws) {
+    constexpr bool split = sizeof(T) == 4;
+    __shared__ float top[4];
+    const int t = blockIdx.x, seg = blockIdx.y, tg = t / TG, nt = min(TG, n - tg * TG);
+    const Tokens l = tokens_of(type, cols, n);
+    uint8_t *base = ws + (size_t)tg * l.group;
+    const int c = seg * SEG + threadIdx.x * 4;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < cols) {
+        T r[4];
+        if constexpr (split) *(uint4 *)r = *(const uint4 *)(x + (size_t)t * ldx + c);
+        else *(uint2 *)r = *(const uint2 *)(x + (size_t)t * ldx + c);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = value(r[j]);
+    }
+    float scale = 1.0f;
+    if (type != MHIP_F16) {
+        float m = 0.0f;  // the largest finite magnitude
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float a = fabsf(v[j]);
+            m = a < __builtin_inff() && a > m ? a : m;
+        }
+        for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+        if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        // 2^(14 - exponent of m); values below 2^-112 keep the factor 2^126
+        const int e = m > 0.0f ? ilogbf(m) : 14;
+        scale = ldexpf(1.0f, min(126, 14 - e));
+    }
+    if (threadIdx.x == 0)
+        ((float *)(base + l.operands))[(size_t)seg * TG + t % TG] = 1.0f / scale;  // exact: a power of two
+    if (c >= cols) return;
+    // columns 4i .. 4i + 3 of an eight: nibbles k and k + 4 are neighbours, so
+    // column k of the eight goes to place 2k (k < 4) or 2 (k - 4) + 1
+    const size_t block = c / 32, pieces = split ? 2 : 1;
+    _Float16 *o = (_Float16 *)base + ((block * pieces) * nt + t % TG) * 32 + (c % 32 / 8) * 8 +
+                  (c % 8 == 4 ? 1 : 0);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float s = v[j] * scale;
+        const _Float16 hi = (_Float16)s;
+        o[2 * j] = hi;
+        if constexpr (split) {
+            // an infinity or NaN is in hi alone
+            const float rest = (s - (float)hi) * 2048.0f;
+            o[(size_t)nt * 32 + 2 * j] = fabsf(rest) < __builtin_inff() ? (_Float16)rest : (_Float16)0.0f;
+        }
+    }
+}
+
+// Eight codes (nibbles of w) as fp16, nibble k next to nibble k + 4.
+__device__ __forceinline__ h8 codes(unsigned w) {
+    const h2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f}, off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const h2 by = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const unsigned z = w >> 8;
+    const h2 a = __builtin_bit_cast(h2, (w & 0x000f000fu) ^ 0x64086408u) + off;
+    const h2 b = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00f000f0u) ^ 0x64806480u), by, off16);
+    const h2 c = __builtin_bit_cast(h2, (z & 0x000f000fu) ^ 0x64086408u) + off;
+    const h2 d = __builtin_elementwise_fma(__builtin_bit_cast(h2, (z & 0x00f000f0u) ^ 0x64806480u), by, off16);
+    return (h8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// A lane of group g (16 lanes) has loaded words 0..3 of column block g; the matrix
+// instructions want word g of block j: the transpose of words and lane
+// groups, by exchanging halves (32 lanes) and quarters (16).
+__device__ __forceinline__ void blocks_from_lanes(unsigned w[4]) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const auto r = __builtin_amdgcn_permlane32_swap(w[j], w[j + 2], false, false);
+        w[j] = r[0];
+        w[j + 2] = r[1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+        const auto r = __builtin_amdgcn_permlane16_swap(w[j], w[j + 1], false, false);
+        w[j] = r[0];
+        w[j + 1] = r[1];
+    }
+}
+
+__device__ inline void put(float *o, float v) { *o = v; }
+__device__ inline void put(_Float16 *o, float v) { *o = (_Float16)v; }
+__device__ inline void put(__bf16 *o, float v) { *o = (__bf16)v; }
+
+constexpr int DEPTH = 4;  // chunks of 128 columns requested ahead per wavefront
+
+// WR x WK wavefronts: RT tiles of 16 rows for each of WR, the columns' chunks of
+// 128 dealt out to WK; TT tiles of 16 tokens. The tokens' operands come
+// through LDS, kc columns at a time.
+template <class T, int G, int TT, int RT, int WR, int WK>
+__global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const uint8_t *w,
+                                                     const uint16_t *scales, int rows, int cols,
+                                                     int n, int kc, const uint8_t *ws) {
+    constexpr bool split = sizeof(T) == 4;
+    constexpr int P = split ? 2 : 1, NT = 64 * WR * WK, GC = 128 / G;  // groups of a chunk
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave % WR, wk = wave / WR, g = lane >> 4, lr = lane & 15;
+    const int tg = blockIdx.y, nt = min(TG, n - tg * TG), type = split ? MHIP_F32 : MHIP_F16;
+    const Tokens l = tokens_of(type, cols, n);
+    const uint8_t *xg = ws + (size_t)tg * l.group;
+    const float *fg = (const float *)(xg + l.operands);
+    const int nchunk = (cols + 127) / 128, nblock = cols / 32, ngroup = cols / G;
+    const int row0 = (blockIdx.x * WR + wr) * RT * 16;
+    const uint8_t *wrow[RT];
+    const uint16_t *srow[RT];
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+        const size_t r = min(row0 + i * 16 + lr, rows - 1);
+        wrow[i] = w + r * (cols / 2) + g * 16;
+        srow[i] = scales + r * ngroup;
+    }
+    f4 total[RT][TT];
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int t = 0; t < TT; t++) total[i][t] = (f4){0, 0, 0, 0};
+
+    u4 wq[DEPTH][RT];
+    uint16_t sq[DEPTH][RT][GC];
+    auto request = [&](int d, int chunk) {
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            wq[d][i] = (u4){0, 0, 0, 0};
+            if (chunk * 4 + g < nblock) wq[d][i] = *(const u4 *)(wrow[i] + (size_t)chunk * 64);
+#pragma unroll
+            for (int j = 0; j < GC; j++) {
+                const int q = chunk * GC + j;
+                sq[d][i][j] = q < ngroup ? srow[i][q] : (uint16_t)0;
+            }
+        }
+    };
+    // chunks wk, wk + WK, ... : chunk number c of this wavefront is wk + c * WK
+    const int mine = nchunk > wk ? (nchunk - wk + WK - 1) / WK : 0;
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++)
+        if (d < mine) request(d, wk + d * WK);
+
+    const size_t step = (size_t)P * nt * 64;  // bytes of a block of 32 columns
+    float *fl = (float *)(lds + (size_t)(kc / 32) * step);
+    int k0 = -kc;  // the columns in LDS: k0 .. k0 + kc - 1
+    // The next columns' operands into LDS: every wavefront gets here equally
+    // often, whichever chunk it is at.
+    auto stage = [&]() {
+        k0 += kc;
+        const int kn = min(kc, cols - k0), segs = (kn + SEG - 1) / SEG;
+        __syncthreads();
+        const uint4 *from = (const uint4 *)(xg + (size_t)(k0 / 32) * step);
+        const int units = (int)((size_t)(kn / 32) * step / 16);
+        for (int i = tid; i < units; i += NT) ((uint4 *)lds)[i] = from[i];
+        for (int i = tid; i < segs * TG; i += NT)
+            fl[i] = i % TG < nt ? fg[(size_t)(k0 / SEG) * TG + i] : 0.0f;
+        __syncthreads();
+    };
+    for (int c = 0; c < mine; c += DEPTH) {
+        {
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++) {
+                if (c + d >= mine) break;
+                const int chunk = wk + (c + d) * WK;
+                while (chunk * 128 >= k0 + kc) stage();
+                unsigned q[RT][4];
+                float sc[RT][GC];
+#pragma unroll
+                for (int i = 0; i < RT; i++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) q[i][j] = wq[d][i][j];
+#pragma unroll
+                    for (int j = 0; j < GC; j++)
+                        sc[i][j] = (float)__builtin_bit_cast(_Float16, sq[d][i][j]);
+                    blocks_from_lanes(q[i]);
+                }
+                if (c + d + DEPTH < mine) request(d, chunk + DEPTH * WK);
+                const int b0 = chunk * 4 - k0 / 32;
+                f4 part[RT][TT];
+#pragma unroll
+                for (int i = 0; i < RT; i++)
+#pragma unroll
+                    for (int t = 0; t < TT; t++) part[i][t] = (f4){0, 0, 0, 0};
+                f4 hi[RT][TT], lo[RT][TT];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (chunk * 4 + j < nblock) {
+                        h8 b[RT];
+#pragma unroll
+                        for (int i = 0; i < RT; i++) b[i] = codes(q[i][j]);
+                        const bool begin = j % (G / 32) == 0, end = (j + 1) % (G / 32) == 0;
+#pragma unroll
+                        for (int t = 0; t < TT; t++) {
+                            // (a lane past the last token reads the last one's; its
+                            // results are not stored)
+                            const int tok = min(t * 16 + lr, nt - 1);
+                            const uint8_t *x = lds + (size_t)(b0 + j) * step + tok * 64 + g * 16;
+                            const h8 a = *(const h8 *)x;
+                            h8 a2;
+                            if constexpr (split) a2 = *(const h8 *)(x + (size_t)nt * 64);
+#pragma unroll
+                            for (int i = 0; i < RT; i++) {
+                                const f4 z = {0, 0, 0, 0};
+                                hi[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    a, b[i], begin ? z : hi[i][t], 0, 0, 0);
+                                if constexpr (split)
+                                    lo[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                        a2, b[i], begin ? z : lo[i][t], 0, 0, 0);
+                                if (end) {
+#pragma unroll
+                                    for (int r = 0; r < 4; r++) {
+                                        float v = hi[i][t][r];
+                                        if constexpr (split)
+                                            v = __builtin_fmaf(lo[i][t][r], 0x1p-11f, v);
+                                        part[i][t][r] = __builtin_fmaf(sc[i][j / (G / 32)], v,
+                                                                       part[i][t][r]);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                }
+                // back to x's own scale
+                const float *f = fl + (chunk * 128 - k0) / SEG * TG;
+#pragma unroll
+                for (int t = 0; t < TT; t++) {
+                    const f4 b = *(const f4 *)(f + t * 16 + g * 4);
+#pragma unroll
+                    for (int i = 0; i < RT; i++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            total[i][t][r] = __builtin_fmaf(part[i][t][r], b[r], total[i][t][r]);
+                }
+            }
+        }
+    }
+    while (k0 + kc < cols) stage();  // a wavefront whose chunks ended earlier
+    if constexpr (WK > 1) {
+        // the column shares' sums, added in their order by the first of them
+        __syncthreads();
+        f4 *sum = (f4 *)lds;
+        if (wk > 0) {
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int t = 0; t < TT; t++)
+                    sum[(((wk - 1) * WR + wr) * RT * TT + i * TT + t) * 64 + lane] = total[i][t];
+        }
+        __syncthreads();
+        if (wk > 0) return;
+        for (int k = 0; k < WK - 1; k++)
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int t = 0; t < TT; t++)
+                    total[i][t] += sum[((k * WR + wr) * RT * TT + i * TT + t) * 64 + lane];
+    }
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+        const int row = row0 + i * 16 + lr;
+#pragma unroll
+        for (int t = 0; t < TT; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int tok = t * 16 + g * 4 + r;
+                if (row < rows && tok < nt) put(out + (size_t)(tg * TG + tok) * ldo + row, total[i][t][r]);
+            }
+    }
+}
+
+// One thread a group (weights are quantized once, when a model is loaded).
+__global__ __launch_bounds__(256) void k_quantize_q4(const float *w, size_t groups, int group,
+                                                     uint8_t *codes, uint16_t *scales) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= groups) return;
+    const float *v = w + i * group;
+    float top = 0.0f;
+    for (int j = 0; j < group; j++) top = fmaxf(top, fabsf(v[j]));
+    const _Float16 h = (_Float16)fminf(top / 7.0f, 65504.0f);
+    const float s = (float)h;
+    scales[i] = __builtin_bit_cast(uint16_t, h);
+    unsigned *o = (unsigned *)(codes + i * group / 2);
+    for (int j = 0; j < group; j += 8) {
+        unsigned word = 0;
+        for (int k = 0; k < 8; k++) {
+            const float q = s > 0.0f ? rintf(v[j + k] / s) : 0.0f;
+            word |= ((unsigned)(int)fminf(fmaxf(q, -8.0f), 7.0f) & 15u) << (4 * k);
+        }
+        o[j / 8] = word;
+    }
+}
+
+__global__ __launch_bounds__(256) void k_dequantize_q4(const uint8_t *codes, const uint16_t *scales,
+                                                       size_t n, int group, float *w) {
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= n) return;
+    const float s = (float)__builtin_bit_cast(_Float16, scales[i / group]);
+    const unsigned word = *(const unsigned *)(codes + i / 2);
+    for (int k = 0; k < 8; k++) w[i + k] = s * (float)((int)(word << (28 - 4 * k)) >> 28);
+}
+
+int check_q4(mhip_ctx *c, const char *what, const void *d_codes, const void *d_scales, int rows,
+             int cols, int group) {
+    if (rows < 0 || cols < 0 || (group != 32 && group != 64 && group != 128) || cols % group)
+        return mhip::fail(c, "%s: %d rows of %d in groups of %d (32, 64 or 128, dividing the row)",
+                          what, rows, cols, group);
+    if (rows && cols && (!d_codes || !d_scales)) return mhip::fail(c, "%s: a null argument", what);
+    if ((uintptr_t)d_codes % 16 || (uintptr_t)d_scales % 2)
+        return mhip::fail(c, "%s: the codes must be 16-byte aligned", what);
+    return 0;
+}
+
+// One shape of the kernel.
+template <class T, int G, int TT, int RT, int WR, int WK>
+int launch(mhip_ctx *c, T *out, int ldo, const void *w, const void *s, int rows, int cols, int n,
+           const void *ws) {
+    constexpr int P = sizeof(T) == 4 ? 2 : 1;
+    const int nt = n < TG ? n : TG;
+    // columns per LDS stage: whole segments, or a half, a quarter, an eighth of
+    // one; up to 48 KB, more where that is less than a chunk per column share
+    int kc = SEG;
+    if ((size_t)kc * P * nt * 2 <= 48 * 1024)
+        kc = 48 * 1024 / (P * nt * 2) / SEG * SEG;
+    else
+        while ((size_t)kc * P * nt * 2 > 128 * 1024) kc /= 2;
+    if (kc > cols) kc = (cols + 127) / 128 * 128;
+    size_t lds = (size_t)kc * P * nt * 2 + (size_t)((kc + SEG - 1) / SEG) * TG * 4;
+    const size_t join = (size_t)(WK - 1) * WR * RT * TT * 1024;
+    if (lds < join) lds = join;
+    auto k = k_q4<T, G, TT, RT, WR, WK>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 160 * 1024);
+        if (mhip::check(c, e, "matvec_q4 LDS attribute")) return -1;
+    }
+    const dim3 grid((rows + RT * WR * 16 - 1) / (RT * WR * 16), (n + TG - 1) / TG);
+    k<<<grid, 64 * WR * WK, lds, c->stream>>>(out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows,
+                                              cols, n, kc, (const uint8_t *)ws);
+    return mhip::check_launch(c, "matvec_q4");
+}
+
+template <class T, int G>
+int choose(mhip_ctx *c, T *out, int ldo, const void *w, const void *s, int rows, int cols, int n,
+           const void *ws) {
+    const bool many = rows >= 32768;
+    if (n > 32)
+        return many ? launch<T, G, 4, 1, 4, 2>(c, out, ldo, w, s, rows, cols, n, ws)
+                    : launch<T, G, 4, 1, 1, 8>(c, out, ldo, w, s, rows, cols, n, ws);
+    if (n > 16)
+        return many ? launch<T, G, 2, 1, 4, 2>(c, out, ldo, w, s, rows, cols, n, ws)
+                    : launch<T, G, 2, 1, 1, 8>(c, out, ldo, w, s, rows, cols, n, ws);
+    return many ? launch<T, G, 1, 2, 4, 1>(c, out, ldo, w, s, rows, cols, n, ws)
+                : launch<T, G, 1, 1, 1, 8>(c, out, ldo, w, s, rows, cols, n, ws);
+}
+
+template <class T>
+int run(mhip_ctx *c, int type, void *out, int ldo, const void *w, const void *s, int group,
+        const void *x, int ldx, int rows, int cols, int n, void *ws) {
+    k_q4_tokens<T><<<dim3(n, (cols + SEG - 1) / SEG), 256, 0, c->stream>>>(
+        (const T *)x, ldx, cols, n, type, (uint8_t *)ws);
+    if (group == 32) return choose<T, 32>(c, (T *)out, ldo, w, s, rows, cols, n, ws);
+    if (group == 64) return choose<T, 64>(c, (T *)out, ldo, w, s, rows, cols, n, ws);
+    return choose<T, 128>(c, (T *)out, ldo, w, s, rows, cols, n, ws);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mhip_quantize_q4(mhip_ctx *c, const float *d_w, int rows, int cols, int group, void *d_codes,
+                     void *d_scales) {
+    if (check_q4(c, "quantize_q4", d_codes, d_scales, rows, cols, group)) return -1;
+    if (!rows || !cols) return 0;
+    if (!d_w) return mhip::fail(c, "quantize_q4: a null argument");
+    if (mhip::use_device(c)) return -1;
+    const size_t groups = (size_t)rows * (cols / group);
+    k_quantize_q4<<<mhip::blocks_for(groups, 256), 256, 0, c->stream>>>(
+        d_w, groups, group, (uint8_t *)d_codes, (uint16_t *)d_scales);
+    return mhip::check_launch(c, "quantize_q4");
+}
+
+int mhip_dequantize_q4(mhip_ctx *c, const void *d_codes, const void *d_scales, int rows, int cols,
+                       int group, float *d_w) {
+    if (check_q4(c, "dequantize_q4", d_codes, d_scales, rows, cols, group)) return -1;
+    if (!rows || !cols) return 0;
+    if (!d_w) return mhip::fail(c, "dequantize_q4: a null argument");
+    if (mhip::use_device(c)) return -1;
+    const size_t n = (size_t)rows * cols;
+    k_dequantize_q4<<<mhip::blocks_for(n / 8, 256), 256, 0, c->stream>>>(
+        (const uint8_t *)d_codes, (const uint16_t *)d_scales, n, group, d_w);
+    return mhip::check_launch(c, "dequantize_q4");
+}
+
+size_t mhip_matvec_q4_ws_bytes(int type, int cols, int n) {
+    if (type < MHIP_F32 || type > MHIP_BF16 || cols <= 0 || cols % 32 || n <= 0) return 0;
+    return tokens_of(type, cols, n).group * (size_t)((n + TG - 1) / TG);
+}
+
+int mhip_matvec_q4(mhip_ctx *c, int type, void *d_out, int ldo, const void *d_codes,
+                   const void *d_scales, int group, const void *d_x, int ldx, int rows, int cols,
+                   int n, void *d_ws) {
+    if (check_q4(c, "matvec_q4", d_codes, d_scales, rows, cols, group)) return -1;
+    if (type < MHIP_F32 || type > MHIP_BF16) return mhip::fail(c, "matvec_q4: type %d", type);
+    if (n < 0 || ldx < cols || ldo < rows)
+        return mhip::fail(c, "matvec_q4: %d tokens, rows %d and %d apart (%d columns, %d rows)", n,
+                          ldx, ldo, cols, rows);
+    if (!n || !rows) return 0;
+    if (!cols) return mhip::fail(c, "matvec_q4: no columns");
+    if (!d_out || !d_x || !d_ws) return mhip::fail(c, "matvec_q4: a null argument");
+    const int esz = mhip::type_bytes(type);
+    if ((uintptr_t)d_x % 16 || (size_t)ldx * esz % 16 || (uintptr_t)d_out % esz ||
+        (uintptr_t)d_ws % 256)
+        return mhip::fail(c, "matvec_q4: x rows must start on 16 bytes, the workspace on 256");
+    if (n > 65535 * TG || (cols + SEG - 1) / SEG > 65535)
+        return mhip::fail(c, "matvec_q4: %d tokens of %d columns in one call", n, cols);
+    if (mhip::use_device(c)) return -1;
+    if (type == MHIP_F32)
+        return run<float>(c, type, d_out, ldo, d_codes, d_scales, group, d_x, ldx, rows, cols, n, d_ws);
+    if (type == MHIP_F16)
+        return run<_Float16>(c, type, d_out, ldo, d_codes, d_scales, group, d_x, ldx, rows, cols, n, d_ws);
+    return run<__bf16>(c, type, d_out, ldo, d_codes, d_scales, group, d_x, ldx, rows, cols, n, d_ws);
+}
+
+}  // extern "C"
