@@ -541,8 +541,8 @@ int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * Row i * max_count + j of d_q ([n_heads][head_dim] values of the cache's
  * type, rows ldq values apart) is token j of slot d_seqs[i], at position
  * t = len - d_count[i] + j (d_count NULL: max_count each); it attends to its
- * slot's positions 0 .. t: softmax(scale q.k) v per query head, n_heads a
- * multiple of n_kv_heads. Rows past d_count[i], and rows of an empty slot, are
+ * slot's positions 0 .. t: softmax(scale q.k) v per query head (scale > 0),
+ * n_heads a multiple of n_kv_heads. Rows past d_count[i], and rows of an empty slot, are
  * zeros in d_out (rows ldo values apart).
  *
  * The slots may share their first `prefix` tokens (0: they do not): those

@@ -19,8 +19,8 @@ Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int 
     Cut k;
     const int group = n_heads / s->n_kv_heads;
     const long long rows = (long long)n * mc * group;
-    k.wr = rows > 32 ? 4 : rows > 16 ? 2 : 1;
-    k.rt = rows > 64 && s->head_dim <= 128 ? 2 : 1;
+    k.wr = prefix == 0 ? 1 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
+    k.rt = prefix > 0 && rows > 64 && s->head_dim <= 128 ? 2 : 1;
     const int tile = k.wr * k.rt * 16;
     k.ptiles = prefix > 0 ? (int)((rows + tile - 1) / tile) : 0;
     k.sp = 0;
@@ -77,6 +77,8 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
     const int esz = mhip::type_bytes(s->type);
     if (ldq < n_heads * s->head_dim || ldo < n_heads * s->head_dim)
         return mhip::fail(c, "%s: rows %d and %d apart (width %d)", what, ldq, ldo, n_heads * s->head_dim);
+    if (!(scale > 0.0f) || !(scale * 1.44269504f < __builtin_inff()))
+        return mhip::fail(c, "%s: scale %g is not a positive number", what, scale);
     if (!d_q || !d_out || !d_seqs || !d_ws) return mhip::fail(c, "%s: a null argument", what);
     if (((uintptr_t)d_q | (uintptr_t)d_out) % 16 || (size_t)ldq * esz % 16 || (size_t)ldo * esz % 16 ||
         (uintptr_t)d_ws % 256)

@@ -85,7 +85,8 @@ def test_attention():
     for bad in (dict(layer=-1), dict(layer=2), dict(heads=0), dict(heads=3), dict(q=None), dict(q=4104),
                 dict(ldq=255), dict(ldq=260), dict(out=None), dict(out=4098), dict(ldo=240), dict(seqs=None),
                 dict(n=-1), dict(n=5), dict(top=-2), dict(prefix=-1), dict(prefix=65), dict(prefix_seq=-1),
-                dict(prefix_seq=4), dict(max_len=81), dict(max_len=-1), dict(ws=None), dict(ws=4096 + 128)):
+                dict(prefix_seq=4), dict(max_len=81), dict(max_len=-1), dict(scale=0.0), dict(scale=-1.0),
+                dict(scale=float("nan")), dict(scale=float("inf")), dict(ws=None), dict(ws=4096 + 128)):
         assert L.mhip_attention_shared(None, D, A, *dict(good, **bad).values()) == -1, bad
     for none in (dict(n=0), dict(top=0)):
         assert L.mhip_attention_shared(None, D, A, *dict(good, **none).values()) == 0
