@@ -26,14 +26,14 @@ struct Job {
     float c;                       // scale * log2(e)
     int lp;                        // log2(page)
     int sp, plen, ptiles;          // prefix parts, positions of each, row tiles
-    int ss, stiles;                // parts behind the prefix, row tiles of a slot
+    int ss, slen, stiles;          // parts behind the prefix, positions of each, row tiles of a slot
     float *o, *ml;                 // partial results [part][row][hd], [part][row][2]
 };
 
 // How a call is cut: rows of a prefix tile (wr * rt tiles of 16), parts of the
 // prefix and of the slots.
 struct Cut {
-    int wr, rt, ptiles, sp, plen, ss, stiles;
+    int wr, rt, ptiles, sp, plen, ss, slen, stiles;
 };
 
 int launch_f32(mhip_ctx *c, const Job &a, const Cut &k);

@@ -12,34 +12,48 @@ using mhip_shared::TILE;
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// How a call is cut. Every workgroup of the prefix reads its part for up to 128 rows, and
-// there should be one for every CU; a part of a slot is at least 256
-// positions while there are two workgroups per CU.
+// How a call is cut. A part of the prefix serves up to 128 rows; tiles of 64
+// rows do better up to 128 rows in all (16 slots behind 16000 tokens, bf16: 28 us,
+// with tiles of 128 rows 32; 64 slots behind 8000: 35 and 33). Every part's
+// results pass through memory once more, so there are only as many as
+// keep the CUs busy: 256 workgroups for the prefix (64 x 8000: with 8 parts 41
+// us, 16 parts 33, 32 parts 41) and 256 for the slots (32 unshared slots of up
+// to 8000 tokens: 2 parts 79 us, 8 parts 90; 64 of 300 tokens: 1 part 12 us, 2
+// parts 18). Where a CU holds one workgroup only (tiles of 128 KB: fp32 heads of
+// 128, or heads of 256) the two together should not be more than the CUs.
 Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int max_len) {
     Cut k;
-    const int group = n_heads / s->n_kv_heads;
+    const int group = n_heads / s->n_kv_heads, rest = max_len - prefix;
     const long long rows = (long long)n * mc * group;
+    k.stiles = (mc * group + 15) / 16;
+    const long long items = (long long)n * s->n_kv_heads * k.stiles;
+    long long parts = 256 / items;
+    const int most = (rest + 255) / 256, least = (rest + PART_MAX - 1) / PART_MAX;
+    if (parts > most) parts = most;
+    if (parts < least) parts = least;
+    if (parts < 1) parts = 1;
+    k.slen = rest > 0 ? (int)((rest + parts - 1) / parts + TILE - 1) / TILE * TILE : TILE;
+    k.ss = rest > 0 ? (rest + k.slen - 1) / k.slen : 1;
+
     k.wr = prefix == 0 ? 1 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
-    k.rt = prefix > 0 && rows > 64 && s->head_dim <= 128 ? 2 : 1;
+    k.rt = prefix > 0 && rows > 128 && s->head_dim <= 128 ? 2 : 1;
     const int tile = k.wr * k.rt * 16;
     k.ptiles = prefix > 0 ? (int)((rows + tile - 1) / tile) : 0;
     k.sp = 0;
     k.plen = 0;
     if (prefix > 0) {
-        long long parts = 256 / ((long long)k.ptiles * s->n_kv_heads);
-        const int most = (prefix + 127) / 128, least = (prefix + PART_MAX - 1) / PART_MAX;
-        if (parts > most) parts = most;
-        if (parts < least) parts = least;
-        k.plen = (int)((prefix + parts - 1) / parts + TILE - 1) / TILE * TILE;
+        const int padded = s->head_dim <= 64 ? 64 : s->head_dim <= 128 ? 128 : 256;
+        const long long slots = padded * mhip::type_bytes(s->type) > 256 ? 256 : 512;
+        long long wgs = slots - items * k.ss;
+        if (wgs > 256) wgs = 256;
+        if (wgs < 128) wgs = 128;
+        long long pp = wgs / ((long long)k.ptiles * s->n_kv_heads);
+        const int pmost = (prefix + 127) / 128, pleast = (prefix + PART_MAX - 1) / PART_MAX;
+        if (pp > pmost) pp = pmost;
+        if (pp < pleast) pp = pleast;
+        k.plen = (int)((prefix + pp - 1) / pp + TILE - 1) / TILE * TILE;
         k.sp = (prefix + k.plen - 1) / k.plen;
     }
-    const int rest = max_len - prefix;
-    k.stiles = (mc * group + 15) / 16;
-    long long parts = 512 / ((long long)n * s->n_kv_heads * k.stiles) + 1;
-    const int most = (rest + 255) / 256, least = (rest + PART_MAX - 1) / PART_MAX;
-    if (parts > most) parts = most;
-    if (parts < least) parts = least;
-    k.ss = parts < 1 ? 1 : (int)parts;
     return k;
 }
 
@@ -108,6 +122,7 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
     a.plen = k.plen;
     a.ptiles = k.ptiles;
     a.ss = k.ss;
+    a.slen = k.slen;
     a.stiles = k.stiles;
     const size_t rows = (size_t)n * max_count * n_heads, parts = (size_t)k.sp + k.ss;
     a.o = (float *)d_ws;
