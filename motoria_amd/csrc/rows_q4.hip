@@ -49,6 +49,21 @@ __device__ inline float value(float x) { return x; }
 __device__ inline float value(_Float16 x) { return (float)x; }
 __device__ inline float value(__bf16 x) { return (float)x; }
 
+// 2^(14 - exponent of the largest magnitude m of a segment); values below
+// 2^-112 keep the factor 2^126.
+__device__ __forceinline__ float segment_scale(float m) {
+    return ldexpf(1.0f, min(126, 14 - (m > 0.0f ? ilogbf(m) : 14)));
+}
+__device__ __forceinline__ float finite_max(float m, float v) {
+    const float a = fabsf(v);
+    return a < __builtin_inff() && a > m ? a : m;
+}
+// hi and lo of a scaled value (an infinity or NaN is in hi alone)
+__device__ __forceinline__ _Float16 lo_of(float s, _Float16 hi) {
+    const float rest = (s - (float)hi) * 2048.0f;
+    return fabsf(rest) < __builtin_inff() ? (_Float16)rest : (_Float16)0.0f;
+}
+
 // One workgroup a token and segment, four columns a thread.
 template <class T>
 __global__ __launch_bounds__(256) void k_q4_tokens(const T *x, int ldx, int cols, int n, int type,
@@ -69,19 +84,13 @@ __global__ __launch_bounds__(256) void k_q4_tokens(const T *x, int ldx, int cols
     }
     float scale = 1.0f;
     if (type != MHIP_F16) {
-        float m = 0.0f;  // the largest finite magnitude
+        float m = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float a = fabsf(v[j]);
-            m = a < __builtin_inff() && a > m ? a : m;
-        }
+        for (int j = 0; j < 4; j++) m = finite_max(m, v[j]);
         for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
         if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
         __syncthreads();
-        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        // 2^(14 - exponent of m); values below 2^-112 keep the factor 2^126
-        const int e = m > 0.0f ? ilogbf(m) : 14;
-        scale = ldexpf(1.0f, min(126, 14 - e));
+        scale = segment_scale(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
     }
     if (threadIdx.x == 0)
         ((float *)(base + l.operands))[(size_t)seg * TG + t % TG] = 1.0f / scale;  // exact: a power of two
@@ -96,11 +105,7 @@ __global__ __launch_bounds__(256) void k_q4_tokens(const T *x, int ldx, int cols
         const float s = v[j] * scale;
         const _Float16 hi = (_Float16)s;
         o[2 * j] = hi;
-        if constexpr (split) {
-            // an infinity or NaN is in hi alone
-            const float rest = (s - (float)hi) * 2048.0f;
-            o[(size_t)nt * 32 + 2 * j] = fabsf(rest) < __builtin_inff() ? (_Float16)rest : (_Float16)0.0f;
-        }
+        if constexpr (split) o[(size_t)nt * 32 + 2 * j] = lo_of(s, hi);
     }
 }
 
@@ -138,26 +143,31 @@ __device__ inline void put(float *o, float v) { *o = v; }
 __device__ inline void put(_Float16 *o, float v) { *o = (_Float16)v; }
 __device__ inline void put(__bf16 *o, float v) { *o = (__bf16)v; }
 
-constexpr int DEPTH = 4;  // chunks of 128 columns requested ahead per wavefront
+constexpr int DEPTH = 4;       // chunks of 128 columns requested ahead per wavefront
+constexpr int FEW = 8;         // tokens whose operands a workgroup forms itself
+constexpr int FEW_LDS = 65536; // bytes of LDS for them
 
 // WR x WK wavefronts: RT tiles of 16 rows for each of WR, the columns' chunks of
 // 128 dealt out to WK; TT tiles of 16 tokens. The tokens' operands come
-// through LDS, kc columns at a time.
-template <class T, int G, int TT, int RT, int WR, int WK>
+// through LDS, kc columns at a time, from the workspace; with N > 0 (1: one token,
+// 8: up to FEW) the workgroup forms them from x itself, which saves a launch, and for fp32
+// x hi and lo of a token are two of the instruction's sixteen token rows.
+template <class T, int G, int N, int TT, int RT, int WR, int WK>
 __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const uint8_t *w,
                                                      const uint16_t *scales, int rows, int cols,
-                                                     int n, int kc, const uint8_t *ws) {
-    constexpr bool split = sizeof(T) == 4;
+                                                     int n, int kc, const uint8_t *ws, const T *x,
+                                                     size_t ldx, int type) {
+    constexpr bool split = sizeof(T) == 4, pair = split && N > 0;
     constexpr int P = split ? 2 : 1, NT = 64 * WR * WK, GC = 128 / G;  // groups of a chunk
+    constexpr int TL = N == 1 ? 1 : pair ? 2 : 4;                      // tokens of a lane and tile
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR, g = lane >> 4, lr = lane & 15;
-    const int tg = blockIdx.y, nt = min(TG, n - tg * TG), type = split ? MHIP_F32 : MHIP_F16;
-    const Tokens l = tokens_of(type, cols, n);
-    const uint8_t *xg = ws + (size_t)tg * l.group;
-    const float *fg = (const float *)(xg + l.operands);
+    const int tg = blockIdx.y, nt = min(TG, n - tg * TG);
     const int nchunk = (cols + 127) / 128, nblock = cols / 32, ngroup = cols / G;
     const int row0 = (blockIdx.x * WR + wr) * RT * 16;
+    // a chunk's scales in one load, where every row's stand on its boundary
+    const bool whole = GC == 1 || (ngroup % GC == 0 && (uintptr_t)scales % (2 * GC) == 0);
     const uint8_t *wrow[RT];
     const uint16_t *srow[RT];
 #pragma unroll
@@ -166,11 +176,13 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
         wrow[i] = w + r * (cols / 2) + g * 16;
         srow[i] = scales + r * ngroup;
     }
-    f4 total[RT][TT];
+    float total[RT][TT][TL];
 #pragma unroll
     for (int i = 0; i < RT; i++)
 #pragma unroll
-        for (int t = 0; t < TT; t++) total[i][t] = (f4){0, 0, 0, 0};
+        for (int t = 0; t < TT; t++)
+#pragma unroll
+            for (int r = 0; r < TL; r++) total[i][t][r] = 0.0f;
 
     u4 wq[DEPTH][RT];
     uint16_t sq[DEPTH][RT][GC];
@@ -179,10 +191,17 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
         for (int i = 0; i < RT; i++) {
             wq[d][i] = (u4){0, 0, 0, 0};
             if (chunk * 4 + g < nblock) wq[d][i] = *(const u4 *)(wrow[i] + (size_t)chunk * 64);
+            if (whole) {
+                const uint16_t *at = srow[i] + chunk * GC;
+                if constexpr (GC == 4) *(uint2 *)sq[d][i] = *(const uint2 *)at;
+                else if constexpr (GC == 2) *(unsigned *)sq[d][i] = *(const unsigned *)at;
+                else sq[d][i][0] = at[0];
+            } else {
 #pragma unroll
-            for (int j = 0; j < GC; j++) {
-                const int q = chunk * GC + j;
-                sq[d][i][j] = q < ngroup ? srow[i][q] : (uint16_t)0;
+                for (int j = 0; j < GC; j++) {
+                    const int q = chunk * GC + j;
+                    sq[d][i][j] = q < ngroup ? srow[i][q] : (uint16_t)0;
+                }
             }
         }
     };
@@ -199,104 +218,164 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
     // often, whichever chunk it is at.
     auto stage = [&]() {
         k0 += kc;
-        const int kn = min(kc, cols - k0), segs = (kn + SEG - 1) / SEG;
-        __syncthreads();
-        const uint4 *from = (const uint4 *)(xg + (size_t)(k0 / 32) * step);
-        const int units = (int)((size_t)(kn / 32) * step / 16);
-        for (int i = tid; i < units; i += NT) ((uint4 *)lds)[i] = from[i];
-        for (int i = tid; i < segs * TG; i += NT)
-            fl[i] = i % TG < nt ? fg[(size_t)(k0 / SEG) * TG + i] : 0.0f;
-        __syncthreads();
-    };
-    for (int c = 0; c < mine; c += DEPTH) {
-        {
+        if constexpr (N > 0) {
+            // a wavefront per token and segment, 16 columns a lane
+            const int segs = (cols + SEG - 1) / SEG;
+            for (int i = wave; i < n * segs; i += WR * WK) {
+                const int t = i % n, seg = i / n;
+                float v[2][8];
+                float m = 0.0f;
 #pragma unroll
-            for (int d = 0; d < DEPTH; d++) {
-                if (c + d >= mine) break;
-                const int chunk = wk + (c + d) * WK;
-                while (chunk * 128 >= k0 + kc) stage();
-                unsigned q[RT][4];
-                float sc[RT][GC];
+                for (int h = 0; h < 2; h++) {
+                    const int c = seg * SEG + h * 512 + lane * 8;
+                    T r[8] = {};
+                    if (c < cols) {
+                        const T *at = x + (size_t)t * ldx + c;
+                        *(uint4 *)r = *(const uint4 *)at;
+                        if constexpr (split) *(uint4 *)(r + 4) = *(const uint4 *)(at + 4);
+                    }
 #pragma unroll
-                for (int i = 0; i < RT; i++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) q[i][j] = wq[d][i][j];
-#pragma unroll
-                    for (int j = 0; j < GC; j++)
-                        sc[i][j] = (float)__builtin_bit_cast(_Float16, sq[d][i][j]);
-                    blocks_from_lanes(q[i]);
+                    for (int j = 0; j < 8; j++) {
+                        v[h][j] = value(r[j]);
+                        m = finite_max(m, v[h][j]);
+                    }
                 }
-                if (c + d + DEPTH < mine) request(d, chunk + DEPTH * WK);
-                const int b0 = chunk * 4 - k0 / 32;
-                f4 part[RT][TT];
+                float scale = 1.0f;
+                if (type != MHIP_F16) {
+                    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+                    scale = segment_scale(m);
+                }
+                if (lane == 0) fl[seg * TG + t] = 1.0f / scale;
 #pragma unroll
-                for (int i = 0; i < RT; i++)
+                for (int h = 0; h < 2; h++) {
+                    const int c = seg * SEG + h * 512 + lane * 8;
+                    if (c >= cols) continue;
+                    _Float16 *o = (_Float16 *)(lds + (size_t)(c / 32) * step) + t * 32 + c % 32;
+                    h8 hi, lo;
 #pragma unroll
-                    for (int t = 0; t < TT; t++) part[i][t] = (f4){0, 0, 0, 0};
-                f4 hi[RT][TT], lo[RT][TT];
+                    for (int j = 0; j < 8; j++) {
+                        const int to = j < 4 ? 2 * j : 2 * j - 7;  // column j next to j + 4
+                        hi[to] = (_Float16)(v[h][j] * scale);
+                        if constexpr (split) lo[to] = lo_of(v[h][j] * scale, hi[to]);
+                    }
+                    *(h8 *)o = hi;
+                    if constexpr (split) *(h8 *)(o + n * 32) = lo;
+                }
+            }
+            __syncthreads();
+        } else {
+            const Tokens l = tokens_of(split ? MHIP_F32 : MHIP_F16, cols, n);
+            const uint8_t *xg = ws + (size_t)tg * l.group;
+            const float *fg = (const float *)(xg + l.operands);
+            const int kn = min(kc, cols - k0), segs = (kn + SEG - 1) / SEG;
+            __syncthreads();
+            const uint4 *from = (const uint4 *)(xg + (size_t)(k0 / 32) * step);
+            const int units = (int)((size_t)(kn / 32) * step / 16);
+            for (int i = tid; i < units; i += NT) ((uint4 *)lds)[i] = from[i];
+            for (int i = tid; i < segs * TG; i += NT)
+                fl[i] = i % TG < nt ? fg[(size_t)(k0 / SEG) * TG + i] : 0.0f;
+            __syncthreads();
+        }
+    };
+    // a lane's token rows of the operands (past the last token: the last one's,
+    // whose results are not stored), and its own tokens
+    int from[TT], own[TT][TL];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (chunk * 4 + j < nblock) {
-                        h8 b[RT];
+    for (int t = 0; t < TT; t++) {
+        from[t] = pair ? (min(lr >> 1, nt - 1) + (lr & 1) * nt) * 64 + g * 16
+                       : min(t * 16 + lr, nt - 1) * 64 + g * 16;
 #pragma unroll
-                        for (int i = 0; i < RT; i++) b[i] = codes(q[i][j]);
-                        const bool begin = j % (G / 32) == 0, end = (j + 1) % (G / 32) == 0;
+        for (int r = 0; r < TL; r++) own[t][r] = pair ? 2 * g + r : t * 16 + 4 * g + r;
+    }
+    for (int c = 0; c < mine; c += DEPTH) {
 #pragma unroll
-                        for (int t = 0; t < TT; t++) {
-                            // (a lane past the last token reads the last one's; its
-                            // results are not stored)
-                            const int tok = min(t * 16 + lr, nt - 1);
-                            const uint8_t *x = lds + (size_t)(b0 + j) * step + tok * 64 + g * 16;
-                            const h8 a = *(const h8 *)x;
-                            h8 a2;
-                            if constexpr (split) a2 = *(const h8 *)(x + (size_t)nt * 64);
+        for (int d = 0; d < DEPTH; d++) {
+            if (c + d >= mine) break;
+            const int chunk = wk + (c + d) * WK;
+            while (chunk * 128 >= k0 + kc) stage();
+            unsigned q[RT][4];
+            float sc[RT][GC];
 #pragma unroll
-                            for (int i = 0; i < RT; i++) {
-                                const f4 z = {0, 0, 0, 0};
-                                hi[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    a, b[i], begin ? z : hi[i][t], 0, 0, 0);
-                                if constexpr (split)
-                                    lo[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                        a2, b[i], begin ? z : lo[i][t], 0, 0, 0);
-                                if (end) {
+            for (int i = 0; i < RT; i++) {
 #pragma unroll
-                                    for (int r = 0; r < 4; r++) {
-                                        float v = hi[i][t][r];
-                                        if constexpr (split)
-                                            v = __builtin_fmaf(lo[i][t][r], 0x1p-11f, v);
-                                        part[i][t][r] = __builtin_fmaf(sc[i][j / (G / 32)], v,
-                                                                       part[i][t][r]);
-                                    }
+                for (int j = 0; j < 4; j++) q[i][j] = wq[d][i][j];
+#pragma unroll
+                for (int j = 0; j < GC; j++)
+                    sc[i][j] = (float)__builtin_bit_cast(_Float16, sq[d][i][j]);
+                blocks_from_lanes(q[i]);
+            }
+            if (c + d + DEPTH < mine) request(d, chunk + DEPTH * WK);
+            const int b0 = chunk * 4 - k0 / 32;
+            float part[RT][TT][TL];
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int t = 0; t < TT; t++)
+#pragma unroll
+                    for (int r = 0; r < TL; r++) part[i][t][r] = 0.0f;
+            f4 hi[RT][TT], lo[RT][TT];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (chunk * 4 + j < nblock) {
+                    h8 b[RT];
+#pragma unroll
+                    for (int i = 0; i < RT; i++) b[i] = codes(q[i][j]);
+                    const bool begin = j % (G / 32) == 0, end = (j + 1) % (G / 32) == 0;
+#pragma unroll
+                    for (int t = 0; t < TT; t++) {
+                        const uint8_t *at = lds + (size_t)(b0 + j) * step + from[t];
+                        const h8 a = *(const h8 *)at;
+                        h8 a2;
+                        if constexpr (split && !pair) a2 = *(const h8 *)(at + (size_t)nt * 64);
+#pragma unroll
+                        for (int i = 0; i < RT; i++) {
+                            const f4 z = {0, 0, 0, 0};
+                            hi[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                a, b[i], begin ? z : hi[i][t], 0, 0, 0);
+                            if constexpr (split && !pair)
+                                lo[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    a2, b[i], begin ? z : lo[i][t], 0, 0, 0);
+                            if (end) {
+#pragma unroll
+                                for (int r = 0; r < TL; r++) {
+                                    float v = pair ? __builtin_fmaf(hi[i][t][2 * r + 1 & 3], 0x1p-11f,
+                                                                    hi[i][t][2 * r & 3])
+                                                   : hi[i][t][r];
+                                    if constexpr (split && !pair)
+                                        v = __builtin_fmaf(lo[i][t][r], 0x1p-11f, v);
+                                    part[i][t][r] = __builtin_fmaf(sc[i][j / (G / 32)], v, part[i][t][r]);
                                 }
                             }
                         }
                     }
                 }
-                // back to x's own scale
-                const float *f = fl + (chunk * 128 - k0) / SEG * TG;
+            }
+            // back to x's own scale
+            const float *f = fl + (chunk * 128 - k0) / SEG * TG;
 #pragma unroll
-                for (int t = 0; t < TT; t++) {
-                    const f4 b = *(const f4 *)(f + t * 16 + g * 4);
+            for (int t = 0; t < TT; t++)
+#pragma unroll
+                for (int r = 0; r < TL; r++) {
+                    const float back = f[N > 0 ? min(own[t][r], nt - 1) : own[t][r]];
 #pragma unroll
                     for (int i = 0; i < RT; i++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            total[i][t][r] = __builtin_fmaf(part[i][t][r], b[r], total[i][t][r]);
+                        total[i][t][r] = __builtin_fmaf(part[i][t][r], back, total[i][t][r]);
                 }
-            }
         }
     }
     while (k0 + kc < cols) stage();  // a wavefront whose chunks ended earlier
     if constexpr (WK > 1) {
         // the column shares' sums, added in their order by the first of them
         __syncthreads();
-        f4 *sum = (f4 *)lds;
+        float *sum = (float *)lds;
         if (wk > 0) {
 #pragma unroll
             for (int i = 0; i < RT; i++)
 #pragma unroll
                 for (int t = 0; t < TT; t++)
-                    sum[(((wk - 1) * WR + wr) * RT * TT + i * TT + t) * 64 + lane] = total[i][t];
+#pragma unroll
+                    for (int r = 0; r < TL; r++)
+                        sum[((((wk - 1) * WR + wr) * RT + i) * TT * TL + t * TL + r) * 64 + lane] = total[i][t][r];
         }
         __syncthreads();
         if (wk > 0) return;
@@ -305,7 +384,9 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
             for (int i = 0; i < RT; i++)
 #pragma unroll
                 for (int t = 0; t < TT; t++)
-                    total[i][t] += sum[((k * WR + wr) * RT * TT + i * TT + t) * 64 + lane];
+#pragma unroll
+                    for (int r = 0; r < TL; r++)
+                        total[i][t][r] += sum[(((k * WR + wr) * RT + i) * TT * TL + t * TL + r) * 64 + lane];
     }
 #pragma unroll
     for (int i = 0; i < RT; i++) {
@@ -313,10 +394,9 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
 #pragma unroll
         for (int t = 0; t < TT; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int tok = t * 16 + g * 4 + r;
-                if (row < rows && tok < nt) put(out + (size_t)(tg * TG + tok) * ldo + row, total[i][t][r]);
-            }
+            for (int r = 0; r < TL; r++)
+                if (row < rows && own[t][r] < nt)
+                    put(out + (size_t)(tg * TG + own[t][r]) * ldo + row, total[i][t][r]);
     }
 }
 
@@ -363,23 +443,24 @@ int check_q4(mhip_ctx *c, const char *what, const void *d_codes, const void *d_s
 }
 
 // One shape of the kernel.
-template <class T, int G, int TT, int RT, int WR, int WK>
-int launch(mhip_ctx *c, T *out, int ldo, const void *w, const void *s, int rows, int cols, int n,
-           const void *ws) {
+template <class T, int G, int N, int TT, int RT, int WR, int WK>
+int launch(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
+           int n, const void *ws, const T *x, int ldx) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
     const int nt = n < TG ? n : TG;
-    // columns per LDS stage: whole segments, or a half, a quarter, an eighth of
-    // one; up to 48 KB, more where that is less than a chunk per column share
+    // columns per LDS stage: all of them for operands formed in place; else
+    // whole segments, or a half, a quarter, an eighth of one, up to 48 KB, more
+    // where that is less than a chunk per column share
     int kc = SEG;
     if ((size_t)kc * P * nt * 2 <= 48 * 1024)
         kc = 48 * 1024 / (P * nt * 2) / SEG * SEG;
     else
         while ((size_t)kc * P * nt * 2 > 128 * 1024) kc /= 2;
-    if (kc > cols) kc = (cols + 127) / 128 * 128;
+    if (kc > cols || N > 0) kc = (cols + 127) / 128 * 128;
     size_t lds = (size_t)kc * P * nt * 2 + (size_t)((kc + SEG - 1) / SEG) * TG * 4;
     const size_t join = (size_t)(WK - 1) * WR * RT * TT * 1024;
     if (lds < join) lds = join;
-    auto k = k_q4<T, G, TT, RT, WR, WK>;
+    auto k = k_q4<T, G, N, TT, RT, WR, WK>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                  160 * 1024);
@@ -387,32 +468,44 @@ int launch(mhip_ctx *c, T *out, int ldo, const void *w, const void *s, int rows,
     }
     const dim3 grid((rows + RT * WR * 16 - 1) / (RT * WR * 16), (n + TG - 1) / TG);
     k<<<grid, 64 * WR * WK, lds, c->stream>>>(out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows,
-                                              cols, n, kc, (const uint8_t *)ws);
+                                              cols, n, kc, (const uint8_t *)ws, x, ldx, type);
     return mhip::check_launch(c, "matvec_q4");
 }
 
+template <class T, int G, int N, int TT>
+int by_rows(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
+            int n, const void *ws, const T *x, int ldx) {
+    if (rows >= 32768) {
+        if constexpr (TT == 1)
+            return launch<T, G, N, 1, 2, 4, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+        else
+            return launch<T, G, N, TT, 1, 4, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    }
+    return launch<T, G, N, TT, 1, 1, 8>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+}
+
 template <class T, int G>
-int choose(mhip_ctx *c, T *out, int ldo, const void *w, const void *s, int rows, int cols, int n,
-           const void *ws) {
-    const bool many = rows >= 32768;
-    if (n > 32)
-        return many ? launch<T, G, 4, 1, 4, 2>(c, out, ldo, w, s, rows, cols, n, ws)
-                    : launch<T, G, 4, 1, 1, 8>(c, out, ldo, w, s, rows, cols, n, ws);
-    if (n > 16)
-        return many ? launch<T, G, 2, 1, 4, 2>(c, out, ldo, w, s, rows, cols, n, ws)
-                    : launch<T, G, 2, 1, 1, 8>(c, out, ldo, w, s, rows, cols, n, ws);
-    return many ? launch<T, G, 1, 2, 4, 1>(c, out, ldo, w, s, rows, cols, n, ws)
-                : launch<T, G, 1, 1, 1, 8>(c, out, ldo, w, s, rows, cols, n, ws);
+int choose(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
+           int n, void *ws, const T *x, int ldx) {
+    constexpr int P = sizeof(T) == 4 ? 2 : 1;
+    if (n <= FEW && (size_t)(cols + 127) / 128 * 128 * n * P * 2 <= FEW_LDS) {
+        if (n == 1) return by_rows<T, G, 1, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+        return by_rows<T, G, FEW, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    }
+    k_q4_tokens<T><<<dim3(n, (cols + SEG - 1) / SEG), 256, 0, c->stream>>>(x, ldx, cols, n, type,
+                                                                           (uint8_t *)ws);
+    if (mhip::check_launch(c, "matvec_q4 tokens")) return -1;
+    if (n > 32) return by_rows<T, G, 0, 4>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    if (n > 16) return by_rows<T, G, 0, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    return by_rows<T, G, 0, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
 }
 
 template <class T>
 int run(mhip_ctx *c, int type, void *out, int ldo, const void *w, const void *s, int group,
         const void *x, int ldx, int rows, int cols, int n, void *ws) {
-    k_q4_tokens<T><<<dim3(n, (cols + SEG - 1) / SEG), 256, 0, c->stream>>>(
-        (const T *)x, ldx, cols, n, type, (uint8_t *)ws);
-    if (group == 32) return choose<T, 32>(c, (T *)out, ldo, w, s, rows, cols, n, ws);
-    if (group == 64) return choose<T, 64>(c, (T *)out, ldo, w, s, rows, cols, n, ws);
-    return choose<T, 128>(c, (T *)out, ldo, w, s, rows, cols, n, ws);
+    if (group == 32) return choose<T, 32>(c, type, (T *)out, ldo, w, s, rows, cols, n, ws, (const T *)x, ldx);
+    if (group == 64) return choose<T, 64>(c, type, (T *)out, ldo, w, s, rows, cols, n, ws, (const T *)x, ldx);
+    return choose<T, 128>(c, type, (T *)out, ldo, w, s, rows, cols, n, ws, (const T *)x, ldx);
 }
 
 }  // namespace
