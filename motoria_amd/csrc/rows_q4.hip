@@ -143,16 +143,19 @@ __device__ inline void put(float *o, float v) { *o = v; }
 __device__ inline void put(_Float16 *o, float v) { *o = (_Float16)v; }
 __device__ inline void put(__bf16 *o, float v) { *o = (__bf16)v; }
 
-constexpr int DEPTH = 4;       // chunks of 128 columns requested ahead per wavefront
+template <int N> struct Words { typedef unsigned type __attribute__((ext_vector_type(N))); };
+template <> struct Words<1> { typedef unsigned type; };
+
 constexpr int FEW = 8;         // tokens whose operands a workgroup forms itself
 constexpr int FEW_LDS = 65536; // bytes of LDS for them
 
+// DEPTH: chunks of 128 columns requested ahead per wavefront.
 // WR x WK wavefronts: RT tiles of 16 rows for each of WR, the columns' chunks of
 // 128 dealt out to WK; TT tiles of 16 tokens. The tokens' operands come
 // through LDS, kc columns at a time, from the workspace; with N > 0 (1: one token,
 // 8: up to FEW) the workgroup forms them from x itself, which saves a launch, and for fp32
 // x hi and lo of a token are two of the instruction's sixteen token rows.
-template <class T, int G, int N, int TT, int RT, int WR, int WK>
+template <class T, int G, bool WHOLE, int N, int TT, int RT, int WR, int WK, int DEPTH>
 __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const uint8_t *w,
                                                      const uint16_t *scales, int rows, int cols,
                                                      int n, int kc, const uint8_t *ws, const T *x,
@@ -166,14 +169,12 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
     const int tg = blockIdx.y, nt = min(TG, n - tg * TG);
     const int nchunk = (cols + 127) / 128, nblock = cols / 32, ngroup = cols / G;
     const int row0 = (blockIdx.x * WR + wr) * RT * 16;
-    // a chunk's scales in one load, where every row's stand on its boundary
-    const bool whole = GC == 1 || (ngroup % GC == 0 && (uintptr_t)scales % (2 * GC) == 0);
     const uint8_t *wrow[RT];
     const uint16_t *srow[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) {
         const size_t r = min(row0 + i * 16 + lr, rows - 1);
-        wrow[i] = w + r * (cols / 2) + g * 16;
+        wrow[i] = w + r * (cols / 2);
         srow[i] = scales + r * ngroup;
     }
     float total[RT][TT][TL];
@@ -184,32 +185,36 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
 #pragma unroll
             for (int r = 0; r < TL; r++) total[i][t][r] = 0.0f;
 
+    // A slot per chunk on its way: codes, and the scales of its groups, two a word
+    // (one where they are loaded one by one).
+    constexpr int SW = WHOLE ? (GC + 1) / 2 : GC;
+    using scale_words = typename Words<SW>::type;
     u4 wq[DEPTH][RT];
-    uint16_t sq[DEPTH][RT][GC];
-    auto request = [&](int d, int chunk) {
+    scale_words sq[DEPTH][RT];
+    // chunks wk, wk + WK, ... : chunk number c of this wavefront is wk + c * WK
+    const int mine = nchunk > wk ? (nchunk - wk + WK - 1) / WK : 0;
+    // Loads without a branch, so that the waits count them: past the row's end
+    // (or this wavefront's last chunk) they read what is there and nobody uses.
+    auto request = [&](int d, int c) {
+        const int chunk = min(wk + c * WK, nchunk - 1);
+        const int block = min(chunk * 4 + g, nblock - 1);
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-            wq[d][i] = (u4){0, 0, 0, 0};
-            if (chunk * 4 + g < nblock) wq[d][i] = *(const u4 *)(wrow[i] + (size_t)chunk * 64);
-            if (whole) {
-                const uint16_t *at = srow[i] + chunk * GC;
-                if constexpr (GC == 4) *(uint2 *)sq[d][i] = *(const uint2 *)at;
-                else if constexpr (GC == 2) *(unsigned *)sq[d][i] = *(const unsigned *)at;
-                else sq[d][i][0] = at[0];
+            wq[d][i] = *(const u4 *)(wrow[i] + (size_t)block * 16);
+            if constexpr (WHOLE && GC > 1) {
+                sq[d][i] = *(const scale_words *)(srow[i] + chunk * GC);
             } else {
 #pragma unroll
                 for (int j = 0; j < GC; j++) {
-                    const int q = chunk * GC + j;
-                    sq[d][i][j] = q < ngroup ? srow[i][q] : (uint16_t)0;
+                    const unsigned h = srow[i][min(chunk * GC + j, ngroup - 1)];
+                    if constexpr (SW == 1) sq[d][i] = h;
+                    else sq[d][i][j] = h;
                 }
             }
         }
     };
-    // chunks wk, wk + WK, ... : chunk number c of this wavefront is wk + c * WK
-    const int mine = nchunk > wk ? (nchunk - wk + WK - 1) / WK : 0;
 #pragma unroll
-    for (int d = 0; d < DEPTH; d++)
-        if (d < mine) request(d, wk + d * WK);
+    for (int d = 0; d < DEPTH; d++) request(d, d);
 
     const size_t step = (size_t)P * nt * 64;  // bytes of a block of 32 columns
     float *fl = (float *)(lds + (size_t)(kc / 32) * step);
@@ -287,82 +292,101 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
 #pragma unroll
         for (int r = 0; r < TL; r++) own[t][r] = pair ? 2 * g + r : t * 16 + 4 * g + r;
     }
-    for (int c = 0; c < mine; c += DEPTH) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++) {
-            if (c + d >= mine) break;
-            const int chunk = wk + (c + d) * WK;
+    if constexpr (N > 0) stage();
+    // chunk c of this wavefront, from slot d; blocks: those of 32 columns that it has
+    auto work = [&](int d, int c, int blocks) {
+        const int chunk = wk + c * WK;
+        if constexpr (N == 0)
             while (chunk * 128 >= k0 + kc) stage();
-            unsigned q[RT][4];
-            float sc[RT][GC];
+        unsigned q[RT][4];
+        float sc[RT][GC];
 #pragma unroll
-            for (int i = 0; i < RT; i++) {
+        for (int i = 0; i < RT; i++) {
+            // (the slot is taken apart here and not, with a wait, where it was loaded)
+            u4 cw = wq[d][i];
+            scale_words sw = sq[d][i];
+            asm volatile("" : "+v"(cw));
+            asm volatile("" : "+v"(sw));
 #pragma unroll
-                for (int j = 0; j < 4; j++) q[i][j] = wq[d][i][j];
+            for (int j = 0; j < 4; j++) q[i][j] = cw[j];
 #pragma unroll
-                for (int j = 0; j < GC; j++)
-                    sc[i][j] = (float)__builtin_bit_cast(_Float16, sq[d][i][j]);
-                blocks_from_lanes(q[i]);
+            for (int j = 0; j < GC; j++) {
+                unsigned h;
+                if constexpr (SW == 1) h = sw >> (16 * j);
+                else h = WHOLE ? sw[j / 2] >> (16 * (j & 1)) : sw[j];
+                sc[i][j] = (float)__builtin_bit_cast(_Float16, (uint16_t)h);
             }
-            if (c + d + DEPTH < mine) request(d, chunk + DEPTH * WK);
-            const int b0 = chunk * 4 - k0 / 32;
-            float part[RT][TT][TL];
+        }
+        request(d, c + DEPTH);
+        __builtin_amdgcn_sched_barrier(0);  // (nothing below is worth more than these loads)
 #pragma unroll
-            for (int i = 0; i < RT; i++)
+        for (int i = 0; i < RT; i++) blocks_from_lanes(q[i]);
+        const int b0 = chunk * 4 - k0 / 32;
+        float part[RT][TT][TL];
 #pragma unroll
-                for (int t = 0; t < TT; t++)
+        for (int i = 0; i < RT; i++)
 #pragma unroll
-                    for (int r = 0; r < TL; r++) part[i][t][r] = 0.0f;
-            f4 hi[RT][TT], lo[RT][TT];
+            for (int t = 0; t < TT; t++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (chunk * 4 + j < nblock) {
-                    h8 b[RT];
+                for (int r = 0; r < TL; r++) part[i][t][r] = 0.0f;
+        f4 hi[RT][TT], lo[RT][TT];
 #pragma unroll
-                    for (int i = 0; i < RT; i++) b[i] = codes(q[i][j]);
-                    const bool begin = j % (G / 32) == 0, end = (j + 1) % (G / 32) == 0;
+        for (int j = 0; j < 4; j++) {
+            if (j < blocks) {
+                h8 b[RT];
 #pragma unroll
-                    for (int t = 0; t < TT; t++) {
-                        const uint8_t *at = lds + (size_t)(b0 + j) * step + from[t];
-                        const h8 a = *(const h8 *)at;
-                        h8 a2;
-                        if constexpr (split && !pair) a2 = *(const h8 *)(at + (size_t)nt * 64);
+                for (int i = 0; i < RT; i++) b[i] = codes(q[i][j]);
+                const bool begin = j % (G / 32) == 0, end = (j + 1) % (G / 32) == 0;
 #pragma unroll
-                        for (int i = 0; i < RT; i++) {
-                            const f4 z = {0, 0, 0, 0};
-                            hi[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                a, b[i], begin ? z : hi[i][t], 0, 0, 0);
-                            if constexpr (split && !pair)
-                                lo[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    a2, b[i], begin ? z : lo[i][t], 0, 0, 0);
-                            if (end) {
+                for (int t = 0; t < TT; t++) {
+                    const uint8_t *at = lds + (size_t)(b0 + j) * step + from[t];
+                    const h8 a = *(const h8 *)at;
+                    h8 a2;
+                    if constexpr (split && !pair) a2 = *(const h8 *)(at + (size_t)nt * 64);
 #pragma unroll
-                                for (int r = 0; r < TL; r++) {
-                                    float v = pair ? __builtin_fmaf(hi[i][t][2 * r + 1 & 3], 0x1p-11f,
-                                                                    hi[i][t][2 * r & 3])
-                                                   : hi[i][t][r];
-                                    if constexpr (split && !pair)
-                                        v = __builtin_fmaf(lo[i][t][r], 0x1p-11f, v);
-                                    part[i][t][r] = __builtin_fmaf(sc[i][j / (G / 32)], v, part[i][t][r]);
-                                }
+                    for (int i = 0; i < RT; i++) {
+                        const f4 z = {0, 0, 0, 0};
+                        hi[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            a, b[i], begin ? z : hi[i][t], 0, 0, 0);
+                        if constexpr (split && !pair)
+                            lo[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                a2, b[i], begin ? z : lo[i][t], 0, 0, 0);
+                        if (end) {
+#pragma unroll
+                            for (int r = 0; r < TL; r++) {
+                                float v = pair ? __builtin_fmaf(hi[i][t][2 * r + 1 & 3], 0x1p-11f,
+                                                                hi[i][t][2 * r & 3])
+                                               : hi[i][t][r];
+                                if constexpr (split && !pair)
+                                    v = __builtin_fmaf(lo[i][t][r], 0x1p-11f, v);
+                                part[i][t][r] = __builtin_fmaf(sc[i][j / (G / 32)], v, part[i][t][r]);
                             }
                         }
                     }
                 }
             }
-            // back to x's own scale
-            const float *f = fl + (chunk * 128 - k0) / SEG * TG;
-#pragma unroll
-            for (int t = 0; t < TT; t++)
-#pragma unroll
-                for (int r = 0; r < TL; r++) {
-                    const float back = f[N > 0 ? min(own[t][r], nt - 1) : own[t][r]];
-#pragma unroll
-                    for (int i = 0; i < RT; i++)
-                        total[i][t][r] = __builtin_fmaf(part[i][t][r], back, total[i][t][r]);
-                }
         }
-    }
+        // back to x's own scale
+        const float *f = fl + (chunk * 128 - k0) / SEG * TG;
+#pragma unroll
+        for (int t = 0; t < TT; t++)
+#pragma unroll
+            for (int r = 0; r < TL; r++) {
+                const float back = f[N > 0 ? min(own[t][r], nt - 1) : own[t][r]];
+#pragma unroll
+                for (int i = 0; i < RT; i++)
+                    total[i][t][r] = __builtin_fmaf(part[i][t][r], back, total[i][t][r]);
+            }
+    };
+    // whole rounds of whole chunks, and the rest
+    const int plain = cols / 128 > wk ? (cols / 128 - wk + WK - 1) / WK : 0;
+    int c = 0;
+    for (; c + DEPTH <= plain; c += DEPTH)
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++) work(d, c + d, 4);
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++)
+        if (c + d < mine) work(d, c + d, min(4, nblock - (wk + (c + d) * WK) * 4));
     while (k0 + kc < cols) stage();  // a wavefront whose chunks ended earlier
     if constexpr (WK > 1) {
         // the column shares' sums, added in their order by the first of them
@@ -443,7 +467,7 @@ int check_q4(mhip_ctx *c, const char *what, const void *d_codes, const void *d_s
 }
 
 // One shape of the kernel.
-template <class T, int G, int N, int TT, int RT, int WR, int WK>
+template <class T, int G, bool WHOLE, int N, int TT, int RT, int WR, int WK, int DEPTH>
 int launch(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
            int n, const void *ws, const T *x, int ldx) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
@@ -460,7 +484,7 @@ int launch(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s,
     size_t lds = (size_t)kc * P * nt * 2 + (size_t)((kc + SEG - 1) / SEG) * TG * 4;
     const size_t join = (size_t)(WK - 1) * WR * RT * TT * 1024;
     if (lds < join) lds = join;
-    auto k = k_q4<T, G, N, TT, RT, WR, WK>;
+    auto k = k_q4<T, G, WHOLE, N, TT, RT, WR, WK, DEPTH>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                  160 * 1024);
@@ -472,40 +496,44 @@ int launch(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s,
     return mhip::check_launch(c, "matvec_q4");
 }
 
-template <class T, int G, int N, int TT>
+template <class T, int G, bool WHOLE, int N, int TT>
 int by_rows(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
             int n, const void *ws, const T *x, int ldx) {
     if (rows >= 32768) {
         if constexpr (TT == 1)
-            return launch<T, G, N, 1, 2, 4, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+            return launch<T, G, WHOLE, N, 1, 2, 4, 1, 4>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
         else
-            return launch<T, G, N, TT, 1, 4, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+            return launch<T, G, WHOLE, N, TT, 1, 4, 2, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
     }
-    return launch<T, G, N, TT, 1, 1, 8>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    return launch<T, G, WHOLE, N, TT, 1, 1, 8, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
 }
 
-template <class T, int G>
+template <class T, int G, bool WHOLE>
 int choose(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
            int n, void *ws, const T *x, int ldx) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
     if (n <= FEW && (size_t)(cols + 127) / 128 * 128 * n * P * 2 <= FEW_LDS) {
-        if (n == 1) return by_rows<T, G, 1, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
-        return by_rows<T, G, FEW, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+        if (n == 1) return by_rows<T, G, WHOLE, 1, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+        return by_rows<T, G, WHOLE, FEW, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
     }
     k_q4_tokens<T><<<dim3(n, (cols + SEG - 1) / SEG), 256, 0, c->stream>>>(x, ldx, cols, n, type,
                                                                            (uint8_t *)ws);
     if (mhip::check_launch(c, "matvec_q4 tokens")) return -1;
-    if (n > 32) return by_rows<T, G, 0, 4>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
-    if (n > 16) return by_rows<T, G, 0, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
-    return by_rows<T, G, 0, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    if (n > 32) return by_rows<T, G, WHOLE, 0, 4>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    if (n > 16) return by_rows<T, G, WHOLE, 0, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    return by_rows<T, G, WHOLE, 0, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
 }
 
 template <class T>
 int run(mhip_ctx *c, int type, void *out, int ldo, const void *w, const void *s, int group,
         const void *x, int ldx, int rows, int cols, int n, void *ws) {
-    if (group == 32) return choose<T, 32>(c, type, (T *)out, ldo, w, s, rows, cols, n, ws, (const T *)x, ldx);
-    if (group == 64) return choose<T, 64>(c, type, (T *)out, ldo, w, s, rows, cols, n, ws, (const T *)x, ldx);
-    return choose<T, 128>(c, type, (T *)out, ldo, w, s, rows, cols, n, ws, (const T *)x, ldx);
+    // a chunk's scales in one load, where every row's stand on its boundary
+    const int gc = 128 / group;
+    const bool whole = cols / group % gc == 0 && (uintptr_t)s % (2 * gc) == 0;
+    auto call = [&](auto f) { return f(c, type, (T *)out, ldo, w, s, rows, cols, n, ws, (const T *)x, ldx); };
+    if (group == 32) return whole ? call(choose<T, 32, true>) : call(choose<T, 32, false>);
+    if (group == 64) return whole ? call(choose<T, 64, true>) : call(choose<T, 64, false>);
+    return call(choose<T, 128, true>);
 }
 
 }  // namespace
