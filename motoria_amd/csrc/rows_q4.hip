@@ -19,11 +19,13 @@
 // segment's largest value, as lo carries its own exponent; their products
 // are accumulated apart and joined in fp32. fp16 x is taken as it is.
 #include "mhip_internal.h"
+#include <type_traits>
 
 namespace {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
@@ -121,8 +123,16 @@ __device__ __forceinline__ h8 codes(unsigned w) {
     return (h8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A lane of group g (16 lanes) has loaded words 0..3 of column block g; the matrix
-// instructions want word g of block j: the transpose of words and lane
+// Eight codes in their order as bf16 (exact), through fp32.
+__device__ __forceinline__ b8 codes_bf(unsigned w) {
+    b8 r;
+#pragma unroll
+    for (int k = 0; k < 8; k++) r[k] = (__bf16)((float)((int)(w << (28 - 4 * k)) >> 28));
+    return r;
+}
+
+// A lane of group g (16 lanes) has loaded words 0..3 of its column block; the matrix
+// instructions want word g of group j's block: the transpose of words and lane
 // groups, by exchanging halves (32 lanes) and quarters (16).
 __device__ __forceinline__ void blocks_from_lanes(unsigned w[4]) {
 #pragma unroll
@@ -146,75 +156,78 @@ __device__ inline void put(__bf16 *o, float v) { *o = (__bf16)v; }
 template <int N> struct Words { typedef unsigned type __attribute__((ext_vector_type(N))); };
 template <> struct Words<1> { typedef unsigned type; };
 
+constexpr int CHUNK = 256;     // columns of a wavefront's step
 constexpr int FEW = 8;         // tokens whose operands a workgroup forms itself
 constexpr int FEW_LDS = 65536; // bytes of LDS for them
 
-// DEPTH: chunks of 128 columns requested ahead per wavefront.
-// WR x WK wavefronts: RT tiles of 16 rows for each of WR, the columns' chunks of
-// 128 dealt out to WK; TT tiles of 16 tokens. The tokens' operands come
-// through LDS, kc columns at a time, from the workspace; with N > 0 (1: one token,
-// 8: up to FEW) the workgroup forms them from x itself, which saves a launch, and for fp32
-// x hi and lo of a token are two of the instruction's sixteen token rows.
-template <class T, int G, bool WHOLE, int N, int TT, int RT, int WR, int WK, int DEPTH>
+// WR x WK wavefronts: a tile of 16 rows for each of WR, the columns' chunks of
+// 256 dealt out to WK; TT tiles of 16 tokens; DEPTH chunks requested ahead. The
+// tokens' operands come through LDS, kc columns at a time, from the workspace;
+// with N > 0 (1: one token, FEW: up to FEW) the workgroup forms them from x itself,
+// which saves a launch, and for fp32 x hi and lo of a token are two of the
+// instruction's sixteen token rows. With N > 0 and WK = 1 a wavefront takes one
+// tile after another, `stride` apart, with the next one's chunks on their
+// way. WHOLE: rows of whole chunks, a chunk's scales on their boundary (one
+// load). A chunk of 256 codes is 128 bytes of a row: with half of that the lines of
+// sixteen rows had left the CU's cache before their second half was asked for.
+template <class T, int G, bool WHOLE, int N, int TT, int WR, int WK, int DEPTH>
 __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const uint8_t *w,
                                                      const uint16_t *scales, int rows, int cols,
                                                      int n, int kc, const uint8_t *ws, const T *x,
                                                      size_t ldx, int type) {
     constexpr bool split = sizeof(T) == 4, pair = split && N > 0;
-    constexpr int P = split ? 2 : 1, NT = 64 * WR * WK, GC = 128 / G;  // groups of a chunk
-    constexpr int TL = N == 1 ? 1 : pair ? 2 : 4;                      // tokens of a lane and tile
+    constexpr int P = split ? 2 : 1, NT = 64 * WR * WK, GC = CHUNK / G;  // groups of a chunk
+    constexpr int TL = N == 1 ? 1 : pair ? 2 : 4;                        // tokens of a lane and tile
+    constexpr bool MANY = N > 0 && WK == 1;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR, g = lane >> 4, lr = lane & 15;
     const int tg = blockIdx.y, nt = min(TG, n - tg * TG);
-    const int nchunk = (cols + 127) / 128, nblock = cols / 32, ngroup = cols / G;
-    const int row0 = (blockIdx.x * WR + wr) * RT * 16;
-    const uint8_t *wrow[RT];
-    const uint16_t *srow[RT];
+    const int nchunk = (cols + CHUNK - 1) / CHUNK, nblock = cols / 32, ngroup = cols / G;
+    const int ntile = (rows + 15) / 16, stride = gridDim.x * WR;
+    int tile = blockIdx.x * WR + wr;
+    const int my_tiles = MANY ? (tile < ntile ? (ntile - tile + stride - 1) / stride : 0) : 1;
+    float total[TT][TL];
 #pragma unroll
-    for (int i = 0; i < RT; i++) {
-        const size_t r = min(row0 + i * 16 + lr, rows - 1);
-        wrow[i] = w + r * (cols / 2);
-        srow[i] = scales + r * ngroup;
-    }
-    float total[RT][TT][TL];
+    for (int t = 0; t < TT; t++)
 #pragma unroll
-    for (int i = 0; i < RT; i++)
-#pragma unroll
-        for (int t = 0; t < TT; t++)
-#pragma unroll
-            for (int r = 0; r < TL; r++) total[i][t][r] = 0.0f;
+        for (int r = 0; r < TL; r++) total[t][r] = 0.0f;
 
-    // A slot per chunk on its way: codes, and the scales of its groups, two a word
-    // (one where they are loaded one by one).
+    // A slot per chunk on its way: codes (blocks 2g and 2g + 1 of 32 columns for
+    // lane group g), and the scales of its groups, two a word (one where they are
+    // loaded one by one).
     constexpr int SW = WHOLE ? (GC + 1) / 2 : GC;
     using scale_words = typename Words<SW>::type;
-    u4 wq[DEPTH][RT];
-    scale_words sq[DEPTH][RT];
-    // chunks wk, wk + WK, ... : chunk number c of this wavefront is wk + c * WK
+    u4 wq[DEPTH][2];
+    scale_words sq[DEPTH];
+    // chunks wk, wk + WK, ... of each tile
     const int mine = nchunk > wk ? (nchunk - wk + WK - 1) / WK : 0;
-    // Loads without a branch, so that the waits count them: past the row's end
-    // (or this wavefront's last chunk) they read what is there and nobody uses.
-    auto request = [&](int d, int c) {
-        const int chunk = min(wk + c * WK, nchunk - 1);
-        const int block = min(chunk * 4 + g, nblock - 1);
+    int next_tile = tile, next_c = 0;
+    // Loads without a branch, so that the waits count them: past the end they
+    // read what is there and nobody uses.
+    auto request = [&](int d) {
+        const int chunk = min(wk + next_c * WK, nchunk - 1);
+        const size_t row = min(next_tile * 16 + lr, rows - 1);
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
-            wq[d][i] = *(const u4 *)(wrow[i] + (size_t)block * 16);
-            if constexpr (WHOLE && GC > 1) {
-                sq[d][i] = *(const scale_words *)(srow[i] + chunk * GC);
-            } else {
+        for (int h = 0; h < 2; h++) {
+            int block = chunk * (CHUNK / 32) + 2 * g + h;
+            if constexpr (!WHOLE) block = min(block, nblock - 1);
+            wq[d][h] = *(const u4 *)(w + row * (cols / 2) + (size_t)block * 16);
+        }
+        const uint16_t *at = scales + row * ngroup;
+        if constexpr (WHOLE) {
+            sq[d] = *(const scale_words *)(at + chunk * GC);
+        } else {
 #pragma unroll
-                for (int j = 0; j < GC; j++) {
-                    const unsigned h = srow[i][min(chunk * GC + j, ngroup - 1)];
-                    if constexpr (SW == 1) sq[d][i] = h;
-                    else sq[d][i][j] = h;
-                }
-            }
+            for (int j = 0; j < GC; j++) sq[d][j] = at[min(chunk * GC + j, ngroup - 1)];
+        }
+        if (++next_c >= mine) {
+            next_c = 0;
+            next_tile = min(next_tile + stride, ntile - 1);
         }
     };
 #pragma unroll
-    for (int d = 0; d < DEPTH; d++) request(d, d);
+    for (int d = 0; d < DEPTH; d++) request(d);
 
     const size_t step = (size_t)P * nt * 64;  // bytes of a block of 32 columns
     float *fl = (float *)(lds + (size_t)(kc / 32) * step);
@@ -293,100 +306,102 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
         for (int r = 0; r < TL; r++) own[t][r] = pair ? 2 * g + r : t * 16 + 4 * g + r;
     }
     if constexpr (N > 0) stage();
-    // chunk c of this wavefront, from slot d; blocks: those of 32 columns that it has
-    auto work = [&](int d, int c, int blocks) {
+    int c = 0;
+    auto store = [&]() {
+        const int row = tile * 16 + lr;
+#pragma unroll
+        for (int t = 0; t < TT; t++)
+#pragma unroll
+            for (int r = 0; r < TL; r++)
+                if (row < rows && own[t][r] < nt)
+                    put(out + (size_t)(tg * TG + own[t][r]) * ldo + row, total[t][r]);
+    };
+    auto work = [&](int d) {  // the next chunk, from slot d
         const int chunk = wk + c * WK;
         if constexpr (N == 0)
-            while (chunk * 128 >= k0 + kc) stage();
-        unsigned q[RT][4];
-        float sc[RT][GC];
-#pragma unroll
-        for (int i = 0; i < RT; i++) {
+            while (chunk * CHUNK >= k0 + kc) stage();
+        unsigned q[2][4];
+        float sc[GC];
+        {
             // (the slot is taken apart here and not, with a wait, where it was loaded)
-            u4 cw = wq[d][i];
-            scale_words sw = sq[d][i];
-            asm volatile("" : "+v"(cw));
-            asm volatile("" : "+v"(sw));
+            u4 c0 = wq[d][0], c1 = wq[d][1];
+            scale_words sw = sq[d];
+            asm volatile("" : "+v"(c0), "+v"(c1), "+v"(sw));
 #pragma unroll
-            for (int j = 0; j < 4; j++) q[i][j] = cw[j];
+            for (int j = 0; j < 4; j++) {
+                q[0][j] = c0[j];
+                q[1][j] = c1[j];
+            }
 #pragma unroll
             for (int j = 0; j < GC; j++) {
                 unsigned h;
                 if constexpr (SW == 1) h = sw >> (16 * j);
                 else h = WHOLE ? sw[j / 2] >> (16 * (j & 1)) : sw[j];
-                sc[i][j] = (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+                sc[j] = (float)__builtin_bit_cast(_Float16, (uint16_t)h);
             }
         }
-        request(d, c + DEPTH);
-        __builtin_amdgcn_sched_barrier(0);  // (nothing below is worth more than these loads)
+        request(d);
+        __builtin_amdgcn_sched_barrier(0x78f);  // (all but memory reads may pass)
+        blocks_from_lanes(q[0]);
+        blocks_from_lanes(q[1]);
+        const int b0 = chunk * (CHUNK / 32) - k0 / 32, blocks = nblock - chunk * (CHUNK / 32);
+        float part[TT][TL];
 #pragma unroll
-        for (int i = 0; i < RT; i++) blocks_from_lanes(q[i]);
-        const int b0 = chunk * 4 - k0 / 32;
-        float part[RT][TT][TL];
+        for (int t = 0; t < TT; t++)
 #pragma unroll
-        for (int i = 0; i < RT; i++)
+            for (int r = 0; r < TL; r++) part[t][r] = 0.0f;
+        f4 hi[TT], lo[TT];
 #pragma unroll
-            for (int t = 0; t < TT; t++)
-#pragma unroll
-                for (int r = 0; r < TL; r++) part[i][t][r] = 0.0f;
-        f4 hi[RT][TT], lo[RT][TT];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j < blocks) {
-                h8 b[RT];
-#pragma unroll
-                for (int i = 0; i < RT; i++) b[i] = codes(q[i][j]);
+        for (int j = 0; j < CHUNK / 32; j++) {
+            if (WHOLE || j < blocks) {
+                const h8 b = codes(q[j & 1][j >> 1]);
                 const bool begin = j % (G / 32) == 0, end = (j + 1) % (G / 32) == 0;
 #pragma unroll
                 for (int t = 0; t < TT; t++) {
                     const uint8_t *at = lds + (size_t)(b0 + j) * step + from[t];
-                    const h8 a = *(const h8 *)at;
-                    h8 a2;
-                    if constexpr (split && !pair) a2 = *(const h8 *)(at + (size_t)nt * 64);
+                    const f4 z = {0, 0, 0, 0};
+                    hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8 *)at, b, begin ? z : hi[t], 0, 0, 0);
+                    if constexpr (split && !pair)
+                        lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8 *)(at + (size_t)nt * 64), b,
+                                                                       begin ? z : lo[t], 0, 0, 0);
+                    if (end) {
 #pragma unroll
-                    for (int i = 0; i < RT; i++) {
-                        const f4 z = {0, 0, 0, 0};
-                        hi[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            a, b[i], begin ? z : hi[i][t], 0, 0, 0);
-                        if constexpr (split && !pair)
-                            lo[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                a2, b[i], begin ? z : lo[i][t], 0, 0, 0);
-                        if (end) {
-#pragma unroll
-                            for (int r = 0; r < TL; r++) {
-                                float v = pair ? __builtin_fmaf(hi[i][t][2 * r + 1 & 3], 0x1p-11f,
-                                                                hi[i][t][2 * r & 3])
-                                               : hi[i][t][r];
-                                if constexpr (split && !pair)
-                                    v = __builtin_fmaf(lo[i][t][r], 0x1p-11f, v);
-                                part[i][t][r] = __builtin_fmaf(sc[i][j / (G / 32)], v, part[i][t][r]);
-                            }
+                        for (int r = 0; r < TL; r++) {
+                            float v = pair ? __builtin_fmaf(hi[t][(2 * r + 1) & 3], 0x1p-11f, hi[t][2 * r & 3])
+                                           : hi[t][r];
+                            if constexpr (split && !pair) v = __builtin_fmaf(lo[t][r], 0x1p-11f, v);
+                            part[t][r] = __builtin_fmaf(sc[j / (G / 32)], v, part[t][r]);
                         }
                     }
                 }
             }
         }
         // back to x's own scale
-        const float *f = fl + (chunk * 128 - k0) / SEG * TG;
+        const float *f = fl + (chunk * CHUNK - k0) / SEG * TG;
 #pragma unroll
         for (int t = 0; t < TT; t++)
 #pragma unroll
-            for (int r = 0; r < TL; r++) {
-                const float back = f[N > 0 ? min(own[t][r], nt - 1) : own[t][r]];
+            for (int r = 0; r < TL; r++)
+                total[t][r] = __builtin_fmaf(part[t][r], f[N > 0 ? min(own[t][r], nt - 1) : own[t][r]], total[t][r]);
+        if (++c == mine && MANY) {
+            store();
 #pragma unroll
-                for (int i = 0; i < RT; i++)
-                    total[i][t][r] = __builtin_fmaf(part[i][t][r], back, total[i][t][r]);
-            }
+            for (int t = 0; t < TT; t++)
+#pragma unroll
+                for (int r = 0; r < TL; r++) total[t][r] = 0.0f;
+            c = 0;
+            tile += stride;
+        }
     };
-    // whole rounds of whole chunks, and the rest
-    const int plain = cols / 128 > wk ? (cols / 128 - wk + WK - 1) / WK : 0;
-    int c = 0;
-    for (; c + DEPTH <= plain; c += DEPTH)
+    const int steps = my_tiles * mine;
+    int i = 0;
+    for (; i + DEPTH <= steps; i += DEPTH)
 #pragma unroll
-        for (int d = 0; d < DEPTH; d++) work(d, c + d, 4);
+        for (int d = 0; d < DEPTH; d++) work(d);
 #pragma unroll
     for (int d = 0; d < DEPTH; d++)
-        if (c + d < mine) work(d, c + d, min(4, nblock - (wk + (c + d) * WK) * 4));
+        if (i + d < steps) work(d);
+    if constexpr (MANY) return;
     while (k0 + kc < cols) stage();  // a wavefront whose chunks ended earlier
     if constexpr (WK > 1) {
         // the column shares' sums, added in their order by the first of them
@@ -394,34 +409,146 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
         float *sum = (float *)lds;
         if (wk > 0) {
 #pragma unroll
-            for (int i = 0; i < RT; i++)
+            for (int t = 0; t < TT; t++)
 #pragma unroll
-                for (int t = 0; t < TT; t++)
-#pragma unroll
-                    for (int r = 0; r < TL; r++)
-                        sum[((((wk - 1) * WR + wr) * RT + i) * TT * TL + t * TL + r) * 64 + lane] = total[i][t][r];
+                for (int r = 0; r < TL; r++)
+                    sum[(((wk - 1) * WR + wr) * TT * TL + t * TL + r) * 64 + lane] = total[t][r];
         }
         __syncthreads();
         if (wk > 0) return;
         for (int k = 0; k < WK - 1; k++)
 #pragma unroll
-            for (int i = 0; i < RT; i++)
+            for (int t = 0; t < TT; t++)
 #pragma unroll
-                for (int t = 0; t < TT; t++)
-#pragma unroll
-                    for (int r = 0; r < TL; r++)
-                        total[i][t][r] += sum[(((k * WR + wr) * RT + i) * TT * TL + t * TL + r) * 64 + lane];
+                for (int r = 0; r < TL; r++)
+                    total[t][r] += sum[((k * WR + wr) * TT * TL + t * TL + r) * 64 + lane];
     }
+    store();
+}
+
+// More than FEW tokens and not so many rows: one tile of 16 rows, the chunks of
+// 256 columns dealt out to eight wavefronts. Each operand of the tokens is used
+// once in the workgroup, so it comes straight from memory (L2) into registers: 16-bit
+// x from x itself, unscaled and whole -- bf16 codes for a bf16 product, which
+// cost twice the instructions that fp16 ones do, shared by the TT tiles of 16 tokens
+// -- and fp32 x from the workspace.
+template <class T, int G, bool WHOLE, int TT>
+__global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8_t *w,
+                                                 const uint16_t *scales, int rows, int cols, int n,
+                                                 const uint8_t *ws, const T *x, size_t ldx) {
+    constexpr bool split = sizeof(T) == 4, bf = std::is_same<T, __bf16>::value;
+    constexpr int GC = CHUNK / G, WK = 8;
+    __shared__ float sum[(WK - 1) * TT * 4 * 64];
+    const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, lr = lane & 15, tg = blockIdx.y, nt = min(TG, n - tg * TG);
+    const int nchunk = (cols + CHUNK - 1) / CHUNK, nblock = cols / 32, ngroup = cols / G;
+    const size_t row = min((int)blockIdx.x * 16 + lr, rows - 1);
+    const uint8_t *wr = w + row * (cols / 2);
+    const uint16_t *sr = scales + row * ngroup;
+    const Tokens l = tokens_of(split ? MHIP_F32 : MHIP_F16, cols, n);
+    const uint8_t *xg = ws + (size_t)tg * l.group;
+    const float *fg = (const float *)(xg + l.operands);
+    const uint8_t *from[TT];  // a lane's token row (past the last: the last one's)
 #pragma unroll
-    for (int i = 0; i < RT; i++) {
-        const int row = row0 + i * 16 + lr;
+    for (int t = 0; t < TT; t++) {
+        const int tok = min(t * 16 + lr, nt - 1);
+        from[t] = split ? xg + tok * 64 + g * 16 : (const uint8_t *)(x + (size_t)(tg * TG + tok) * ldx + g * 8);
+    }
+    const size_t step = split ? (size_t)2 * nt * 64 : 64;  // bytes from a block of 32 columns to the next
+    f4 total[TT];
+#pragma unroll
+    for (int t = 0; t < TT; t++) total[t] = (f4){0, 0, 0, 0};
+    for (int chunk = wk; chunk < nchunk; chunk += WK) {
+        unsigned q[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            int block = chunk * (CHUNK / 32) + 2 * g + h;
+            if constexpr (!WHOLE) block = min(block, nblock - 1);
+            *(u4 *)q[h] = *(const u4 *)(wr + (size_t)block * 16);
+        }
+        float sc[GC];
+        uint16_t raw[GC];
+        if constexpr (WHOLE) {
+            using words = typename Words<GC / 2>::type;
+            *(words *)raw = *(const words *)(sr + chunk * GC);
+        } else {
+#pragma unroll
+            for (int j = 0; j < GC; j++) raw[j] = sr[min(chunk * GC + j, ngroup - 1)];
+        }
+#pragma unroll
+        for (int j = 0; j < GC; j++) sc[j] = (float)__builtin_bit_cast(_Float16, raw[j]);
+        blocks_from_lanes(q[0]);
+        blocks_from_lanes(q[1]);
+        const int b0 = chunk * (CHUNK / 32), blocks = nblock - b0;
+        f4 part[TT], hi[TT], lo[TT];
+#pragma unroll
+        for (int t = 0; t < TT; t++) part[t] = (f4){0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < CHUNK / 32; j++) {
+            if (WHOLE || j < blocks) {
+                const unsigned code = q[j & 1][j >> 1];
+                const bool begin = j % (G / 32) == 0, end = (j + 1) % (G / 32) == 0;
+#pragma unroll
+                for (int t = 0; t < TT; t++) {
+                    const uint8_t *at = from[t] + (size_t)(b0 + j) * step;
+                    const u4 a = *(const u4 *)at;
+                    const f4 z = {0, 0, 0, 0}, c = begin ? z : hi[t];
+                    if constexpr (bf) {
+                        hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), codes_bf(code), c, 0, 0, 0);
+                    } else if constexpr (split) {
+                        const h8 b = codes(code);
+                        hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), b, c, 0, 0, 0);
+                        lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8 *)(at + (size_t)nt * 64), b,
+                                                                       begin ? z : lo[t], 0, 0, 0);
+                    } else {
+                        // column k of an eight next to column k + 4, as codes() has them
+                        const u4 p = {__builtin_amdgcn_perm(a[2], a[0], 0x05040100), __builtin_amdgcn_perm(a[2], a[0], 0x07060302),
+                                      __builtin_amdgcn_perm(a[3], a[1], 0x05040100), __builtin_amdgcn_perm(a[3], a[1], 0x07060302)};
+                        hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, p), codes(code), c, 0, 0, 0);
+                    }
+                    if (end) {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            float v = hi[t][r];
+                            if constexpr (split) v = __builtin_fmaf(lo[t][r], 0x1p-11f, v);
+                            part[t][r] = __builtin_fmaf(sc[j / (G / 32)], v, part[t][r]);
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TT; t++) {
+            if constexpr (split) {  // back to x's own scale
+                const f4 back = *(const f4 *)(fg + (size_t)(chunk * CHUNK / SEG) * TG + t * 16 + g * 4);
+#pragma unroll
+                for (int r = 0; r < 4; r++) total[t][r] = __builtin_fmaf(part[t][r], back[r], total[t][r]);
+            } else {
+                total[t] += part[t];
+            }
+        }
+    }
+    // the column shares' sums, added in their order
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (wk > 0) sum[((wk - 1) * TT * 4 + t * 4 + r) * 64 + lane] = total[t][r];
+    __syncthreads();
+    if (wk > 0) return;
+    for (int k = 0; k < WK - 1; k++)
 #pragma unroll
         for (int t = 0; t < TT; t++)
 #pragma unroll
-            for (int r = 0; r < TL; r++)
-                if (row < rows && own[t][r] < nt)
-                    put(out + (size_t)(tg * TG + own[t][r]) * ldo + row, total[i][t][r]);
-    }
+            for (int r = 0; r < 4; r++) total[t][r] += sum[(k * TT * 4 + t * 4 + r) * 64 + lane];
+    const int at = blockIdx.x * 16 + lr;
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int tok = t * 16 + 4 * g + r;
+            if (at < rows && tok < nt) put(out + (size_t)(tg * TG + tok) * ldo + at, total[t][r]);
+        }
 }
 
 // One thread a group (weights are quantized once, when a model is loaded).
@@ -467,7 +594,7 @@ int check_q4(mhip_ctx *c, const char *what, const void *d_codes, const void *d_s
 }
 
 // One shape of the kernel.
-template <class T, int G, bool WHOLE, int N, int TT, int RT, int WR, int WK, int DEPTH>
+template <class T, int G, bool WHOLE, int N, int TT, int WR, int WK, int DEPTH>
 int launch(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
            int n, const void *ws, const T *x, int ldx) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
@@ -479,61 +606,72 @@ int launch(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s,
     if ((size_t)kc * P * nt * 2 <= 48 * 1024)
         kc = 48 * 1024 / (P * nt * 2) / SEG * SEG;
     else
-        while ((size_t)kc * P * nt * 2 > 128 * 1024) kc /= 2;
-    if (kc > cols || N > 0) kc = (cols + 127) / 128 * 128;
+        while ((size_t)kc * P * nt * 2 > 128 * 1024) kc /= 2;  // 512 at least
+    if (kc > cols || N > 0) kc = (cols + CHUNK - 1) / CHUNK * CHUNK;
     size_t lds = (size_t)kc * P * nt * 2 + (size_t)((kc + SEG - 1) / SEG) * TG * 4;
-    const size_t join = (size_t)(WK - 1) * WR * RT * TT * 1024;
+    const size_t join = (size_t)(WK - 1) * WR * TT * 1024;
     if (lds < join) lds = join;
-    auto k = k_q4<T, G, WHOLE, N, TT, RT, WR, WK, DEPTH>;
+    auto k = k_q4<T, G, WHOLE, N, TT, WR, WK, DEPTH>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                  160 * 1024);
         if (mhip::check(c, e, "matvec_q4 LDS attribute")) return -1;
     }
-    const dim3 grid((rows + RT * WR * 16 - 1) / (RT * WR * 16), (n + TG - 1) / TG);
+    int wgs = (rows + WR * 16 - 1) / (WR * 16);
+    if (N > 0 && WK == 1 && wgs > 768) wgs = 768;  // three a CU: each takes tile after tile
+    const dim3 grid(wgs, (n + TG - 1) / TG);
     k<<<grid, 64 * WR * WK, lds, c->stream>>>(out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows,
                                               cols, n, kc, (const uint8_t *)ws, x, ldx, type);
     return mhip::check_launch(c, "matvec_q4");
 }
 
-template <class T, int G, bool WHOLE, int N, int TT>
-int by_rows(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
-            int n, const void *ws, const T *x, int ldx) {
-    if (rows >= 32768) {
-        if constexpr (TT == 1)
-            return launch<T, G, WHOLE, N, 1, 2, 4, 1, 4>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
-        else
-            return launch<T, G, WHOLE, N, TT, 1, 4, 2, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+// From 12288 rows on there is a tile for each of three workgroups' wavefronts on every
+// CU, which then take whole rows one after another; below, the columns are split
+// over a workgroup's wavefronts (2048 columns, one token: 8192 rows 6.4 us, whole
+// rows 7.9; 16384 rows 11.3 us, whole rows 8.1; head of 151936 rows 73 and 40 us).
+constexpr int MANY_ROWS = 12288;
+
+template <class T, int G, bool WHOLE, int TT>
+int many_tokens(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows,
+                int cols, int n, void *ws, const T *x, int ldx) {
+    const bool many = rows >= MANY_ROWS;
+    if (many || type == MHIP_F32) {
+        k_q4_tokens<T><<<dim3(n, (cols + SEG - 1) / SEG), 256, 0, c->stream>>>(x, ldx, cols, n, type,
+                                                                               (uint8_t *)ws);
+        if (mhip::check_launch(c, "matvec_q4 tokens")) return -1;
     }
-    return launch<T, G, WHOLE, N, TT, 1, 1, 8, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    if (many) return launch<T, G, WHOLE, 0, TT, 4, 2, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    k_q4_wide<T, G, WHOLE, TT><<<dim3((rows + 15) / 16, (n + TG - 1) / TG), 512, 0, c->stream>>>(
+        out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows, cols, n, (const uint8_t *)ws, x, ldx);
+    return mhip::check_launch(c, "matvec_q4");
 }
 
 template <class T, int G, bool WHOLE>
 int choose(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows, int cols,
            int n, void *ws, const T *x, int ldx) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
-    if (n <= FEW && (size_t)(cols + 127) / 128 * 128 * n * P * 2 <= FEW_LDS) {
-        if (n == 1) return by_rows<T, G, WHOLE, 1, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
-        return by_rows<T, G, WHOLE, FEW, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    if (n <= FEW && (size_t)(cols + CHUNK - 1) / CHUNK * CHUNK * n * P * 2 <= FEW_LDS) {
+        const bool many = rows >= MANY_ROWS;
+        if (n == 1)
+            return many ? launch<T, G, WHOLE, 1, 1, 4, 1, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx)
+                        : launch<T, G, WHOLE, 1, 1, 1, 8, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+        return many ? launch<T, G, WHOLE, FEW, 1, 4, 1, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx)
+                    : launch<T, G, WHOLE, FEW, 1, 1, 8, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
     }
-    k_q4_tokens<T><<<dim3(n, (cols + SEG - 1) / SEG), 256, 0, c->stream>>>(x, ldx, cols, n, type,
-                                                                           (uint8_t *)ws);
-    if (mhip::check_launch(c, "matvec_q4 tokens")) return -1;
-    if (n > 32) return by_rows<T, G, WHOLE, 0, 4>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
-    if (n > 16) return by_rows<T, G, WHOLE, 0, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
-    return by_rows<T, G, WHOLE, 0, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    if (n > 32) return many_tokens<T, G, WHOLE, 4>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    if (n > 16) return many_tokens<T, G, WHOLE, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    return many_tokens<T, G, WHOLE, 1>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
 }
 
 template <class T>
 int run(mhip_ctx *c, int type, void *out, int ldo, const void *w, const void *s, int group,
         const void *x, int ldx, int rows, int cols, int n, void *ws) {
-    // a chunk's scales in one load, where every row's stand on its boundary
-    const int gc = 128 / group;
-    const bool whole = cols / group % gc == 0 && (uintptr_t)s % (2 * gc) == 0;
+    // rows of whole chunks, a chunk's scales in one load
+    const bool whole = cols % CHUNK == 0 && (uintptr_t)s % (2 * CHUNK / group) == 0;
     auto call = [&](auto f) { return f(c, type, (T *)out, ldo, w, s, rows, cols, n, ws, (const T *)x, ldx); };
     if (group == 32) return whole ? call(choose<T, 32, true>) : call(choose<T, 32, false>);
     if (group == 64) return whole ? call(choose<T, 64, true>) : call(choose<T, 64, false>);
-    return call(choose<T, 128, true>);
+    return whole ? call(choose<T, 128, true>) : call(choose<T, 128, false>);
 }
 
 }  // namespace
