@@ -20,14 +20,17 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // us, 16 parts 33, 32 parts 41) and 256 for the slots (32 unshared slots of up
 // to 8000 tokens: 2 parts 79 us, 8 parts 90; 64 of 300 tokens: 1 part 12 us, 2
 // parts 18). Where a CU holds one workgroup only (tiles of 128 KB: fp32 heads of
-// 128, or heads of 256) the two together should not be more than the CUs.
+// 128, or heads of 256) the two together should not be more than the CUs, and a
+// tile of the prefix takes longest (fp32: 64 rows 4.7 us, a slot's rows 1.6).
 Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int max_len) {
     Cut k;
     const int group = n_heads / s->n_kv_heads, rest = max_len - prefix;
     const long long rows = (long long)n * mc * group;
     k.stiles = (mc * group + 15) / 16;
     const long long items = (long long)n * s->n_kv_heads * k.stiles;
-    long long parts = 256 / items;
+    const int padded = s->head_dim <= 64 ? 64 : s->head_dim <= 128 ? 128 : 256;
+    const bool single = padded * mhip::type_bytes(s->type) > 256;  // one workgroup a CU
+    long long parts = (prefix > 0 && single ? 96 : 256) / items;
     const int most = (rest + 255) / 256, least = (rest + PART_MAX - 1) / PART_MAX;
     if (parts > most) parts = most;
     if (parts < least) parts = least;
@@ -42,9 +45,7 @@ Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int 
     k.sp = 0;
     k.plen = 0;
     if (prefix > 0) {
-        const int padded = s->head_dim <= 64 ? 64 : s->head_dim <= 128 ? 128 : 256;
-        const long long slots = padded * mhip::type_bytes(s->type) > 256 ? 256 : 512;
-        long long wgs = slots - items * k.ss;
+        long long wgs = (single ? 256 : 512) - items * k.ss;
         if (wgs > 256) wgs = 256;
         if (wgs < 128) wgs = 128;
         long long pp = wgs / ((long long)k.ptiles * s->n_kv_heads);
