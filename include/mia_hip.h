@@ -507,7 +507,7 @@ int mhip_pages_extend(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * slot (NULL: max_count each): token j < d_count[i] of entry i is row
  * i * max_count + j of d_k and d_v (rows of n_kv_heads * head_dim values, ld
  * values apart, 16-byte aligned as the rows' step is; rows past d_count[i] are
- * not read). */
+ * in the arrays, but not used). */
 int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,
                      const int *d_seqs, const int *d_count, int n, int max_count,
                      const void *d_k, const void *d_v, int ld);

@@ -574,7 +574,7 @@ class Pages:
     def __init__(self, gpu, dims, **arrays):
         self.gpu, self.dims, self.mem = gpu, dims, None
         self.arrays = PageArrays(**arrays)
-        self._d, self._a = ctypes.byref(self.dims), ctypes.byref(self.arrays)
+        self._d, self._a, self._fns = ctypes.byref(self.dims), ctypes.byref(self.arrays), {}
         if not arrays:
             nbytes = lib().mhip_pages_bytes(self._d)
             if not nbytes:
@@ -589,28 +589,31 @@ class Pages:
             self.gpu.free(self.mem)
             self.mem = None
 
+    # (one call per layer and token: the bindings are looked up once)
+    def _call(self, name, *args):
+        fn = self._fns.get(name)
+        if fn is None:
+            fn = self._fns[name] = getattr(lib(), name)
+        if fn(self.gpu.h, self._d, self._a, *args):
+            self.gpu.check(-1, name)
+
     def clear(self):
-        self.gpu.check(lib().mhip_pages_clear(self.gpu.h, self._d, self._a), "mhip_pages_clear")
+        self._call("mhip_pages_clear")
 
     def extend(self, d_seqs, d_count, n):
-        self.gpu.check(lib().mhip_pages_extend(self.gpu.h, self._d, self._a, d_seqs, d_count, n),
-                       "mhip_pages_extend")
+        self._call("mhip_pages_extend", d_seqs, d_count, n)
 
     def write(self, layer, d_seqs, d_count, n, max_count, d_k, d_v, ld):
-        self.gpu.check(lib().mhip_pages_write(self.gpu.h, self._d, self._a, layer, d_seqs, d_count,
-                                              n, max_count, d_k, d_v, ld), "mhip_pages_write")
+        self._call("mhip_pages_write", layer, d_seqs, d_count, n, max_count, d_k, d_v, ld)
 
     def fork(self, d_src, d_dst, n, flags=0):
-        self.gpu.check(lib().mhip_pages_fork(self.gpu.h, self._d, self._a, d_src, d_dst, n, flags),
-                       "mhip_pages_fork")
+        self._call("mhip_pages_fork", d_src, d_dst, n, flags)
 
     def free(self, d_seqs, n):
-        self.gpu.check(lib().mhip_pages_free(self.gpu.h, self._d, self._a, d_seqs, n),
-                       "mhip_pages_free")
+        self._call("mhip_pages_free", d_seqs, n)
 
     def compact(self):
-        self.gpu.check(lib().mhip_pages_compact(self.gpu.h, self._d, self._a),
-                       "mhip_pages_compact")
+        self._call("mhip_pages_compact")
 
     def status(self):
         """(error bits since the last call, free pages); waits for the stream."""
@@ -625,9 +628,8 @@ class Pages:
 
     def attention(self, layer, n_heads, d_q, ldq, d_out, ldo, d_seqs, d_count, n, max_count,
                   prefix_seq, prefix, max_len, scale, d_ws):
-        self.gpu.check(lib().mhip_attention_shared(
-            self.gpu.h, self._d, self._a, layer, n_heads, d_q, ldq, d_out, ldo, d_seqs, d_count, n,
-            max_count, prefix_seq, prefix, max_len, scale, d_ws), "mhip_attention_shared")
+        self._call("mhip_attention_shared", layer, n_heads, d_q, ldq, d_out, ldo, d_seqs, d_count, n,
+                   max_count, prefix_seq, prefix, max_len, scale, d_ws)
 
 
 def matvec_q4_ws_bytes(type, cols, n):

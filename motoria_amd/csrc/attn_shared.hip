@@ -12,25 +12,23 @@ using mhip_shared::TILE;
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// How a call is cut. A part of the prefix serves up to 128 rows; tiles of 64
-// rows do better up to 128 rows in all (16 slots behind 16000 tokens, bf16: 28 us,
+// How a call is cut. A part of the prefix serves up to 128 rows (16-bit heads up
+// to 128); tiles of 64 rows do better up to 128 rows in all (16 slots behind 16000 tokens, bf16: 28 us,
 // with tiles of 128 rows 32; 64 slots behind 8000: 35 and 33). Every part's
 // results pass through memory once more, so there are only as many as
 // keep the CUs busy: 256 workgroups for the prefix (64 x 8000: with 8 parts 41
 // us, 16 parts 33, 32 parts 41) and 256 for the slots (32 unshared slots of up
 // to 8000 tokens: 2 parts 79 us, 8 parts 90; 64 of 300 tokens: 1 part 12 us, 2
-// parts 18). Where a CU holds one workgroup only (tiles of 128 KB: fp32 heads of
-// 128, or heads of 256) the two together should not be more than the CUs, and a
-// tile of the prefix takes longest (fp32: 64 rows 4.7 us, a slot's rows 1.6).
+// parts 18; fp32 behind a prefix, whose tiles take longest, half as many). Where
+// a CU holds one workgroup only the two together should not be more than the
+// CUs.
 Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int max_len) {
     Cut k;
     const int group = n_heads / s->n_kv_heads, rest = max_len - prefix;
     const long long rows = (long long)n * mc * group;
     k.stiles = (mc * group + 15) / 16;
     const long long items = (long long)n * s->n_kv_heads * k.stiles;
-    const int padded = s->head_dim <= 64 ? 64 : s->head_dim <= 128 ? 128 : 256;
-    const bool single = padded * mhip::type_bytes(s->type) > 256;  // one workgroup a CU
-    long long parts = (prefix > 0 && single ? 96 : 256) / items;
+    long long parts = (prefix > 0 && s->type == MHIP_F32 ? 96 : 256) / items;
     const int most = (rest + 255) / 256, least = (rest + PART_MAX - 1) / PART_MAX;
     if (parts > most) parts = most;
     if (parts < least) parts = least;
@@ -39,12 +37,14 @@ Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int 
     k.ss = rest > 0 ? (rest + k.slen - 1) / k.slen : 1;
 
     k.wr = prefix == 0 ? 1 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
-    k.rt = prefix > 0 && rows > 128 && s->head_dim <= 128 ? 2 : 1;
+    k.rt = prefix > 0 && rows > 128 && s->head_dim <= 128 && s->type != MHIP_F32 ? 2 : 1;
     const int tile = k.wr * k.rt * 16;
     k.ptiles = prefix > 0 ? (int)((rows + tile - 1) / tile) : 0;
     k.sp = 0;
     k.plen = 0;
     if (prefix > 0) {
+        const int padded = s->head_dim <= 64 ? 64 : s->head_dim <= 128 ? 128 : 256;
+        const bool single = padded * mhip::type_bytes(s->type) > (tile > 16 ? 512 : 256);
         long long wgs = (single ? 256 : 512) - items * k.ss;
         if (wgs > 256) wgs = 256;
         if (wgs < 128) wgs = 128;

@@ -58,20 +58,36 @@ __device__ long long scan(long long v, long long *total, long long *lds) {
 
 __device__ inline int blocks_of(int tokens, int page) { return (tokens + page - 1) / page; }
 
+// LDS of a workgroup that decides. Its loads depend on each other (entry,
+// length, pages), and each level costs about 0.7 us, so what can be asked for
+// early is, and lists of up to NT entries and pages stay here.
+struct Desk {
+    unsigned seen[SEQ_WORDS];
+    long long sums[NT / 64];
+    int first[NT], list[NT], slot[NT], len[NT];
+    int bad;
+};
+
+// Which of this thread's PER pages from `base` on are free.
+__device__ unsigned free_mask(const mhip_page_dims &s, const mhip_pages &p, int base) {
+    const int at = base + threadIdx.x * PER;
+    unsigned is = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++)
+        if (at + j < s.n_pages && p.refs[at + j] <= 0) is |= 1u << j;
+    return is;
+}
+
 // The first `want` free pages in ascending order into out[]; whether there
-// are as many. Every page below the hint is in use.
-__device__ bool take_free(const mhip_page_dims &s, const mhip_pages &p, int want, int *out,
-                          long long *lds) {
+// are as many. Every page below `from` (the hint) is in use; is: free_mask there.
+__device__ bool take_free(const mhip_page_dims &s, const mhip_pages &p, int want, int *out, int from,
+                          unsigned is, long long *sums) {
     int got = 0;
-    const int from = max(0, min(p.state[ST_HINT], s.n_pages));
     for (int base = from; base < s.n_pages && got < want; base += NT * PER) {
         const int at = base + threadIdx.x * PER;
-        unsigned is = 0;
-#pragma unroll
-        for (int j = 0; j < PER; j++)
-            if (at + j < s.n_pages && p.refs[at + j] <= 0) is |= 1u << j;
+        if (base != from) is = free_mask(s, p, base);
         long long all;
-        int r = got + (int)scan(__popc(is), &all, lds);
+        int r = got + (int)scan(__popc(is), &all, sums);
         for (int j = 0; j < PER; j++)
             if (is >> j & 1) {
                 if (r < want) out[r] = at + j;
@@ -79,7 +95,7 @@ __device__ bool take_free(const mhip_page_dims &s, const mhip_pages &p, int want
             }
         got = min(want, got + (int)all);
     }
-    __syncthreads();  // out[] is written (by this workgroup, in global memory)
+    __syncthreads();  // out[] is written
     return got == want;
 }
 
@@ -94,102 +110,114 @@ __device__ inline int entry_of(const int *first, int n, int x) {
     return lo;
 }
 
-// Prefix sums of need(i) over the list into first[]; their sum, or -1 where
-// it is more than the pool has.
-template <class F>
-__device__ int sum_needs(int n, int n_pages, int *first, long long *lds, F need) {
+// What a call over n entries needs: need(i, bad) pages for entry i (and error
+// bits). Takes the pages (list[]) if nothing is wrong, with the prefix sums of the
+// needs in first[]. Returns their number, or -1 with the error bits set.
+// late(i): whether entry i is wrong now that all have been looked at.
+template <class F, class L>
+__device__ int decide(const mhip_page_dims &s, const mhip_pages &p, Desk &d, int n, int *&first,
+                      int *&list, F need, L late) {
+    const Plan pl = plan_of(p.plan, s.n_pages);
+    const int from = max(0, min(p.state[ST_HINT], s.n_pages));
+    const unsigned is = free_mask(s, p, from);
+    for (int i = threadIdx.x; i < (s.max_seqs + 31) / 32; i += NT) d.seen[i] = 0;
+    if (threadIdx.x == 0) d.bad = 0;
+    __syncthreads();
+    first = n <= NT ? d.first : pl.first;
     long long run = 0;
     for (int base = 0; base < n; base += NT) {
         const int i = base + threadIdx.x;
         long long all;
-        const long long x = scan(i < n ? need(i) : 0, &all, lds);
+        int bad = 0;
+        const long long mine = i < n ? need(i, bad) : 0;
+        if (bad) atomicOr(&d.bad, bad);
+        const long long x = scan(bad ? 0 : mine, &all, d.sums);
         if (i < n) first[i] = (int)min(run + x, (long long)1 << 30);
         run += all;
     }
+    for (int i = threadIdx.x; i < n; i += NT)
+        if (late(i)) atomicOr(&d.bad, MHIP_PAGES_BAD);
     __syncthreads();
-    return run > n_pages ? -1 : (int)run;
+    int err = d.bad;
+    list = run <= NT ? d.list : pl.dst;
+    if (!err && (run > s.n_pages || !take_free(s, p, (int)run, list, from, is, d.sums)))
+        err = MHIP_PAGES_NO_SPACE;
+    if (err && threadIdx.x == 0) atomicOr(&p.state[ST_BITS], err);
+    return err ? -1 : (int)run;
+}
+
+// Marks slot q as named by the list; whether it was already.
+__device__ inline bool mark(Desk &d, int q) {
+    return atomicOr(&d.seen[q >> 5], 1u << (q & 31)) >> (q & 31) & 1;
 }
 
 __global__ __launch_bounds__(NT) void k_extend(mhip_page_dims s, mhip_pages p, const int *seqs,
                                                const int *count, int n) {
-    __shared__ unsigned seen[SEQ_WORDS];
-    __shared__ long long lds[NT / 64];
-    __shared__ int bad;
-    const Plan pl = plan_of(p.plan, s.n_pages);
-    for (int i = threadIdx.x; i < SEQ_WORDS; i += NT) seen[i] = 0;
-    if (threadIdx.x == 0) bad = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += NT) {
+    __shared__ Desk d;
+    int *first, *list;
+    const int want = decide(s, p, d, n, first, list, [&](int i, int &bad) {
         const int q = seqs[i], k = count ? count[i] : 1;
-        if ((unsigned)q >= (unsigned)s.max_seqs || k < 0 || p.len[q] < 0 ||
-            (atomicOr(&seen[q >> 5], 1u << (q & 31)) >> (q & 31) & 1))
-            atomicOr(&bad, MHIP_PAGES_BAD);
-        else if ((long long)p.len[q] + k > (long long)s.max_blocks * s.page)
-            atomicOr(&bad, MHIP_PAGES_NO_SPACE);
-    }
-    __syncthreads();
-    int err = bad;
-    int want = 0;
-    if (!err) {
-        want = sum_needs(n, s.n_pages, pl.first, lds, [&](int i) {
-            const int l = p.len[seqs[i]], k = count ? count[i] : 1;
-            return (long long)(blocks_of(l + k, s.page) - blocks_of(l, s.page));
-        });
-        if (want < 0 || !take_free(s, p, want, pl.dst, lds)) err = MHIP_PAGES_NO_SPACE;
-    }
-    if (err) {
-        if (threadIdx.x == 0) atomicOr(&p.state[ST_BITS], err);
-        return;
-    }
+        if ((unsigned)q >= (unsigned)s.max_seqs || k < 0 || mark(d, q)) {
+            bad = MHIP_PAGES_BAD;
+            return 0LL;
+        }
+        const int l = p.len[q];
+        if (n <= NT) {
+            d.slot[i] = q;
+            d.len[i] = l;
+        }
+        if (l < 0) bad = MHIP_PAGES_BAD;
+        else if ((long long)l + k > (long long)s.max_blocks * s.page) bad = MHIP_PAGES_NO_SPACE;
+        return bad ? 0LL : (long long)(blocks_of(l + k, s.page) - blocks_of(l, s.page));
+    }, [](int) { return false; });
+    if (want < 0) return;
     for (int x = threadIdx.x; x < want; x += NT) {
-        const int i = entry_of(pl.first, n, x), q = seqs[i], g = pl.dst[x];
-        const int b = blocks_of(p.len[q], s.page) + (x - pl.first[i]);
+        const int i = entry_of(first, n, x), q = n <= NT ? d.slot[i] : seqs[i], g = list[x];
+        const int b = blocks_of(n <= NT ? d.len[i] : p.len[q], s.page) + (x - first[i]);
         p.table[(size_t)q * s.max_blocks + b] = g;
         p.refs[g] = 1;
         if (x == want - 1) p.state[ST_HINT] = g + 1;
     }
-    __syncthreads();  // every length has been read
-    for (int i = threadIdx.x; i < n; i += NT) p.len[seqs[i]] += count ? count[i] : 1;
+    if (n > NT) __syncthreads();  // every length has been read
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const int q = n <= NT ? d.slot[i] : seqs[i];
+        p.len[q] = (n <= NT ? d.len[i] : p.len[q]) + (count ? count[i] : 1);
+    }
 }
 
 __global__ __launch_bounds__(NT) void k_fork_plan(mhip_page_dims s, mhip_pages p, const int *src,
                                                   const int *dst, int n, int deep) {
-    __shared__ unsigned seen[SEQ_WORDS];
-    __shared__ long long lds[NT / 64];
-    __shared__ int bad;
+    __shared__ Desk d;
     const Plan pl = plan_of(p.plan, s.n_pages);
-    for (int i = threadIdx.x; i < SEQ_WORDS; i += NT) seen[i] = 0;
-    if (threadIdx.x == 0) bad = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += NT) {
+    int *first, *list;
+    const int want = decide(s, p, d, n, first, list, [&](int i, int &bad) {
         const int a = src[i], b = dst[i];
         if ((unsigned)a >= (unsigned)s.max_seqs || (unsigned)b >= (unsigned)s.max_seqs ||
-            p.len[b] != 0 || (atomicOr(&seen[b >> 5], 1u << (b & 31)) >> (b & 31) & 1) ||
-            p.len[a] < 0 || p.len[a] > (long long)s.max_blocks * s.page)
+            mark(d, b)) {
             bad = MHIP_PAGES_BAD;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n && !bad; i += NT)
-        if (seen[src[i] >> 5] >> (src[i] & 31) & 1) bad = MHIP_PAGES_BAD;
-    __syncthreads();
-    int err = bad, want = 0;
-    if (!err) {
-        want = sum_needs(n, s.n_pages, pl.first, lds, [&](int i) {
-            const int l = p.len[src[i]];
-            return (long long)(deep ? blocks_of(l, s.page) : l % s.page != 0);
-        });
-        if (want < 0 || !take_free(s, p, want, pl.dst, lds)) err = MHIP_PAGES_NO_SPACE;
-    }
+            return 0LL;
+        }
+        const int l = p.len[a], lb = p.len[b];
+        if (n <= NT) {
+            d.slot[i] = a;
+            d.len[i] = l;
+        }
+        if (lb != 0 || l < 0 || l > (long long)s.max_blocks * s.page) bad = MHIP_PAGES_BAD;
+        return bad ? 0LL : (long long)(deep ? blocks_of(l, s.page) : l % s.page != 0);
+    }, [&](int i) {  // a source that is also a destination
+        const int a = src[i];
+        return (unsigned)a < (unsigned)s.max_seqs && (d.seen[a >> 5] >> (a & 31) & 1);
+    });
     if (threadIdx.x == 0) {
-        pl.head[PL_PAIRS] = err ? 0 : want;
-        pl.head[PL_OK] = !err;
-        if (err) atomicOr(&p.state[ST_BITS], err);
+        pl.head[PL_PAIRS] = max(want, 0);
+        pl.head[PL_OK] = want >= 0;
     }
-    if (err) return;
     for (int x = threadIdx.x; x < want; x += NT) {
-        const int i = entry_of(pl.first, n, x), a = src[i], l = p.len[a], g = pl.dst[x];
-        const int b = deep ? x - pl.first[i] : l / s.page;
+        const int i = entry_of(first, n, x), g = list[x];
+        const int a = n <= NT ? d.slot[i] : src[i], l = n <= NT ? d.len[i] : p.len[a];
+        const int b = deep ? x - first[i] : l / s.page;
         pl.src[x] = p.table[(size_t)a * s.max_blocks + b];
+        pl.dst[x] = g;
         pl.rows[x] = min(s.page, l - b * s.page);
         p.table[(size_t)dst[i] * s.max_blocks + b] = g;
         p.refs[g] = 1;
@@ -343,32 +371,43 @@ __global__ __launch_bounds__(256) void k_free(mhip_page_dims s, mhip_pages p, co
     }
 }
 
-// A thread per 16-byte piece of the rows: keys' pieces, then values'.
+// A thread per 16-byte piece of the rows (keys' pieces, then values'):
+// gridDim.y workgroups share a row, or one takes several (`each`).
 __global__ __launch_bounds__(256) void k_write(mhip_page_dims s, mhip_pages p, int layer,
-                                               const int *seqs, const int *count, int n,
+                                               const int *seqs, const int *count, int rows,
                                                int max_count, const uint4 *k, const uint4 *v,
-                                               size_t step, int unit) {
-    const size_t pieces = (size_t)s.n_kv_heads * unit;  // of one row
-    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const size_t row = t / (2 * pieces);
-    const unsigned x = (unsigned)(t % (2 * pieces));
-    const int i = (int)(row / max_count), j = (int)(row % max_count);
-    if (i >= n) return;
+                                               size_t step, int unit, int each) {
+    const unsigned pieces = (unsigned)s.n_kv_heads * unit;  // of one array's row
+    unsigned x, row;
+    if (each > 1) {
+        const unsigned in = threadIdx.x / (2 * pieces);
+        if (in >= (unsigned)each) return;
+        row = blockIdx.x * each + in;
+        x = threadIdx.x - in * 2 * pieces;
+    } else {
+        row = blockIdx.x;
+        x = blockIdx.y * 256 + threadIdx.x;
+    }
+    if (row >= (unsigned)rows || x >= 2 * pieces) return;
+    const int i = max_count == 1 ? row : row / max_count, j = max_count == 1 ? 0 : row % max_count;
+    const unsigned y = x < pieces ? x : x - pieces;
+    // (the row's bytes are in the caller's arrays whether its slot is right or not)
+    const uint4 piece = (x < pieces ? k : v)[(size_t)row * step + y];
     const int q = seqs[i], m = count ? count[i] : max_count;
     if (j >= m) return;
     int g = -1;
     const int pos = (unsigned)q < (unsigned)s.max_seqs ? p.len[q] - m + j : -1;
-    if (pos >= 0 && pos / s.page < s.max_blocks && m <= max_count)
-        g = p.table[(size_t)q * s.max_blocks + pos / s.page];
+    const int lp = __builtin_ctz(s.page);
+    if (pos >= 0 && pos >> lp < s.max_blocks && m <= max_count)
+        g = p.table[(size_t)q * s.max_blocks + (pos >> lp)];
     if ((unsigned)g >= (unsigned)s.n_pages) {
         if (x == 0) atomicOr(&p.state[ST_BITS], MHIP_PAGES_BAD);
         return;
     }
-    const unsigned y = x % (unsigned)pieces, h = y / unit, c = y % unit;
-    const size_t to = ((((size_t)layer * s.n_pages + g) * s.n_kv_heads + h) * s.page +
-                       pos % s.page) * unit + c;
-    if (x < pieces) ((uint4 *)p.k)[to] = k[row * step + y];
-    else ((uint4 *)p.v)[to] = v[row * step + y];
+    const unsigned h = y / unit, c = y % unit;
+    const size_t to = (((((size_t)layer * s.n_pages + g) * s.n_kv_heads + h) << lp) +
+                       (pos & (s.page - 1))) * unit + c;
+    ((uint4 *)(x < pieces ? p.k : p.v))[to] = piece;
 }
 
 __global__ __launch_bounds__(256) void k_clear(mhip_page_dims s, mhip_pages p) {
@@ -505,13 +544,15 @@ int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, 
     if (!d_k || !d_v) return mhip::fail(c, "pages write: a null argument");
     if (((uintptr_t)d_k | (uintptr_t)d_v) % 16 || (size_t)ld * esz % 16)
         return mhip::fail(c, "pages write: rows must start on 16 bytes");
-    const size_t threads = (size_t)n * max_count * 2 * (width * esz / 16);
-    if (threads / 256 >= (size_t)1 << 31)
+    if ((long long)n * max_count >= 1 << 30)
         return mhip::fail(c, "pages write: %d x %d rows in one call", n, max_count);
     if (mhip::use_device(c)) return -1;
-    k_write<<<mhip::blocks_for(threads, 256), 256, 0, c->stream>>>(
-        *s, *p, layer, d_seqs, d_count, n, max_count, (const uint4 *)d_k, (const uint4 *)d_v,
-        (size_t)ld * esz / 16, s->head_dim * esz / 16);
+    const int unit = s->head_dim * esz / 16, pieces = 2 * s->n_kv_heads * unit, rows = n * max_count;
+    const int each = pieces <= 128 ? 256 / pieces : 1;
+    const dim3 grid(mhip::blocks_for(rows, each), (pieces + 255) / 256);
+    k_write<<<grid, 256, 0, c->stream>>>(*s, *p, layer, d_seqs, d_count, rows, max_count,
+                                         (const uint4 *)d_k, (const uint4 *)d_v,
+                                         (size_t)ld * esz / 16, unit, each);
     return mhip::check_launch(c, "pages write");
 }
 
