@@ -432,19 +432,24 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
 // x from x itself, unscaled and whole -- bf16 codes for a bf16 product, which
 // cost twice the instructions that fp16 ones do, shared by the TT tiles of 16 tokens
 // -- and fp32 x from the workspace.
-template <class T, int G, bool WHOLE, int TT>
+template <class T, int G, bool WHOLE, int TT, int RT>
 __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8_t *w,
                                                  const uint16_t *scales, int rows, int cols, int n,
                                                  const uint8_t *ws, const T *x, size_t ldx) {
     constexpr bool split = sizeof(T) == 4, bf = std::is_same<T, __bf16>::value;
     constexpr int GC = CHUNK / G, WK = 8;
-    __shared__ float sum[(WK - 1) * TT * 4 * 64];
+    __shared__ float sum[WK * RT * TT * 4 * 64];
     const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, lr = lane & 15, tg = blockIdx.y, nt = min(TG, n - tg * TG);
     const int nchunk = (cols + CHUNK - 1) / CHUNK, nblock = cols / 32, ngroup = cols / G;
-    const size_t row = min((int)blockIdx.x * 16 + lr, rows - 1);
-    const uint8_t *wr = w + row * (cols / 2);
-    const uint16_t *sr = scales + row * ngroup;
+    const uint8_t *wr[RT];
+    const uint16_t *sr[RT];
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+        const size_t row = min(((int)blockIdx.x * RT + i) * 16 + lr, rows - 1);
+        wr[i] = w + row * (cols / 2);
+        sr[i] = scales + row * ngroup;
+    }
     const Tokens l = tokens_of(split ? MHIP_F32 : MHIP_F16, cols, n);
     const uint8_t *xg = ws + (size_t)tg * l.group;
     const float *fg = (const float *)(xg + l.operands);
@@ -455,100 +460,123 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
         from[t] = split ? xg + tok * 64 + g * 16 : (const uint8_t *)(x + (size_t)(tg * TG + tok) * ldx + g * 8);
     }
     const size_t step = split ? (size_t)2 * nt * 64 : 64;  // bytes from a block of 32 columns to the next
-    f4 total[TT];
+    f4 total[RT][TT];
 #pragma unroll
-    for (int t = 0; t < TT; t++) total[t] = (f4){0, 0, 0, 0};
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int t = 0; t < TT; t++) total[i][t] = (f4){0, 0, 0, 0};
     for (int chunk = wk; chunk < nchunk; chunk += WK) {
-        unsigned q[2][4];
+        unsigned q[RT][2][4];
+        float sc[RT][GC];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            int block = chunk * (CHUNK / 32) + 2 * g + h;
-            if constexpr (!WHOLE) block = min(block, nblock - 1);
-            *(u4 *)q[h] = *(const u4 *)(wr + (size_t)block * 16);
+        for (int i = 0; i < RT; i++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                int block = chunk * (CHUNK / 32) + 2 * g + h;
+                if constexpr (!WHOLE) block = min(block, nblock - 1);
+                *(u4 *)q[i][h] = *(const u4 *)(wr[i] + (size_t)block * 16);
+            }
+            uint16_t raw[GC];
+            if constexpr (WHOLE) {
+                using words = typename Words<GC / 2>::type;
+                *(words *)raw = *(const words *)(sr[i] + chunk * GC);
+            } else {
+#pragma unroll
+                for (int j = 0; j < GC; j++) raw[j] = sr[i][min(chunk * GC + j, ngroup - 1)];
+            }
+#pragma unroll
+            for (int j = 0; j < GC; j++) sc[i][j] = (float)__builtin_bit_cast(_Float16, raw[j]);
+            blocks_from_lanes(q[i][0]);
+            blocks_from_lanes(q[i][1]);
         }
-        float sc[GC];
-        uint16_t raw[GC];
-        if constexpr (WHOLE) {
-            using words = typename Words<GC / 2>::type;
-            *(words *)raw = *(const words *)(sr + chunk * GC);
-        } else {
-#pragma unroll
-            for (int j = 0; j < GC; j++) raw[j] = sr[min(chunk * GC + j, ngroup - 1)];
-        }
-#pragma unroll
-        for (int j = 0; j < GC; j++) sc[j] = (float)__builtin_bit_cast(_Float16, raw[j]);
-        blocks_from_lanes(q[0]);
-        blocks_from_lanes(q[1]);
         const int b0 = chunk * (CHUNK / 32), blocks = nblock - b0;
-        f4 part[TT], hi[TT], lo[TT];
+        // the tokens' operands of the next blocks on their way
+        constexpr int AHEAD = split ? 2 : 4;
+        u4 xa[AHEAD][TT], xb[AHEAD][TT];
+        auto fetch = [&](int j) {
+            const int block = WHOLE ? b0 + j : min(b0 + j, nblock - 1);
 #pragma unroll
-        for (int t = 0; t < TT; t++) part[t] = (f4){0, 0, 0, 0};
+            for (int t = 0; t < TT; t++) {
+                const uint8_t *at = from[t] + (size_t)block * step;
+                xa[j % AHEAD][t] = *(const u4 *)at;
+                if constexpr (split) xb[j % AHEAD][t] = *(const u4 *)(at + (size_t)nt * 64);
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) fetch(j);
+        f4 part[RT][TT], hi[RT][TT], lo[RT][TT];
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int t = 0; t < TT; t++) part[i][t] = (f4){0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < CHUNK / 32; j++) {
             if (WHOLE || j < blocks) {
-                const unsigned code = q[j & 1][j >> 1];
+                using weights = std::conditional_t<bf, b8, h8>;
+                weights b[RT];
+#pragma unroll
+                for (int i = 0; i < RT; i++) {
+                    if constexpr (bf) b[i] = codes_bf(q[i][j & 1][j >> 1]);
+                    else b[i] = codes(q[i][j & 1][j >> 1]);
+                }
                 const bool begin = j % (G / 32) == 0, end = (j + 1) % (G / 32) == 0;
 #pragma unroll
                 for (int t = 0; t < TT; t++) {
-                    const uint8_t *at = from[t] + (size_t)(b0 + j) * step;
-                    const u4 a = *(const u4 *)at;
-                    const f4 z = {0, 0, 0, 0}, c = begin ? z : hi[t];
-                    if constexpr (bf) {
-                        hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), codes_bf(code), c, 0, 0, 0);
-                    } else if constexpr (split) {
-                        const h8 b = codes(code);
-                        hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), b, c, 0, 0, 0);
-                        lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8 *)(at + (size_t)nt * 64), b,
-                                                                       begin ? z : lo[t], 0, 0, 0);
-                    } else {
-                        // column k of an eight next to column k + 4, as codes() has them
-                        const u4 p = {__builtin_amdgcn_perm(a[2], a[0], 0x05040100), __builtin_amdgcn_perm(a[2], a[0], 0x07060302),
-                                      __builtin_amdgcn_perm(a[3], a[1], 0x05040100), __builtin_amdgcn_perm(a[3], a[1], 0x07060302)};
-                        hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, p), codes(code), c, 0, 0, 0);
-                    }
-                    if (end) {
+                    u4 a = xa[j % AHEAD][t];
+                    const u4 a2 = xb[j % AHEAD][t];
+                    if constexpr (!split && !bf)  // column k of an eight next to column k + 4, as codes() has them
+                        a = (u4){__builtin_amdgcn_perm(a[2], a[0], 0x05040100), __builtin_amdgcn_perm(a[2], a[0], 0x07060302),
+                                 __builtin_amdgcn_perm(a[3], a[1], 0x05040100), __builtin_amdgcn_perm(a[3], a[1], 0x07060302)};
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            float v = hi[t][r];
-                            if constexpr (split) v = __builtin_fmaf(lo[t][r], 0x1p-11f, v);
-                            part[t][r] = __builtin_fmaf(sc[j / (G / 32)], v, part[t][r]);
+                    for (int i = 0; i < RT; i++) {
+                        const f4 z = {0, 0, 0, 0}, c = begin ? z : hi[i][t];
+                        if constexpr (bf)
+                            hi[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), b[i], c, 0, 0, 0);
+                        else
+                            hi[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), b[i], c, 0, 0, 0);
+                        if constexpr (split)
+                            lo[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a2), b[i],
+                                                                              begin ? z : lo[i][t], 0, 0, 0);
+                        if (end) {
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                float v = hi[i][t][r];
+                                if constexpr (split) v = __builtin_fmaf(lo[i][t][r], 0x1p-11f, v);
+                                part[i][t][r] = __builtin_fmaf(sc[i][j / (G / 32)], v, part[i][t][r]);
+                            }
                         }
                     }
                 }
             }
+            if (j + AHEAD < CHUNK / 32) fetch(j + AHEAD);
+            __builtin_amdgcn_sched_barrier(0x78f);  // (all but memory reads may pass)
         }
 #pragma unroll
         for (int t = 0; t < TT; t++) {
-            if constexpr (split) {  // back to x's own scale
-                const f4 back = *(const f4 *)(fg + (size_t)(chunk * CHUNK / SEG) * TG + t * 16 + g * 4);
+            f4 back = {1.0f, 1.0f, 1.0f, 1.0f};  // to x's own scale
+            if constexpr (split) back = *(const f4 *)(fg + (size_t)(chunk * CHUNK / SEG) * TG + t * 16 + g * 4);
 #pragma unroll
-                for (int r = 0; r < 4; r++) total[t][r] = __builtin_fmaf(part[t][r], back[r], total[t][r]);
-            } else {
-                total[t] += part[t];
-            }
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) total[i][t][r] = __builtin_fmaf(part[i][t][r], back[r], total[i][t][r]);
         }
     }
-    // the column shares' sums, added in their order
+    // the column shares' sums, added in their order, some by each wavefront
+    constexpr int ALL = RT * TT * 4;
 #pragma unroll
-    for (int t = 0; t < TT; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (wk > 0) sum[((wk - 1) * TT * 4 + t * 4 + r) * 64 + lane] = total[t][r];
-    __syncthreads();
-    if (wk > 0) return;
-    for (int k = 0; k < WK - 1; k++)
+    for (int i = 0; i < RT; i++)
 #pragma unroll
         for (int t = 0; t < TT; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) total[t][r] += sum[(k * TT * 4 + t * 4 + r) * 64 + lane];
-    const int at = blockIdx.x * 16 + lr;
+            for (int r = 0; r < 4; r++) sum[(wk * ALL + (i * TT + t) * 4 + r) * 64 + lane] = total[i][t][r];
+    __syncthreads();
+    for (int y = wk; y < ALL; y += WK) {
+        float v = 0.0f;
 #pragma unroll
-    for (int t = 0; t < TT; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int tok = t * 16 + 4 * g + r;
-            if (at < rows && tok < nt) put(out + (size_t)(tg * TG + tok) * ldo + at, total[t][r]);
-        }
+        for (int k = 0; k < WK; k++) v += sum[(k * ALL + y) * 64 + lane];
+        const int at = (blockIdx.x * RT + y / (TT * 4)) * 16 + lr, tok = y / 4 % TT * 16 + 4 * g + y % 4;
+        if (at < rows && tok < nt) put(out + (size_t)(tg * TG + tok) * ldo + at, v);
+    }
 }
 
 // One thread a group (weights are quantized once, when a model is loaded).
@@ -641,8 +669,14 @@ int many_tokens(mhip_ctx *c, int type, T *out, int ldo, const void *w, const voi
         if (mhip::check_launch(c, "matvec_q4 tokens")) return -1;
     }
     if (many) return launch<T, G, WHOLE, 0, TT, 4, 2, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
-    k_q4_wide<T, G, WHOLE, TT><<<dim3((rows + 15) / 16, (n + TG - 1) / TG), 512, 0, c->stream>>>(
-        out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows, cols, n, (const uint8_t *)ws, x, ldx);
+    auto wide = [&](auto k, int rt) {
+        k<<<dim3((rows + 16 * rt - 1) / (16 * rt), (n + TG - 1) / TG), 512, 0, c->stream>>>(
+            out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows, cols, n, (const uint8_t *)ws, x, ldx);
+    };
+    // two tiles of rows a workgroup where one each would be more than one per CU
+    // (64 tokens, bf16, 4096 rows: 10.8 us, two tiles 13.1; 8192 rows: 19.6 and 13.8)
+    if (TT > 1 && rows > 256 * 16) wide(k_q4_wide<T, G, WHOLE, TT, 2>, 2);
+    else wide(k_q4_wide<T, G, WHOLE, TT, 1>, 1);
     return mhip::check_launch(c, "matvec_q4");
 }
 
