@@ -541,15 +541,16 @@ int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * Row i * max_count + j of d_q ([n_heads][head_dim] values of the cache's
  * type, rows ldq values apart) is token j of slot d_seqs[i], at position
  * t = len - d_count[i] + j (d_count NULL: max_count each); it attends to its
- * slot's positions 0 .. t: softmax(scale q.k) v per query head (scale > 0),
- * n_heads a multiple of n_kv_heads. Rows past d_count[i], and rows of an empty slot, are
+ * slot's positions 0 .. t: softmax(scale q.k) v per query head (scale from
+ * 2^-64 to 2^64), n_heads a multiple of n_kv_heads. Rows past d_count[i], and rows of an empty slot, are
  * zeros in d_out (rows ldo values apart).
  *
  * The slots may share their first `prefix` tokens (0: they do not): those
  * are read from slot prefix_seq's pages, once for the whole batch instead of
  * once per slot, so slots that are a fork of prefix_seq or hold the same
  * tokens give the same result as without. A slot shorter than the prefix
- * sees the part that it has. max_len: no slot of the list is longer (the
+ * sees the part that it has; a prefix longer than prefix_seq's slot is an error
+ * bit. max_len: no slot of the list is longer (the
  * work is sized for it; a longer slot is an error bit and its row is NaN).
  * d_q and d_out are 16-byte aligned as their rows' steps are. d_ws:
  * mhip_attention_shared_ws_bytes() bytes, 256-byte aligned, of one call at a
@@ -569,7 +570,7 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
  * weights in groups of `group` (32, 64 or 128, dividing cols): weight =
  * scale * code, code -8 .. 7 in two's complement. d_codes[rows][cols/2]: the
  * even column in the low four bits (16-byte aligned); d_scales
- * [rows][cols/group] in fp16. */
+ * [rows][cols/group] in fp16. rows <= 2^30, cols <= 2^24. */
 /* Codes and scales of fp32 weights: scale = max|w| / 7 rounded to fp16 (at
  * most 65504), code = the nearest integer of w / scale, kept in [-8, 7] (0 where
  * the scale rounds to 0). */

@@ -92,8 +92,8 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
     const int esz = mhip::type_bytes(s->type);
     if (ldq < n_heads * s->head_dim || ldo < n_heads * s->head_dim)
         return mhip::fail(c, "%s: rows %d and %d apart (width %d)", what, ldq, ldo, n_heads * s->head_dim);
-    if (!(scale > 0.0f) || !(scale * 1.44269504f < __builtin_inff()))
-        return mhip::fail(c, "%s: scale %g is not a positive number", what, scale);
+    if (!(scale >= 0x1p-64f && scale <= 0x1p64f))
+        return mhip::fail(c, "%s: scale %g outside [2^-64, 2^64]", what, scale);
     if (!d_q || !d_out || !d_seqs || !d_ws) return mhip::fail(c, "%s: a null argument", what);
     if (((uintptr_t)d_q | (uintptr_t)d_out) % 16 || (size_t)ldq * esz % 16 || (size_t)ldo * esz % 16 ||
         (uintptr_t)d_ws % 256)

@@ -612,7 +612,7 @@ __global__ __launch_bounds__(256) void k_dequantize_q4(const uint8_t *codes, con
 
 int check_q4(mhip_ctx *c, const char *what, const void *d_codes, const void *d_scales, int rows,
              int cols, int group) {
-    if (rows < 0 || cols < 0 || (group != 32 && group != 64 && group != 128) || cols % group)
+    if (rows < 0 || rows > 1 << 30 || cols < 0 || cols > 1 << 24 || (group != 32 && group != 64 && group != 128) || cols % group)
         return mhip::fail(c, "%s: %d rows of %d in groups of %d (32, 64 or 128, dividing the row)",
                           what, rows, cols, group);
     if (rows && cols && (!d_codes || !d_scales)) return mhip::fail(c, "%s: a null argument", what);
@@ -756,7 +756,7 @@ int mhip_matvec_q4(mhip_ctx *c, int type, void *d_out, int ldo, const void *d_co
     if ((uintptr_t)d_x % 16 || (size_t)ldx * esz % 16 || (uintptr_t)d_out % esz ||
         (uintptr_t)d_ws % 256)
         return mhip::fail(c, "matvec_q4: x rows must start on 16 bytes, the workspace on 256");
-    if (n > 65535 * TG || (cols + SEG - 1) / SEG > 65535)
+    if (n > 65535 * TG)
         return mhip::fail(c, "matvec_q4: %d tokens of %d columns in one call", n, cols);
     if (mhip::use_device(c)) return -1;
     if (type == MHIP_F32)

@@ -188,7 +188,8 @@ def attention_tolerance(q, k, v, o, scale, t, parts=64):
         return tol
     g = q.shape[0] // kv
     for h in range(q.shape[0]):
-        size = scale * (np.abs(k[:, h // g]) @ np.abs(q[h])).max()
+        with np.errstate(all="ignore"):  # (rows that are not finite are not compared by it)
+            size = scale * (np.abs(k[:, h // g]) @ np.abs(q[h])).max()
         e = 2 * (hd + 4) * u * size + 2.0 ** -21 + (n + 2 * parts + 16) * u
         weight = 0.0 if t == M.MHIP_F32 else 2 * eps / 2
         tol[h] = (2 * e + weight) * np.abs(v[:, h // g]).max(0) + eps / 2 * np.abs(o[h])

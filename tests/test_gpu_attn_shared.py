@@ -319,6 +319,128 @@ def test_bad_pages_and_slots(g):
         c.close()
 
 
+def test_a_prefix_longer_than_its_slot(g):
+    rng = np.random.default_rng(14)
+    c = Cache(g, n_layers=1, n_kv_heads=1, head_dim=64, max_blocks=10, max_seqs=3, n_pages=40)
+    try:
+        fill(c, [40, 90], 0, rng)
+        q = rng.standard_normal((1, 64))
+        got, bits = run(c, q, 1, [1], None, 1, 64, 100, 0.125)
+        assert bits == M.MHIP_PAGES_BAD
+        got, bits = run(c, q, 1, [1], None, 1, 64, 100, 0.125, prefix_seq=1)
+        assert bits == 0
+        rows, tol = want(c, q, 1, [1], None, 1, 0.125)
+        close(got, rows, tol)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -64, 2.0 ** -20, 4.0, 2.0 ** 64])
+def test_scales(g, scale):
+    """From one that makes all tokens equal to one that leaves the largest score
+    alone (scores of small whole numbers, exact in fp32)."""
+    rng = np.random.default_rng(15)
+    c = Cache(g, n_layers=1, n_kv_heads=1, head_dim=16, max_blocks=20, max_seqs=2, n_pages=40)
+    try:
+        fill(c, [300, 130], 100, rng)
+        c.k = rounded(rng.integers(-3, 4, c.k.shape), c.d.type)[1].reshape(c.k.shape)
+        c.load()
+        q = rng.integers(-2, 3, (2, 32)).astype(float)
+        rows, _ = want(c, q, 2, [0, 1], None, 1, scale)
+        got, bits = run(c, q, 2, [0, 1], None, 1, 100, 300, scale)
+        assert bits == 0
+        # weights of 2^-21 each, sums of 300 tokens
+        assert np.abs(got - rows).max() <= np.abs(values(c.v, c.d.type)).max() * (2.0 ** -20 + 400 * 2.0 ** -24)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("t", [M.MHIP_F32, M.MHIP_BF16])
+def test_offsets_beyond_32_bits(g, t):
+    """The last pages of a cache of over 2^32 bytes (and elements' bytes past
+    2^31): written, forked, moved by compaction to the front, and read."""
+    d = M.PageDims(t, 1, 1, 256, 256, 36000 if t else 18000, 4, 3)
+    size, page = esize(t), 256 * 256 * esize(t)
+    assert d.n_pages * page > 1 << 32
+    c, L = M.Pages(g, d), M.lib()
+    rng = np.random.default_rng(16)
+    dt = np.int32 if t == M.MHIP_F32 else np.int16
+    mem = []
+
+    def up(a, dtype=np.int32):
+        mem.append(g.upload(np.ascontiguousarray(a, dtype)))
+        return mem[-1]
+    try:
+        # all pages but the last four are some other program's
+        refs = np.ones(d.n_pages, np.int32)
+        refs[-4:] = 0
+        g.check(L.mhip_h2d(g.h, c.arrays.refs, refs.ctypes.data, refs.nbytes), "h2d")
+        n = 300
+        k, kr = rounded(rng.standard_normal((n, 256)), t)
+        v, vr = rounded(rng.standard_normal((n, 256)), t)
+        q, qr = rounded(rng.standard_normal((1, 256)) * 2, t)
+        c.extend(up([2]), up([n]), 1)
+        c.write(0, up([2]), up([n]), 1, n, up(kr, dt), up(vr, dt), 256)
+        c.fork(up([2]), up([0]), 1)
+        out = up(np.zeros(256), dt)
+        ws = up(np.zeros(c.attention_ws_bytes(1, 1, 1, 256, 400)), np.uint8)
+        want_row = attention(q.reshape(1, 256), k[:, None], v[:, None], 0.06)
+        tol = attention_tolerance(q.reshape(1, 256), k[:, None], v[:, None], want_row, 0.06, t)
+
+        def check(slot, prefix_seq):
+            c.attention(0, 1, up(qr.reshape(1, 256), dt), 256, out, 256, up([slot]), None, 1, 1, prefix_seq, 256, 400,
+                        0.06, ws)
+            got = values(g.download(out, (256,), dt), t).reshape(1, 256)
+            assert (np.abs(got - want_row) <= tol).all()
+        check(2, 2)
+        check(0, 2)
+        assert c.status() == (0, 1)
+        table = g.download(c.arrays.table, (4, 3), np.int32)
+        assert table[2].tolist() == [d.n_pages - 4, d.n_pages - 3, -1]
+        assert table[0].tolist() == [d.n_pages - 4, d.n_pages - 2, -1]
+        refs = g.download(c.arrays.refs, (d.n_pages,), np.int32)
+        refs[:-4] = 0  # the other program is gone
+        g.check(L.mhip_h2d(g.h, c.arrays.refs, refs.ctypes.data, refs.nbytes), "h2d")
+        c.compact()
+        assert g.download(c.arrays.table, (4, 3), np.int32)[[0, 2]].tolist() == [[0, 2, -1], [0, 1, -1]]
+        check(2, 0)
+        check(0, 2)
+        assert c.status() == (0, d.n_pages - 3)
+    finally:
+        for p in mem:
+            g.free(p)
+        c.close()
+
+
+def test_two_contexts_at_once(g):
+    """Two contexts (streams), each with a cache of its own and calls queued in
+    turn without a wait, give what each gives alone."""
+    rng = np.random.default_rng(17)
+    other = M.Gpu()
+    caches = []
+    try:
+        for gpu in (g, other):
+            c = Cache(gpu, type=M.MHIP_F16, n_layers=1, n_kv_heads=2, head_dim=128, max_blocks=40, max_seqs=6,
+                      n_pages=120)
+            caches.append(c)
+            fill(c, [400 + 30 * i for i in range(6)], 350, rng)
+            c.q = rng.standard_normal((6, 8 * 128)) * 2
+            c.dq = c.up(rounded(c.q, c.d.type)[1], c.int)
+            c.out = c.up(np.zeros((6, 1024)), c.int)
+            c.ws = c.up(np.zeros(c.gpu.attention_ws_bytes(8, 6, 1, 350, 600), np.uint8), np.uint8)
+            c.seqs = c.up(np.arange(6))
+        for _ in range(20):
+            for c in caches:
+                c.gpu.attention(0, 8, c.dq, 1024, c.out, 1024, c.seqs, None, 6, 1, 0, 350, 600, 0.09, c.ws)
+        for c in caches:
+            rows, tol = want(c, c.q, 8, range(6), None, 1, 0.09)
+            close(values(c.g.download(c.out, (6, 1024), c.int), c.d.type).reshape(6, 8, 128), rows, tol)
+    finally:
+        for c in caches:
+            c.close()
+        other.close()
+
+
 def test_repeats_and_replays_give_the_same_bits(g):
     """Two calls, and replays of a graph that shares its workspace with a second
     one, agree to the bit."""

@@ -160,3 +160,31 @@ def test_quantize(g, group):
     assert np.array_equal(back, (q.reshape(b.shape) * s).reshape(rows, cols).astype(np.float32))
     off = np.abs(back - w).reshape(b.shape)[3:]
     assert (off <= (0.5 + 7 * 2.0 ** -10) * s[3:]).all()
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_offsets_beyond_32_bits(g, n):
+    """Codes of over 2^32 bytes, zero but for the last rows."""
+    rows, cols, group = (1 << 19) + 3, 16512, 128
+    rng = np.random.default_rng(9)
+    codes, scales = weights(rng, 3, cols, group)
+    x, raw = rounded(rng.standard_normal((n, cols)), M.MHIP_BF16)
+    L = M.lib()
+    size, ssize = rows * (cols // 2), rows * (cols // group) * 2
+    assert size > 1 << 32
+    mem = [g.malloc(size), g.malloc(ssize), g.upload(raw.reshape(n, cols)), g.malloc(n * rows * 2),
+           g.malloc(M.matvec_q4_ws_bytes(M.MHIP_BF16, cols, n))]
+    try:
+        g.check(L.mhip_zero(g.h, mem[0], size), "zero")
+        g.check(L.mhip_zero(g.h, mem[1], ssize), "zero")
+        g.check(L.mhip_h2d(g.h, mem[0] + size - codes.nbytes, codes.ctypes.data, codes.nbytes), "h2d")
+        g.check(L.mhip_h2d(g.h, mem[1] + ssize - scales.nbytes, scales.ctypes.data, scales.nbytes), "h2d")
+        M.matvec_q4(g, M.MHIP_BF16, mem[3], rows, mem[0], mem[1], group, mem[2], cols, rows, cols, n, mem[4])
+        out = values(g.download(mem[3], (n, rows), np.int16), M.MHIP_BF16)
+    finally:
+        for p in mem:
+            g.free(p)
+    assert (out[:, :-3] == 0).all()
+    w = q4_weights(codes, scales, group)
+    o = x @ w.T
+    assert (np.abs(out[:, -3:] - o) <= q4_tolerance(w, x, o, M.MHIP_BF16)).all()

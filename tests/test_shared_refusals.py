@@ -85,7 +85,7 @@ def test_attention():
     for bad in (dict(layer=-1), dict(layer=2), dict(heads=0), dict(heads=3), dict(q=None), dict(q=4104),
                 dict(ldq=255), dict(ldq=260), dict(out=None), dict(out=4098), dict(ldo=240), dict(seqs=None),
                 dict(n=-1), dict(n=5), dict(top=-2), dict(prefix=-1), dict(prefix=65), dict(prefix_seq=-1),
-                dict(prefix_seq=4), dict(max_len=81), dict(max_len=-1), dict(scale=0.0), dict(scale=-1.0),
+                dict(prefix_seq=4), dict(max_len=81), dict(max_len=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=1e-30), dict(scale=1e30),
                 dict(scale=float("nan")), dict(scale=float("inf")), dict(ws=None), dict(ws=4096 + 128)):
         assert L.mhip_attention_shared(None, D, A, *dict(good, **bad).values()) == -1, bad
     for none in (dict(n=0), dict(top=0)):
@@ -103,6 +103,7 @@ def test_rows():
                 ws=4096)
     for bad in (dict(type=3), dict(type=-1), dict(out=None), dict(ldo=63), dict(codes=None), dict(codes=4104),
                 dict(scales=None), dict(scales=4097), dict(group=16), dict(group=0), dict(group=256), dict(x=None),
+                dict(rows=(1 << 30) + 1, ldo=(1 << 30) + 1), dict(cols=(1 << 24) + 32, ldx=(1 << 24) + 32),
                 dict(x=4100), dict(ldx=127), dict(ldx=130), dict(rows=-1), dict(cols=-32), dict(cols=100),
                 dict(cols=0), dict(n=-1), dict(ws=None), dict(ws=4112), dict(out=4098)):
         assert L.mhip_matvec_q4(None, *dict(good, **bad).values()) == -1, bad
