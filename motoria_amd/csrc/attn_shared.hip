@@ -19,7 +19,8 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // keep the CUs busy: 256 workgroups for the prefix (64 x 8000: with 8 parts 41
 // us, 16 parts 33, 32 parts 41) and 256 for the slots (32 unshared slots of up
 // to 8000 tokens: 2 parts 79 us, 8 parts 90; 64 of 300 tokens: 1 part 12 us, 2
-// parts 18; fp32 behind a prefix, whose tiles take longest, fewer). Without a
+// parts 18; fp32 behind a prefix, whose tiles take longest, fewer and longer ones:
+// 16 slots of 400, 26 us in one part each, 29 in two). Without a
 // prefix one part needs no join, so the number is rounded down (200 workgroups
 // or 400: 13.5 and 16.6 us), else up (168 or 336: 19.0 and 16.5). Where
 // a CU holds one workgroup only the two together should not be more than the
@@ -31,7 +32,8 @@ Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int 
     k.stiles = (mc * group + 15) / 16;
     const long long items = (long long)n * s->n_kv_heads * k.stiles;
     long long parts = prefix == 0 ? 256 / items : ((s->type == MHIP_F32 ? 96 : 256) + items - 1) / items;
-    const int most = (rest + 255) / 256, least = (rest + PART_MAX - 1) / PART_MAX;
+    const int shortest = prefix > 0 && s->type == MHIP_F32 ? 512 : 256;
+    const int most = (rest + shortest - 1) / shortest, least = (rest + PART_MAX - 1) / PART_MAX;
     if (parts > most) parts = most;
     if (parts < least) parts = least;
     if (parts < 1) parts = 1;
