@@ -13,8 +13,9 @@ using mhip_shared::TILE;
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // How a call is cut. A part of the prefix serves up to 128 rows (16-bit heads up
-// to 128); tiles of 64 rows do better up to 128 rows in all (16 slots behind 16000 tokens, bf16: 28 us,
-// with tiles of 128 rows 32; 64 slots behind 8000: 35 and 33). Every part's
+// to 128); tiles of 64 rows do better up to 128 rows in all (16 slots behind 16000
+// tokens, bf16: 28 us, with tiles of 128 rows 32; 64 slots behind 8000: 35 and 33).
+// (The times here compare the two sides; the kernel has become faster since.) Every part's
 // results pass through memory once more, so there are only as many as
 // keep the CUs busy: 256 workgroups for the prefix (64 x 8000: with 8 parts 41
 // us, 16 parts 33, 32 parts 41) and 256 for the slots (32 unshared slots of up

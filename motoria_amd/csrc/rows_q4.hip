@@ -11,13 +11,19 @@
 // instruction with fp32 accumulators; with one token 15 of 16 of its columns are idle,
 // which still is faster than the vector units (2.25 instructions a weight).
 //
-// x as fp16 operands: k_q4_tokens scales each token's segment of 1024 columns by
-// a power of two that brings its largest value to [2^14, 2^15). A bf16 value
-// then is an fp16 value (8 bits; exact down to 2^-32 of the largest). An
-// fp32 value is split: hi = fp16(x'), lo = fp16((x' - hi) 2^11), together
+// x as fp16 operands (up to FEW tokens, and many rows): each token's segment of
+// 1024 columns is scaled by a power of two that brings its largest value to [2^14,
+// 2^15). A bf16 value then is an fp16 value (8 bits; exact down to 2^-32 of the
+// largest). An fp32 value is split: hi = fp16(x'), lo = fp16((x' - hi) 2^11), together
 // within 2^-23 of x (a step of fp32's own rounding) down to 2^-29 of the
 // segment's largest value, as lo carries its own exponent; their products
 // are accumulated apart and joined in fp32. fp16 x is taken as it is.
+//
+// Measured (us; bytes of the weights at what a large copy reaches, 4.92 TB/s, in
+// brackets): a head of 151936 x 2048, fp32, groups of 32, one token 40 [36], fp16 with
+// groups of 128 33 [33]; 512 to 4096 x 2048, one token 5, a launch among others being
+// 3.6; 4096 x 2048 in bf16 with 16 tokens 4.9, with 64 tokens 10, where a workgroup
+// waits for 256 KB of operands from L2.
 #include "mhip_internal.h"
 #include <type_traits>
 
