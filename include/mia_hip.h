@@ -507,7 +507,8 @@ int mhip_pages_extend(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * slot (NULL: max_count each): token j < d_count[i] of entry i is row
  * i * max_count + j of d_k and d_v (rows of n_kv_heads * head_dim values, ld
  * values apart, 16-byte aligned as the rows' step is; rows past d_count[i] are
- * in the arrays, but not used). */
+ * in the arrays, but not used). Less than 2^24 rows. A slot twice in the list
+ * is not looked for: its positions get the rows of either entry. */
 int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,
                      const int *d_seqs, const int *d_count, int n, int max_count,
                      const void *d_k, const void *d_v, int ld);
@@ -519,7 +520,7 @@ int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, 
 int mhip_pages_fork(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, const int *d_src,
                     const int *d_dst, int n, int flags);
 /* Empties the slots; pages that no slot holds any more are free. An empty
- * slot, or one twice in the list, is no error. */
+ * slot, or one twice in the list, is no error. n < 2^24. */
 int mhip_pages_free(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, const int *d_seqs,
                     int n);
 /* Moves pages so that the n pages in use are pages 0 .. n - 1: the i-th free
@@ -542,16 +543,17 @@ int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * type, rows ldq values apart) is token j of slot d_seqs[i], at position
  * t = len - d_count[i] + j (d_count NULL: max_count each); it attends to its
  * slot's positions 0 .. t: softmax(scale q.k) v per query head (scale from
- * 2^-64 to 2^64), n_heads a multiple of n_kv_heads. Rows past d_count[i], and rows of an empty slot, are
- * zeros in d_out (rows ldo values apart).
+ * 2^-64 to 2^64), n_heads a multiple of n_kv_heads, n * max_count * n_heads
+ * less than 2^26. Rows past d_count[i], and rows of an empty slot, are zeros in
+ * d_out (rows ldo values apart).
  *
  * The slots may share their first `prefix` tokens (0: they do not): those
  * are read from slot prefix_seq's pages, once for the whole batch instead of
  * once per slot, so slots that are a fork of prefix_seq or hold the same
  * tokens give the same result as without. A slot shorter than the prefix
  * sees the part that it has; a prefix longer than prefix_seq's slot is an error
- * bit. max_len: no slot of the list is longer (the
- * work is sized for it; a longer slot is an error bit and its row is NaN).
+ * bit. max_len: no slot of the list is longer (the work is sized for it; a
+ * longer slot is an error bit and its row is NaN).
  * d_q and d_out are 16-byte aligned as their rows' steps are. d_ws:
  * mhip_attention_shared_ws_bytes() bytes, 256-byte aligned, of one call at a
  * time (0 for invalid arguments). Scores, softmax and sums are fp32; with a
@@ -570,7 +572,7 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
  * weights in groups of `group` (32, 64 or 128, dividing cols): weight =
  * scale * code, code -8 .. 7 in two's complement. d_codes[rows][cols/2]: the
  * even column in the low four bits (16-byte aligned); d_scales
- * [rows][cols/group] in fp16. rows <= 2^30, cols <= 2^24. */
+ * [rows][cols/group] in fp16. rows <= 2^28, cols <= 2^24, rows * cols <= 2^34. */
 /* Codes and scales of fp32 weights: scale = max|w| / 7 rounded to fp16 (at
  * most 65504), code = the nearest integer of w / scale, kept in [-8, 7] (0 where
  * the scale rounds to 0). */
@@ -582,8 +584,10 @@ int mhip_dequantize_q4(mhip_ctx *c, const void *d_codes, const void *d_scales, i
  * (MHIP_F32, ...), rows ldx and ldo values apart (x 16-byte aligned as its
  * rows' step is), sums in fp32. fp32 x enters the products with 22 bits or
  * more of each value's (values 2^29 below the largest of 1024 columns lose
- * further bits); 16-bit x enters whole. d_ws: mhip_matvec_q4_ws_bytes() bytes, 256-byte
- * aligned, of one call at a time (0 for invalid arguments). */
+ * further bits); fp16 x enters whole, and so do bf16 values down to 2^-32 of
+ * the largest of 1024 columns (smaller ones may lose bits). n <= 65535 * 64. d_ws:
+ * mhip_matvec_q4_ws_bytes() bytes, 256-byte aligned, of one call at a time (0
+ * for invalid arguments). */
 size_t mhip_matvec_q4_ws_bytes(int type, int cols, int n);
 int mhip_matvec_q4(mhip_ctx *c, int type, void *d_out, int ldo, const void *d_codes,
                    const void *d_scales, int group, const void *d_x, int ldx, int rows, int cols,

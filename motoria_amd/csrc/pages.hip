@@ -11,8 +11,8 @@
 //
 // Measured (48 layers, 4 heads of 128 in bf16, pages of 16): compaction of 75 pages,
 // 238 MB read and written, 57 us (4.2 TB/s; a large copy reaches 4.92) after a plan
-// of 5.5; 48 forks, 73 MB, 23 us after 6; extend 5.6, a layer's rows of 64 tokens 3.0,
-// where a launch that does nothing is 2.
+// of 5.5; 48 forks, 73 MB, 23 us after 6; extend 5.6, a layer's rows of 64 tokens 3.0
+// (each alone; small launches one after another take 3.6).
 #include "mhip_internal.h"
 
 namespace {
@@ -552,7 +552,7 @@ int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, 
     if (!d_k || !d_v) return mhip::fail(c, "pages write: a null argument");
     if (((uintptr_t)d_k | (uintptr_t)d_v) % 16 || (size_t)ld * esz % 16)
         return mhip::fail(c, "pages write: rows must start on 16 bytes");
-    if ((long long)n * max_count >= 1 << 30)
+    if ((long long)n * max_count >= 1 << 24)  // (a launch holds less than 2^32 threads)
         return mhip::fail(c, "pages write: %d x %d rows in one call", n, max_count);
     if (mhip::use_device(c)) return -1;
     const int unit = s->head_dim * esz / 16, pieces = 2 * s->n_kv_heads * unit, rows = n * max_count;
@@ -584,7 +584,7 @@ int mhip_pages_free(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, c
                     int n) {
     // (a list may name a slot twice, so it may be longer than there are slots)
     if (mhip::check_pages(c, s, p, "pages free")) return -1;
-    if (n < 0 || (n && !d_seqs)) return mhip::fail(c, "pages free: %d entries", n);
+    if (n < 0 || n >= 1 << 24 || (n && !d_seqs)) return mhip::fail(c, "pages free: %d entries", n);
     if (!n) return 0;
     if (mhip::use_device(c)) return -1;
     k_free<<<n, 256, 0, c->stream>>>(*s, *p, d_seqs);

@@ -17,7 +17,8 @@
 // largest). An fp32 value is split: hi = fp16(x'), lo = fp16((x' - hi) 2^11), together
 // within 2^-23 of x (a step of fp32's own rounding) down to 2^-29 of the
 // segment's largest value, as lo carries its own exponent; their products
-// are accumulated apart and joined in fp32. fp16 x is taken as it is.
+// are accumulated apart and joined in fp32. fp16 x is taken as it is. With more tokens
+// and fewer rows 16-bit x of either type is taken as it is (k_q4_wide).
 //
 // Measured (us; bytes of the weights at what a large copy reaches, 4.92 TB/s, in
 // brackets): a head of 151936 x 2048, fp32, groups of 32, one token 40 [36], fp16 with
@@ -618,7 +619,8 @@ __global__ __launch_bounds__(256) void k_dequantize_q4(const uint8_t *codes, con
 
 int check_q4(mhip_ctx *c, const char *what, const void *d_codes, const void *d_scales, int rows,
              int cols, int group) {
-    if (rows < 0 || rows > 1 << 30 || cols < 0 || cols > 1 << 24 || (group != 32 && group != 64 && group != 128) || cols % group)
+    // (a launch holds less than 2^32 threads: up to 8 a row, and one for 8 weights)
+    if (rows < 0 || rows > 1 << 28 || cols < 0 || cols > 1 << 24 || (long long)rows * cols > 1LL << 34 || (group != 32 && group != 64 && group != 128) || cols % group)
         return mhip::fail(c, "%s: %d rows of %d in groups of %d (32, 64 or 128, dividing the row)",
                           what, rows, cols, group);
     if (rows && cols && (!d_codes || !d_scales)) return mhip::fail(c, "%s: a null argument", what);

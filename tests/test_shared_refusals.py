@@ -115,3 +115,24 @@ def test_rows():
     assert L.mhip_quantize_q4(None, None, 4, 128, 32, 16, 16) == -1
     assert L.mhip_dequantize_q4(None, 16, 16, 4, 128, 31, 16) == -1
     assert L.mhip_dequantize_q4(None, 16, 16, 4, 128, 32, None) == -1
+
+
+def test_launches_have_less_than_2_32_threads():
+    L = M.lib()
+    d, a = cache(max_blocks=1 << 22)
+    D, A = ctypes.byref(d), ctypes.byref(a)
+    assert L.mhip_pages_write(None, D, A, 0, 16, None, 4, 1 << 22, 4096, 4096, 128) == -1
+    assert L.mhip_pages_free(None, D, A, 16, 1 << 24) == -1
+    size = lambda top, heads, prefix, longest: L.mhip_attention_shared_ws_bytes(  # noqa: E731
+        D, heads, 2, top, prefix, longest)
+    call = lambda top, heads, prefix, longest: L.mhip_attention_shared(  # noqa: E731
+        None, D, A, 0, heads, 4096, heads * 64, 4096, heads * 64, 16, None, 2, top, 0, prefix, longest, 0.1, 4096)
+    assert size((1 << 23) - 1, 4, 0, 1 << 12) > 0
+    for args in ((1 << 23, 4, 0, 1 << 12), ((1 << 23) - 1, 4, 0, 1 << 26), ((1 << 23) - 1, 4, 1 << 26, 1 << 26)):
+        assert size(*args) == 0 and call(*args) == -1, args
+    rows = (1 << 28) + 1
+    assert L.mhip_matvec_q4(None, 0, 4096, rows, 4096, 4096, 32, 4096, 32, rows, 32, 1, 4096) == -1
+    rows = (1 << 28) - 1  # 2^36 weights
+    assert L.mhip_matvec_q4(None, 0, 4096, rows, 4096, 4096, 32, 4096, 256, rows, 256, 1, 4096) == -1
+    assert L.mhip_dequantize_q4(None, 16, 16, rows, 256, 32, 16) == -1
+    assert L.mhip_quantize_q4(None, 16, rows, 256, 32, 16, 16) == -1
