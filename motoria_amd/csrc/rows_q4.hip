@@ -460,12 +460,18 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
     const Tokens l = tokens_of(split ? MHIP_F32 : MHIP_F16, cols, n);
     const uint8_t *xg = ws + (size_t)tg * l.group;
     const float *fg = (const float *)(xg + l.operands);
-    const uint8_t *from[TT];  // a lane's token row (past the last: the last one's)
+    // A lane's token row (past the last: the last one's). A load of the same half
+    // line (64 bytes) of sixteen rows runs at half the rate, so of two blocks
+    // of 32 columns every other row asks for the second one first, and swaps them
+    // before the products (4096 x 2048, 64 tokens, bf16: 7.0 us, else 10.0).
+    // (Sixteen rows on, addresses are the same in their last 8 bits.)
+    const uint8_t *from[TT];
 #pragma unroll
     for (int t = 0; t < TT; t++) {
         const int tok = min(t * 16 + lr, nt - 1);
         from[t] = split ? xg + tok * 64 + g * 16 : (const uint8_t *)(x + (size_t)(tg * TG + tok) * ldx + g * 8);
     }
+    const bool swap = ((uintptr_t)from[0] >> 6 ^ lr) & 1;
     const size_t step = split ? (size_t)2 * nt * 64 : 64;  // bytes from a block of 32 columns to the next
     f4 total[RT][TT];
 #pragma unroll
@@ -474,7 +480,7 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
         for (int t = 0; t < TT; t++) total[i][t] = (f4){0, 0, 0, 0};
     for (int chunk = wk; chunk < nchunk; chunk += WK) {
         unsigned q[RT][2][4];
-        float sc[RT][GC];
+        uint16_t raw[RT][GC];
 #pragma unroll
         for (int i = 0; i < RT; i++) {
 #pragma unroll
@@ -483,34 +489,40 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
                 if constexpr (!WHOLE) block = min(block, nblock - 1);
                 *(u4 *)q[i][h] = *(const u4 *)(wr[i] + (size_t)block * 16);
             }
-            uint16_t raw[GC];
             if constexpr (WHOLE) {
                 using words = typename Words<GC / 2>::type;
-                *(words *)raw = *(const words *)(sr[i] + chunk * GC);
+                *(words *)raw[i] = *(const words *)(sr[i] + chunk * GC);
             } else {
 #pragma unroll
-                for (int j = 0; j < GC; j++) raw[j] = sr[i][min(chunk * GC + j, ngroup - 1)];
+                for (int j = 0; j < GC; j++) raw[i][j] = sr[i][min(chunk * GC + j, ngroup - 1)];
             }
-#pragma unroll
-            for (int j = 0; j < GC; j++) sc[i][j] = (float)__builtin_bit_cast(_Float16, raw[j]);
-            blocks_from_lanes(q[i][0]);
-            blocks_from_lanes(q[i][1]);
         }
         const int b0 = chunk * (CHUNK / 32), blocks = nblock - b0;
         // the tokens' operands of the next blocks on their way
         constexpr int AHEAD = split ? 2 : 4;
         u4 xa[AHEAD][TT], xb[AHEAD][TT];
         auto fetch = [&](int j) {
-            const int block = WHOLE ? b0 + j : min(b0 + j, nblock - 1);
 #pragma unroll
             for (int t = 0; t < TT; t++) {
-                const uint8_t *at = from[t] + (size_t)block * step;
+                // (from b0 on: the addresses of a whole chunk differ by constants)
+                const int other = split || !swap ? 0 : j & 1 ? -1 : 1;
+                const uint8_t *at = from[t] + (size_t)b0 * step;
+                at += WHOLE ? other * 64 + j * (ptrdiff_t)step : min(j + other, blocks - 1) * (ptrdiff_t)step;
                 xa[j % AHEAD][t] = *(const u4 *)at;
                 if constexpr (split) xb[j % AHEAD][t] = *(const u4 *)(at + (size_t)nt * 64);
             }
         };
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) fetch(j);
+        __builtin_amdgcn_sched_barrier(0x78f);  // (all but memory reads may pass)
+        float sc[RT][GC];
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+#pragma unroll
+            for (int j = 0; j < GC; j++) sc[i][j] = (float)__builtin_bit_cast(_Float16, raw[i][j]);
+            blocks_from_lanes(q[i][0]);
+            blocks_from_lanes(q[i][1]);
+        }
         f4 part[RT][TT], hi[RT][TT], lo[RT][TT];
 #pragma unroll
         for (int i = 0; i < RT; i++)
@@ -518,6 +530,16 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
             for (int t = 0; t < TT; t++) part[i][t] = (f4){0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < CHUNK / 32; j++) {
+            if (!split && j % 2 == 0) {
+#pragma unroll
+                for (int t = 0; t < TT; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const unsigned u = xa[j % AHEAD][t][e], v = xa[(j + 1) % AHEAD][t][e];
+                        xa[j % AHEAD][t][e] = swap ? v : u;
+                        xa[(j + 1) % AHEAD][t][e] = swap ? u : v;
+                    }
+            }
             if (WHOLE || j < blocks) {
                 using weights = std::conditional_t<bf, b8, h8>;
                 weights b[RT];
@@ -682,9 +704,15 @@ int many_tokens(mhip_ctx *c, int type, T *out, int ldo, const void *w, const voi
             out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows, cols, n, (const uint8_t *)ws, x, ldx);
     };
     // two tiles of rows a workgroup where one each would be more than one per CU
-    // (64 tokens, bf16, 4096 rows: 10.8 us, two tiles 13.1; 8192 rows: 19.6 and 13.8)
-    if (TT > 1 && rows > 256 * 16) wide(k_q4_wide<T, G, WHOLE, TT, 2>, 2);
-    else wide(k_q4_wide<T, G, WHOLE, TT, 1>, 1);
+    // (64 tokens, bf16, 6144 x 2048: 12.2 us, two tiles 8.7; 11008 x 4096: 32 and 30), but
+    // not where registers run out (fp32, 33 tokens or more: 11008 x 4096 74 us, two tiles 102)
+    if constexpr (TT == 2 || (TT == 4 && sizeof(T) == 2)) {
+        if (rows > 256 * 16) {
+            wide(k_q4_wide<T, G, WHOLE, TT, 2>, 2);
+            return mhip::check_launch(c, "matvec_q4");
+        }
+    }
+    wide(k_q4_wide<T, G, WHOLE, TT, 1>, 1);
     return mhip::check_launch(c, "matvec_q4");
 }
 
