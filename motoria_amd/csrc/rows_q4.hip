@@ -447,7 +447,9 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
     constexpr int GC = CHUNK / G, WK = 8;
     __shared__ float sum[WK * RT * TT * 4 * 64];
     const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, lr = lane & 15, tg = blockIdx.y, nt = min(TG, n - tg * TG);
+    const int g = lane >> 4, lr = lane & 15;
+    const int t0 = blockIdx.y * TT * 16, nt = min(TT * 16, n - t0);  // this workgroup's tokens
+    const int tg = t0 / TG, of_group = min(TG, n - tg * TG);         // ... in a group of the workspace
     const int nchunk = (cols + CHUNK - 1) / CHUNK, nblock = cols / 32, ngroup = cols / G;
     const uint8_t *wr[RT];
     const uint16_t *sr[RT];
@@ -459,7 +461,7 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
     }
     const Tokens l = tokens_of(split ? MHIP_F32 : MHIP_F16, cols, n);
     const uint8_t *xg = ws + (size_t)tg * l.group;
-    const float *fg = (const float *)(xg + l.operands);
+    const float *fg = (const float *)(xg + l.operands) + t0 % TG;
     // A lane's token row (past the last: the last one's). A load of the same half
     // line (64 bytes) of sixteen rows runs at half the rate, so of two blocks
     // of 32 columns every other row asks for the second one first, and swaps them
@@ -469,10 +471,10 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
 #pragma unroll
     for (int t = 0; t < TT; t++) {
         const int tok = min(t * 16 + lr, nt - 1);
-        from[t] = split ? xg + tok * 64 + g * 16 : (const uint8_t *)(x + (size_t)(tg * TG + tok) * ldx + g * 8);
+        from[t] = split ? xg + (t0 % TG + tok) * 64 + g * 16 : (const uint8_t *)(x + (size_t)(t0 + tok) * ldx + g * 8);
     }
     const bool swap = ((uintptr_t)from[0] >> 6 ^ lr) & 1;
-    const size_t step = split ? (size_t)2 * nt * 64 : 64;  // bytes from a block of 32 columns to the next
+    const size_t step = split ? (size_t)2 * of_group * 64 : 64;  // bytes from a block of 32 columns to the next
     f4 total[RT][TT];
 #pragma unroll
     for (int i = 0; i < RT; i++)
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
                 const uint8_t *at = from[t] + (size_t)b0 * step;
                 at += WHOLE ? other * 64 + j * (ptrdiff_t)step : min(j + other, blocks - 1) * (ptrdiff_t)step;
                 xa[j % AHEAD][t] = *(const u4 *)at;
-                if constexpr (split) xb[j % AHEAD][t] = *(const u4 *)(at + (size_t)nt * 64);
+                if constexpr (split) xb[j % AHEAD][t] = *(const u4 *)(at + (size_t)of_group * 64);
             }
         };
 #pragma unroll
@@ -604,7 +606,7 @@ __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8
 #pragma unroll
         for (int k = 0; k < WK; k++) v += sum[(k * ALL + y) * 64 + lane];
         const int at = (blockIdx.x * RT + y / (TT * 4)) * 16 + lr, tok = y / 4 % TT * 16 + 4 * g + y % 4;
-        if (at < rows && tok < nt) put(out + (size_t)(tg * TG + tok) * ldo + at, v);
+        if (at < rows && tok < nt) put(out + (size_t)(t0 + tok) * ldo + at, v);
     }
 }
 
@@ -699,20 +701,21 @@ int many_tokens(mhip_ctx *c, int type, T *out, int ldo, const void *w, const voi
         if (mhip::check_launch(c, "matvec_q4 tokens")) return -1;
     }
     if (many) return launch<T, G, WHOLE, 0, TT, 4, 2, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    constexpr int WT = TT == 4 && sizeof(T) == 4 ? 2 : TT;
     auto wide = [&](auto k, int rt) {
-        k<<<dim3((rows + 16 * rt - 1) / (16 * rt), (n + TG - 1) / TG), 512, 0, c->stream>>>(
+        k<<<dim3((rows + 16 * rt - 1) / (16 * rt), (n + 16 * WT - 1) / (16 * WT)), 512, 0, c->stream>>>(
             out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows, cols, n, (const uint8_t *)ws, x, ldx);
     };
     // two tiles of rows a workgroup where one each would be more than one per CU
     // (64 tokens, bf16, 6144 x 2048: 12.2 us, two tiles 8.7; 11008 x 4096: 32 and 30), but
     // not where registers run out (fp32, 33 tokens or more: 11008 x 4096 74 us, two tiles 102)
-    if constexpr (TT == 2 || (TT == 4 && sizeof(T) == 2)) {
+    if constexpr (TT > 1) {
         if (rows > 256 * 16) {
-            wide(k_q4_wide<T, G, WHOLE, TT, 2>, 2);
+            wide(k_q4_wide<T, G, WHOLE, WT, 2>, 2);
             return mhip::check_launch(c, "matvec_q4");
         }
     }
-    wide(k_q4_wide<T, G, WHOLE, TT, 1>, 1);
+    wide(k_q4_wide<T, G, WHOLE, WT, 1>, 1);
     return mhip::check_launch(c, "matvec_q4");
 }
 
