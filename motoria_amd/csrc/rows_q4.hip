@@ -11,20 +11,21 @@
 // instruction with fp32 accumulators; with one token 15 of 16 of its columns are idle,
 // which still is faster than the vector units (2.25 instructions a weight).
 //
-// x as fp16 operands (up to FEW tokens, and many rows): each token's segment of
-// 1024 columns is scaled by a power of two that brings its largest value to [2^14,
+// x as fp16 operands (up to FEW tokens; fp32 x; 17 to 32 tokens of 16-bit x with many
+// rows): each token's segment of 1024 columns is scaled by a power of two that brings its largest value to [2^14,
 // 2^15). A bf16 value then is an fp16 value (8 bits; exact down to 2^-32 of the
 // largest). An fp32 value is split: hi = fp16(x'), lo = fp16((x' - hi) 2^11), together
 // within 2^-23 of x (a step of fp32's own rounding) down to 2^-29 of the
 // segment's largest value, as lo carries its own exponent; their products
-// are accumulated apart and joined in fp32. fp16 x is taken as it is. With more tokens
-// and fewer rows 16-bit x of either type is taken as it is (k_q4_wide).
+// are accumulated apart and joined in fp32. fp16 x is taken as it is; elsewhere
+// 16-bit x of either type is (k_q4_wide).
 //
 // Measured (us; bytes of the weights at what a large copy reaches, 4.92 TB/s, in
 // brackets): a head of 151936 x 2048, fp32, groups of 32, one token 40 [36], fp16 with
 // groups of 128 33 [33]; 512 to 4096 x 2048, one token 5, a launch among others being
-// 3.6; 4096 x 2048 in bf16 with 16 tokens 4.9, with 64 tokens 10, where a workgroup
-// waits for 256 KB of operands from L2.
+// 3.6; 4096 x 2048 in bf16 with 16 tokens 4.5, with 64 tokens 7.0, where a workgroup
+// waits for 256 KB of operands from L2; the head with 16 tokens, fp32 81 [36], bf16,
+// groups of 128, 54 [33].
 #include "mhip_internal.h"
 #include <type_traits>
 
@@ -40,7 +41,7 @@ constexpr int SEG = 1024;  // columns that share a token's power of two
 constexpr int TG = 64;     // tokens of one workgroup, at most
 
 // The workspace: per group of TG tokens (nt of them) the operands
-// [cols/32][pieces][nt][32] fp16, in each 32 the order of pair(), then
+// [cols/32][pieces][nt][32] fp16, in each 32 the order of codes(), then
 // [cols/SEG][TG] the factors back.
 struct Tokens {
     size_t operands, factors, group;  // bytes of each, and of a group
@@ -182,9 +183,10 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
                                                      const uint16_t *scales, int rows, int cols,
                                                      int n, int kc, const uint8_t *ws, const T *x,
                                                      size_t ldx, int type) {
-    constexpr bool split = sizeof(T) == 4, pair = split && N > 0;
+    constexpr bool split = sizeof(T) == 4;  // hi and lo of a token: two token rows
+    static_assert(N > 0 || !split, "from the workspace, 16-bit x");
     constexpr int P = split ? 2 : 1, NT = 64 * WR * WK, GC = CHUNK / G;  // groups of a chunk
-    constexpr int TL = N == 1 ? 1 : pair ? 2 : 4;                        // tokens of a lane and tile
+    constexpr int TL = N == 1 ? 1 : split ? 2 : 4;                       // tokens of a lane and tile
     constexpr bool MANY = N > 0 && WK == 1;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
             }
             __syncthreads();
         } else {
-            const Tokens l = tokens_of(split ? MHIP_F32 : MHIP_F16, cols, n);
+            const Tokens l = tokens_of(type, cols, n);
             const uint8_t *xg = ws + (size_t)tg * l.group;
             const float *fg = (const float *)(xg + l.operands);
             const int kn = min(kc, cols - k0), segs = (kn + SEG - 1) / SEG;
@@ -307,10 +309,10 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
     int from[TT], own[TT][TL];
 #pragma unroll
     for (int t = 0; t < TT; t++) {
-        from[t] = pair ? (min(lr >> 1, nt - 1) + (lr & 1) * nt) * 64 + g * 16
+        from[t] = split ? (min(lr >> 1, nt - 1) + (lr & 1) * nt) * 64 + g * 16
                        : min(t * 16 + lr, nt - 1) * 64 + g * 16;
 #pragma unroll
-        for (int r = 0; r < TL; r++) own[t][r] = pair ? 2 * g + r : t * 16 + 4 * g + r;
+        for (int r = 0; r < TL; r++) own[t][r] = split ? 2 * g + r : t * 16 + 4 * g + r;
     }
     if constexpr (N > 0) stage();
     int c = 0;
@@ -357,7 +359,7 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
         for (int t = 0; t < TT; t++)
 #pragma unroll
             for (int r = 0; r < TL; r++) part[t][r] = 0.0f;
-        f4 hi[TT], lo[TT];
+        f4 sum[TT];
 #pragma unroll
         for (int j = 0; j < CHUNK / 32; j++) {
             if (WHOLE || j < blocks) {
@@ -367,16 +369,12 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
                 for (int t = 0; t < TT; t++) {
                     const uint8_t *at = lds + (size_t)(b0 + j) * step + from[t];
                     const f4 z = {0, 0, 0, 0};
-                    hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8 *)at, b, begin ? z : hi[t], 0, 0, 0);
-                    if constexpr (split && !pair)
-                        lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8 *)(at + (size_t)nt * 64), b,
-                                                                       begin ? z : lo[t], 0, 0, 0);
+                    sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8 *)at, b, begin ? z : sum[t], 0, 0, 0);
                     if (end) {
 #pragma unroll
                         for (int r = 0; r < TL; r++) {
-                            float v = pair ? __builtin_fmaf(hi[t][(2 * r + 1) & 3], 0x1p-11f, hi[t][2 * r & 3])
-                                           : hi[t][r];
-                            if constexpr (split && !pair) v = __builtin_fmaf(lo[t][r], 0x1p-11f, v);
+                            const float v = split ? __builtin_fmaf(sum[t][(2 * r + 1) & 3], 0x1p-11f, sum[t][2 * r & 3])
+                                                  : sum[t][r];
                             part[t][r] = __builtin_fmaf(sc[j / (G / 32)], v, part[t][r]);
                         }
                     }
@@ -433,8 +431,8 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
     store();
 }
 
-// More than FEW tokens and not so many rows: one tile of 16 rows, the chunks of
-// 256 columns dealt out to eight wavefronts. Each operand of the tokens is used
+// More than FEW tokens: RT tiles of 16 rows, the chunks of 256 columns dealt out
+// to eight wavefronts. Each operand of the tokens is used
 // once in the workgroup, so it comes straight from memory (L2) into registers: 16-bit
 // x from x itself, unscaled and whole -- bf16 codes for a bf16 product, which
 // cost twice the instructions that fp16 ones do, shared by the TT tiles of 16 tokens
@@ -659,14 +657,8 @@ int launch(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s,
            int n, const void *ws, const T *x, int ldx) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
     const int nt = n < TG ? n : TG;
-    // columns per LDS stage: all of them for operands formed in place; else
-    // whole segments, or a half, a quarter, an eighth of one, up to 48 KB, more
-    // where that is less than a chunk per column share
+    // columns per LDS stage: all of them for operands formed in place, else a segment
     int kc = SEG;
-    if ((size_t)kc * P * nt * 2 <= 48 * 1024)
-        kc = 48 * 1024 / (P * nt * 2) / SEG * SEG;
-    else
-        while ((size_t)kc * P * nt * 2 > 128 * 1024) kc /= 2;  // 512 at least
     if (kc > cols || N > 0) kc = (cols + CHUNK - 1) / CHUNK * CHUNK;
     size_t lds = (size_t)kc * P * nt * 2 + (size_t)((kc + SEG - 1) / SEG) * TG * 4;
     const size_t join = (size_t)(WK - 1) * WR * TT * 1024;
@@ -685,7 +677,7 @@ int launch(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s,
     return mhip::check_launch(c, "matvec_q4");
 }
 
-// From 12288 rows on there is a tile for each of three workgroups' wavefronts on every
+// Up to FEW tokens: from 12288 rows on there is a tile for each of three workgroups' wavefronts on every
 // CU, which then take whole rows one after another; below, the columns are split
 // over a workgroup's wavefronts (2048 columns, one token: 8192 rows 6.4 us, whole
 // rows 7.9; 16384 rows 11.3 us, whole rows 8.1; head of 151936 rows 73 and 40 us).
@@ -694,28 +686,29 @@ constexpr int MANY_ROWS = 12288;
 template <class T, int G, bool WHOLE, int TT>
 int many_tokens(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows,
                 int cols, int n, void *ws, const T *x, int ldx) {
-    const bool many = rows >= MANY_ROWS;
+    // 17 to 32 tokens of 16-bit x: from LDS where rows are many (bf16, 32 tokens of
+    // 2048 columns: 16384 rows 14.9 us, k_q4_wide 11.3; 32768 rows 18.4 and 20.6; 151936 rows
+    // 72 and 98)
+    constexpr bool may = TT == 2 && sizeof(T) == 2;
+    const bool many = may && rows >= 2 * MANY_ROWS;
     if (many || type == MHIP_F32) {
         k_q4_tokens<T><<<dim3(n, (cols + SEG - 1) / SEG), 256, 0, c->stream>>>(x, ldx, cols, n, type,
                                                                                (uint8_t *)ws);
         if (mhip::check_launch(c, "matvec_q4 tokens")) return -1;
     }
-    if (many) return launch<T, G, WHOLE, 0, TT, 4, 2, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    if constexpr (may)
+        if (many) return launch<T, G, WHOLE, 0, TT, 4, 2, 2>(c, type, out, ldo, w, s, rows, cols, n, ws, x, ldx);
+    // (fp32 x takes twice the registers: 32 tokens a workgroup at most; 64 tokens of
+    // 11008 x 4096 40 us, all in one 74)
     constexpr int WT = TT == 4 && sizeof(T) == 4 ? 2 : TT;
     auto wide = [&](auto k, int rt) {
         k<<<dim3((rows + 16 * rt - 1) / (16 * rt), (n + 16 * WT - 1) / (16 * WT)), 512, 0, c->stream>>>(
             out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows, cols, n, (const uint8_t *)ws, x, ldx);
     };
-    // two tiles of rows a workgroup where one each would be more than one per CU
-    // (64 tokens, bf16, 6144 x 2048: 12.2 us, two tiles 8.7; 11008 x 4096: 32 and 30), but
-    // not where registers run out (fp32, 33 tokens or more: 11008 x 4096 74 us, two tiles 102)
-    if constexpr (TT > 1) {
-        if (rows > 256 * 16) {
-            wide(k_q4_wide<T, G, WHOLE, WT, 2>, 2);
-            return mhip::check_launch(c, "matvec_q4");
-        }
-    }
-    wide(k_q4_wide<T, G, WHOLE, WT, 1>, 1);
+    // two tiles of rows a workgroup where one each would be more than one per CU (64
+    // tokens, bf16, 6144 x 2048: 12.2 us, two tiles 8.7; 16 tokens 5.3 and 5.0, fp32 9.9 and 8.3)
+    if (rows > 256 * 16) wide(k_q4_wide<T, G, WHOLE, WT, 2>, 2);
+    else wide(k_q4_wide<T, G, WHOLE, WT, 1>, 1);
     return mhip::check_launch(c, "matvec_q4");
 }
 

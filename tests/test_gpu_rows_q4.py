@@ -188,3 +188,23 @@ def test_offsets_beyond_32_bits(g, n):
     w = q4_weights(codes, scales, group)
     o = x @ w.T
     assert (np.abs(out[:, -3:] - o) <= q4_tolerance(w, x, o, M.MHIP_BF16)).all()
+
+
+# rows, cols, group, tokens: around the choices of many tokens
+MANY = [(24600, 256, 32, 17), (24577, 1312, 32, 32), (24576, 2304, 128, 20), (5000, 512, 64, 16), (4112, 800, 32, 9),
+        (4100, 1056, 32, 33), (200, 512, 64, 100), (100, 2080, 32, 96), (5000, 256, 128, 64)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("pad", [0, 8, 32])  # rows of x that start in other halves of their lines
+@pytest.mark.parametrize("x", range(len(MANY)))
+def test_many_tokens(g, x, pad, t):
+    rows, cols, group, n = MANY[x]
+    print("test_many_tokens", MANY[x], pad, t, flush=True)
+    rng = np.random.default_rng(100 + x)
+    codes, scales = weights(rng, rows, cols, group)
+    v = rng.standard_normal((n, cols)) * np.exp(rng.standard_normal(cols))
+    got = product(g, t, codes, scales, group, v, padx=pad, pado=x % 3)
+    w, xv = q4_weights(codes, scales, group), rounded(v, t)[0]
+    o = xv @ w.T
+    assert (np.abs(got - o) <= q4_tolerance(w, xv, o, t)).all()
