@@ -14,18 +14,17 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // How a call is cut. A part of the prefix serves up to 128 rows (16-bit heads up
 // to 128); tiles of 64 rows do better up to 128 rows in all (16 slots behind 16000
-// tokens, bf16: 28 us, with tiles of 128 rows 32; 64 slots behind 8000: 35 and 33).
-// (The times here compare the two sides; the kernel has become faster since.) Every part's
-// results pass through memory once more, so there are only as many as
-// keep the CUs busy: 256 workgroups for the prefix (64 x 8000: with 8 parts 41
-// us, 16 parts 33, 32 parts 41) and 256 for the slots (32 unshared slots of up
-// to 8000 tokens: 2 parts 79 us, 8 parts 90; 64 of 300 tokens: 1 part 12 us, 2
-// parts 18; fp32 behind a prefix, whose tiles take longest, fewer and longer ones:
-// 16 slots of 400, 26 us in one part each, 29 in two). Without a
-// prefix one part needs no join, so the number is rounded down (200 workgroups
-// or 400: 13.5 and 16.6 us), else up (168 or 336: 19.0 and 16.5). Where
-// a CU holds one workgroup only the two together should not be more than the
-// CUs.
+// tokens, bf16: 22.6 us, with tiles of 128 rows 24.8; 64 slots behind 8000: 30.4
+// and 29.1). Every part's results pass through memory once more, so there are
+// only as many as keep the CUs busy: 256 workgroups for the prefix (64 slots
+// behind 8000: 8 parts 39 us, 16 parts 30, 32 parts 35) and 256 for the slots (32
+// unshared slots of up to 8000 tokens: 2 parts 77 us, 8 parts 85; 64 of 300
+// tokens: 1 part 9.8 us, 2 parts 14.7; fp32 behind a prefix, whose tiles take
+// longest, fewer and longer ones: 16 slots of 400, 26.6 us in one part each, 29.3
+// in two). Without a prefix one part needs no join, so the number is rounded down
+// (200 workgroups or 400: 13.3 and 17.0 us), else up (168 or 336: 17.0 and 14.9).
+// Where a CU holds one workgroup only the two together should not be more than
+// the CUs.
 Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int max_len) {
     Cut k;
     const int group = n_heads / s->n_kv_heads, rest = max_len - prefix;
