@@ -557,8 +557,8 @@ int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * d_q and d_out are 16-byte aligned as their rows' steps are. d_ws:
  * mhip_attention_shared_ws_bytes() bytes, 256-byte aligned, of one call at a
  * time (0 for invalid arguments). Scores, softmax and sums are fp32; with a
- * 16-bit cache the softmax's weights are rounded to that type for the
- * product with v. Where a page of the table is out of range its tokens
+ * 16-bit cache the softmax's weights meet v in two pieces of that type (2^-16 of
+ * a weight or closer). Where a page of the table is out of range its tokens
  * count as zeros, with an error bit. */
 size_t mhip_attention_shared_ws_bytes(const mhip_page_dims *s, int n_heads, int n, int max_count,
                                       int prefix, int max_len);
