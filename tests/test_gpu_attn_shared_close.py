@@ -86,3 +86,40 @@ def test_one_rounding(g, x, t):
         check(c, q, heads, seqs, counts, top, {prefix, 0}, max(lens), 1 / np.sqrt(hd))
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("scale", [2.0 ** -5, 2.0 ** -4, 2.0 ** -3, 2.0 ** -2, 0.5, 1.0])
+def test_scores_a_step_apart(g, scale, t):
+    """Two scores one step of fp32 apart, which is 8 behind the scale: the second is
+    a weight of e^8 beside the first's 1, in whichever order they come, in one tile or
+    two. Both scores are whole numbers that fp32 has (2^26 / scale, and a step more),
+    all others are 0 and weigh nothing; what is left are the exponentials (2^-21 each
+    and their arguments' roundings, 16 x 2^-23), the pieces and the output."""
+    if t == M.MHIP_F16 and scale < 2.0 ** -4:
+        pytest.skip("the first key, 2^11 / scale, is not an fp16 value")
+    c = Cache(g, type=t, n_layers=1, n_kv_heads=1, head_dim=64, max_blocks=20, max_seqs=1, n_pages=20)
+    try:
+        n, rng = 200, np.random.default_rng(21)
+        c.extend([0], [n])
+        q = np.zeros((1, 64))
+        q[0, :2] = 2.0 ** 15, 8.0
+        top = 2.0 ** 26 / scale
+        c.v = rounded(rng.standard_normal(c.v.shape), t)[1].reshape(c.v.shape)
+        for first, second in ((0, 64), (64, 0), (3, 190), (70, 75), (1, 17)):
+            k = np.zeros(c.k.shape)
+            for at, step in ((first, 0.0), (second, top * 2.0 ** -23 / 8)):
+                k[0, c.table[0][at // 16], 0, at % 16, :2] = top / 2 ** 15, step
+            c.k = rounded(k, t)[1].reshape(c.k.shape)
+            c.load()
+            k, v = c.rows("k", 0, 0, n), c.rows("v", 0, 0, n)
+            assert scale * (k[second, 0] - k[first, 0]) @ q[0] == 8
+            o = attention(q.reshape(1, 64), k, v, scale)
+            eps = 0.0 if t == M.MHIP_F32 else torch.finfo(TORCH[t]).eps
+            tol = np.abs(v).max() * (2.0 ** -18 + 2 * (eps / 2) ** 2 + n * 2.0 ** -30) + eps / 2 * np.abs(o)
+            for prefix in (0, 64, 100):
+                got, bits = run(c, q, 1, [0], None, 1, prefix, n, scale)
+                print(first, second, prefix, got[0, 0, :2], o[0, :2], flush=True)
+                assert bits == 0 and (np.abs(got[0] - o) <= tol).all()
+    finally:
+        c.close()
