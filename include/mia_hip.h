@@ -572,7 +572,8 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
  * weights in groups of `group` (32, 64 or 128, dividing cols): weight =
  * scale * code, code -8 .. 7 in two's complement. d_codes[rows][cols/2]: the
  * even column in the low four bits (16-byte aligned); d_scales
- * [rows][cols/group] in fp16. rows <= 2^28, cols <= 2^24, rows * cols <= 2^34. */
+ * [rows][cols/group] in fp16. rows <= 2^28 (in a product 2^28 - 32), cols <= 2^24,
+ * rows * cols <= 2^34. */
 /* Codes and scales of fp32 weights: scale = max|w| / 7 rounded to fp16 (at
  * most 65504), code = the nearest integer of w / scale, kept in [-8, 7] (0 where
  * the scale rounds to 0). */

@@ -641,8 +641,9 @@ __global__ __launch_bounds__(256) void k_dequantize_q4(const uint8_t *codes, con
 
 int check_q4(mhip_ctx *c, const char *what, const void *d_codes, const void *d_scales, int rows,
              int cols, int group) {
-    // (a launch holds less than 2^32 threads: up to 8 a row, and one for 8 weights)
-    if (rows < 0 || rows > 1 << 28 || cols < 0 || cols > 1 << 24 || (long long)rows * cols > 1LL << 34 || (group != 32 && group != 64 && group != 128) || cols % group)
+    // (a launch holds less than 2^32 threads: one for 8 weights)
+    if (rows < 0 || rows > 1 << 28 || cols < 0 || cols > 1 << 24 || (long long)rows * cols > 1LL << 34 ||
+        (group != 32 && group != 64 && group != 128) || cols % group)
         return mhip::fail(c, "%s: %d rows of %d in groups of %d (32, 64 or 128, dividing the row)",
                           what, rows, cols, group);
     if (rows && cols && (!d_codes || !d_scales)) return mhip::fail(c, "%s: a null argument", what);
@@ -781,6 +782,8 @@ int mhip_matvec_q4(mhip_ctx *c, int type, void *d_out, int ldo, const void *d_co
     if (n < 0 || ldx < cols || ldo < rows)
         return mhip::fail(c, "matvec_q4: %d tokens, rows %d and %d apart (%d columns, %d rows)", n,
                           ldx, ldo, cols, rows);
+    if (rows > (1 << 28) - 32)  // (a launch holds less than 2^32 threads: 512 for two tiles of 16 rows)
+        return mhip::fail(c, "matvec_q4: %d rows in one call", rows);
     if (!n || !rows) return 0;
     if (!cols) return mhip::fail(c, "matvec_q4: no columns");
     if (!d_out || !d_x || !d_ws) return mhip::fail(c, "matvec_q4: a null argument");
