@@ -68,9 +68,10 @@ bool shape_ok(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, i
            max_len >= prefix && max_len <= (long long)s->max_blocks * s->page;
 }
 
-// A launch holds less than 2^32 threads (k_join: 64 a row, and 2^26 rows).
-bool fits(const mhip_page_dims *s, int n, const Cut &k) {
-    return s->n_kv_heads * ((long long)k.ptiles * k.sp + (long long)n * k.stiles * k.ss) < 1 << 24;
+// A launch holds less than 2^32 threads: 2^24 workgroups of 256 (k_join: one for four rows).
+bool fits(const mhip_page_dims *s, int n_heads, int n, int mc, const Cut &k) {
+    return s->n_kv_heads * ((long long)k.ptiles * k.sp + (long long)n * k.stiles * k.ss) < 1 << 24 &&
+           (k.sp + k.ss == 1 || (long long)n * mc * n_heads <= (1 << 26) - 4);
 }
 
 }  // namespace
@@ -81,7 +82,7 @@ size_t mhip_attention_shared_ws_bytes(const mhip_page_dims *s, int n_heads, int 
                                       int prefix, int max_len) {
     if (!mhip_pages_plan_bytes(s) || !shape_ok(s, n_heads, n, max_count, prefix, max_len)) return 0;
     const Cut k = cut_of(s, n_heads, n, max_count, prefix, max_len);
-    if (!fits(s, n, k)) return 0;
+    if (!fits(s, n_heads, n, max_count, k)) return 0;
     const size_t rows = (size_t)n * max_count * n_heads, parts = (size_t)k.sp + k.ss;
     return align256(parts * rows * s->head_dim * 4) + align256(parts * rows * 8);
 }
@@ -109,7 +110,7 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
         (uintptr_t)d_ws % 256)
         return mhip::fail(c, "%s: rows must start on 16 bytes, the workspace on 256", what);
     const Cut k = cut_of(s, n_heads, n, max_count, prefix, max_len);
-    if (!fits(s, n, k)) return mhip::fail(c, "%s: too many parts in one call", what);
+    if (!fits(s, n_heads, n, max_count, k)) return mhip::fail(c, "%s: too many rows or parts in one call", what);
     if (mhip::use_device(c)) return -1;
     Job a;
     a.s = *s;
