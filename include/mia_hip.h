@@ -544,8 +544,9 @@ int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * t = len - d_count[i] + j (d_count NULL: max_count each); it attends to its
  * slot's positions 0 .. t: softmax(scale q.k) v per query head (scale from
  * 2^-64 to 2^64), n_heads a multiple of n_kv_heads, n * max_count * n_heads
- * less than 2^26 (than 2^26 - 3 behind a prefix or with a max_len above 4096). Rows past d_count[i], and rows of an empty slot, are zeros in
- * d_out (rows ldo values apart).
+ * less than 2^26 (than 2^26 - 3 behind a prefix or with a max_len above
+ * 4096). Rows past d_count[i], and rows of an empty slot, are zeros in d_out
+ * (rows ldo values apart).
  *
  * The slots may share their first `prefix` tokens (0: they do not): those
  * are read from slot prefix_seq's pages, once for the whole batch instead of
