@@ -39,6 +39,7 @@ typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 constexpr int SEG = 1024;  // columns that share a token's power of two
 constexpr int TG = 64;     // tokens of one workgroup, at most
+constexpr int MOST_TOKENS = 65535 * TG;
 
 // The workspace: per group of TG tokens (nt of them) the operands
 // [cols/32][pieces][nt][32] fp16, in each 32 the order of codes(), then
@@ -773,7 +774,8 @@ int mhip_dequantize_q4(mhip_ctx *c, const void *d_codes, const void *d_scales, i
 }
 
 size_t mhip_matvec_q4_ws_bytes(int type, int cols, int n) {
-    if (type < MHIP_F32 || type > MHIP_BF16 || cols <= 0 || cols % 32 || n <= 0) return 0;
+    if (type < MHIP_F32 || type > MHIP_BF16 || cols <= 0 || cols > 1 << 24 || cols % 32 || n <= 0 || n > MOST_TOKENS)
+        return 0;
     return tokens_of(type, cols, n).group * (size_t)((n + TG - 1) / TG);
 }
 
@@ -794,7 +796,7 @@ int mhip_matvec_q4(mhip_ctx *c, int type, void *d_out, int ldo, const void *d_co
     if ((uintptr_t)d_x % 16 || (size_t)ldx * esz % 16 || (uintptr_t)d_out % esz ||
         (uintptr_t)d_ws % 256)
         return mhip::fail(c, "matvec_q4: x rows must start on 16 bytes, the workspace on 256");
-    if (n > 65535 * TG)
+    if (n > MOST_TOKENS)
         return mhip::fail(c, "matvec_q4: %d tokens of %d columns in one call", n, cols);
     if (mhip::use_device(c)) return -1;
     if (type == MHIP_F32)

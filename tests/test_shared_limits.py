@@ -35,3 +35,15 @@ def test_rows_of_attention(rows, heads, kv, n, top):
     if not size:
         assert L.mhip_attention_shared(None, D, A, 0, heads, 4096, heads * 64, 4096, heads * 64, 16, None, n, top, 0, 16,
                                        64, 0.1, 4096) == -1
+
+
+def test_workspace_of_calls_that_are_refused():
+    """No workspace for what no product takes: more than 2^24 columns, more than
+    65535 x 64 tokens."""
+    size = M.lib().mhip_matvec_q4_ws_bytes
+    for t in (M.MHIP_F32, M.MHIP_F16, M.MHIP_BF16):
+        assert size(t, 1 << 24, 1) > 0 and size(t, 64, 65535 * 64) > 0
+        for cols, n in (((1 << 24) + 32, 1), (64, 65535 * 64 + 1), ((1 << 31) - 32, 1), (32, (1 << 31) - 1)):
+            assert size(t, cols, n) == 0, (t, cols, n)
+            if n > 65535 * 64:
+                assert M.lib().mhip_matvec_q4(None, t, 4096, 64, 4096, 4096, 32, 4096, cols, 64, cols, n, 4096) == -1
