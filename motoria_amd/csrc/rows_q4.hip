@@ -440,14 +440,14 @@ __global__ __launch_bounds__(64 * WR * WK) void k_q4(T *out, size_t ldo, const u
 // -- and fp32 x from the workspace.
 template <class T, int G, bool WHOLE, int TT, int RT>
 __global__ __launch_bounds__(512) void k_q4_wide(T *out, size_t ldo, const uint8_t *w,
-                                                 const uint16_t *scales, int rows, int cols, int first,
-                                                 int n, const uint8_t *ws, const T *x, size_t ldx) {
+                                                 const uint16_t *scales, int rows, int cols, int n,
+                                                 const uint8_t *ws, const T *x, size_t ldx) {
     constexpr bool split = sizeof(T) == 4, bf = std::is_same<T, __bf16>::value;
     constexpr int GC = CHUNK / G, WK = 8;
     __shared__ float sum[WK * RT * TT * 4 * 64];
     const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, lr = lane & 15;
-    const int t0 = first + blockIdx.y * TT * 16, nt = min(TT * 16, n - t0);  // this workgroup's tokens
+    const int t0 = blockIdx.y * TT * 16, nt = min(TT * 16, n - t0);  // this workgroup's tokens
     const int tg = t0 / TG, of_group = min(TG, n - tg * TG);         // ... in a group of the workspace
     const int nchunk = (cols + CHUNK - 1) / CHUNK, nblock = cols / 32, ngroup = cols / G;
     const uint8_t *wr[RT];
@@ -703,12 +703,16 @@ int many_tokens(mhip_ctx *c, int type, T *out, int ldo, const void *w, const voi
     // (fp32 x takes twice the registers: 32 tokens a workgroup at most; 64 tokens of
     // 11008 x 4096 40 us, all in one 74)
     constexpr int WT = TT == 4 && sizeof(T) == 4 ? 2 : TT;
+    // (at most 65535 workgroups in a launch's second dimension: fp32 calls may take several
+    // launches of whole groups of the workspace, the last one of more than a group)
     auto wide = [&](auto k, int rt) {
-        constexpr int most = 65535 * 16 * WT;  // tokens of a launch (workgroups in its second dimension)
-        for (int t = 0; t < n; t += most)
-            k<<<dim3((rows + 16 * rt - 1) / (16 * rt), ((n - t < most ? n - t : most) + 16 * WT - 1) / (16 * WT)), 512, 0,
-                c->stream>>>(out, ldo, (const uint8_t *)w, (const uint16_t *)s, rows, cols, t, n, (const uint8_t *)ws, x,
-                             ldx);
+        const size_t group = tokens_of(type, cols, n).group;
+        for (int t = 0, part; t < n; t += part) {
+            part = n - t <= 65535 * 16 * WT ? n - t : 1 << 20;
+            k<<<dim3((rows + 16 * rt - 1) / (16 * rt), (part + 16 * WT - 1) / (16 * WT)), 512, 0, c->stream>>>(
+                out + (size_t)t * ldo, ldo, (const uint8_t *)w, (const uint16_t *)s, rows, cols, part,
+                (const uint8_t *)ws + t / TG * group, x + (size_t)t * ldx, ldx);
+        }
     };
     // two tiles of rows a workgroup where one each would be more than one per CU (64
     // tokens, bf16, 6144 x 2048: 12.2 us, two tiles 8.7; 16 tokens 5.3 and 5.0, fp32 9.9 and 8.3)
