@@ -7,7 +7,7 @@ import torch
 
 import motoria_amd as M
 from shared_model import TORCH, TYPES, Cache, attention, attention_tolerance, rounded
-from test_gpu_attn_shared import fill, run
+from test_gpu_attn_shared import close, fill, run
 
 pytestmark = pytest.mark.gpu
 
@@ -66,6 +66,15 @@ LAYOUTS = [
     (5, 1, 256, 128, [260, 300, 257, 514], 256, 1),
     (32, 4, 128, 16, [900] * 7, 850, 2),
     (24, 8, 64, 16, [2600, 2599], 2049, 1),
+    # behind a prefix that ends inside a page and a tile: tiles of 64 rows of heads of 129 to
+    # 256, and of 128 rows of 16-bit heads up to 64 and 128
+    (16, 2, 256, 32, [340, 341, 350, 339, 400, 338, 339, 361], 338, 1),
+    (8, 1, 144, 16, [203, 210, 204, 300, 203, 203, 251, 203], 203, 1),
+    (12, 1, 208, 64, [450, 449, 500, 449], 449, 2),
+    (8, 1, 64, 16, [310 + 3 * i for i in range(20)], 310, 1),
+    (8, 1, 48, 16, [77 + i for i in range(18)], 77, 1),
+    (8, 1, 112, 32, [500 + 9 * i for i in range(9)], 500, 2),
+    (16, 2, 128, 16, [3020] * 20, 3007, 1),
 ]
 
 
@@ -121,5 +130,69 @@ def test_scores_a_step_apart(g, scale, t):
                 got, bits = run(c, q, 1, [0], None, 1, prefix, n, scale)
                 print(first, second, prefix, got[0, 0, :2], o[0, :2], flush=True)
                 assert bits == 0 and (np.abs(got[0] - o) <= tol).all()
+    finally:
+        c.close()
+
+
+# heads, head size, slots
+TILES = [(8, 64, 20), (8, 128, 18), (8, 80, 17), (8, 32, 24), (10, 112, 4), (4, 256, 9), (8, 144, 3), (16, 208, 6),
+         (2, 96, 7)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("x", range(len(TILES)))
+def test_values_that_are_not_finite(g, x, bad, t):
+    """Infinities and NaN among the values, for every tile of rows and padded heads: where
+    all rows see them, where short slots end before them in the same tile, in
+    some slots' own tokens, and behind every end."""
+    heads, hd, n = TILES[x]
+    print("test_values_that_are_not_finite", TILES[x], bad, t, flush=True)
+    rng = np.random.default_rng(300 + x)
+    c = Cache(g, type=t, n_layers=1, n_kv_heads=1, head_dim=hd, max_blocks=16, max_seqs=n + 1, n_pages=17 * (n + 1))
+    try:
+        prefix = 150
+        c.extend([0], [prefix])
+        c.fork([0] * (n - 1), list(range(2, n + 1)))
+        c.extend([1], [40])  # the prefix's first 40 tokens and no more
+        for mine in (c.k, c.v):
+            for b in range(3):
+                mine[:, c.table[1][b]] = mine[:, c.table[0][b]]
+        c.extend([0] + list(range(2, n + 1)), [5] + [3 + 2 * (i % 30) for i in range(2, n + 1)])
+        worst = rounded(np.array([bad]), t)[1][0]
+        for s in range(n + 1):
+            b, r = divmod(c.len[s], 16)
+            if r:
+                c.k[:, c.table[s][b], :, r:] = worst
+                c.v[:, c.table[s][b], :, r:] = worst
+        c.load()
+        q = rng.standard_normal((n + 1, heads * hd))
+        seqs = rng.permutation(n + 1).tolist()
+        own = [s for s in range(2, n + 1) if s % 3 == 0]
+        for seen in ((), (100,), (50,), (20, 120)):
+            was = c.v.copy()
+            for at in seen:
+                # (a page that slot 1 does not share is its own copy)
+                for s in (0, 1):
+                    if at < c.len[s]:
+                        c.v[0, c.table[s][at // 16], 0, at % 16, (at + s) % hd] = worst
+            for s in own:
+                b, r = divmod(c.len[s] - 1, 16)
+                c.v[0, c.table[s][b], 0, r, 1] = worst
+            c.load()
+            qv = rounded(q, t)[0].reshape(n + 1, heads, hd)
+            rows, tol = np.zeros(qv.shape), np.zeros(qv.shape)
+            for i, s in enumerate(seqs):
+                k, v = c.rows("k", 0, s, c.len[s]), c.rows("v", 0, s, c.len[s])
+                rows[i] = attention(qv[i], k, v, 0.1)
+                fine = np.where(np.isfinite(v), v, 0.0)
+                tol[i] = one_rounding(qv[i], k, fine, attention(qv[i], k, fine, 0.1), 0.1, t)
+            # (slot 1 is a copy of the prefix only where nothing in it differs)
+            with_prefix = (prefix, 99, 0) if not any(at < 40 for at in seen) else (0,)
+            for p in with_prefix:
+                got, bits = run(c, q, heads, seqs, None, 1, p, 230, 0.1)
+                assert bits == 0
+                close(got, rows, tol)
+            c.v = was
     finally:
         c.close()
