@@ -19,34 +19,32 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // only as many as keep the CUs busy: 256 workgroups for the prefix (64 slots
 // behind 8000: 8 parts 39 us, 16 parts 30, 32 parts 35) and 256 for the slots (32
 // unshared slots of up to 8000 tokens: 2 parts 77 us, 8 parts 85; 64 of 300
-// tokens: 1 part 9.8 us, 2 parts 14.7; fp32 behind a prefix, whose tiles take
-// longest, fewer and longer ones: 16 slots of 400, 26.6 us in one part each, 29.3
-// in two). Without a prefix one part needs no join, so the number is rounded down
-// (200 workgroups or 400: 13.3 and 17.0 us), else up (168 or 336: 17.0 and 14.9).
-// Where a CU holds one workgroup only the two together should not be more than
-// the CUs.
+// tokens: 1 part 9.8 us, 2 parts 14.7). Without a prefix one part needs no join, so the
+// number is rounded down (200 workgroups or 400: 13.3 and 17.0 us), else up (168 or 336:
+// 17.0 and 14.9). Where a CU holds one workgroup only the two together should not be more
+// than the CUs. fp32 tiles keep the matrix cores busy, so that two workgroups on a CU
+// take twice as long: slots of up to 512 positions behind a prefix stay in one part each
+// where that keeps the launch at one a CU (64 slots' workgroups or 128 beside 160 of the
+// prefix: 300 positions 22.8 us and 26.9, 400 26.5 and 29.0, 500 29.0 and 29.3, 600 31.4 and
+// 29.1; 128 or 256 beside 56: 300 positions 15.2 and 17.3, 600 20.1 and 19.9); else they
+// are cut as others are (beside 248: 400 positions 36.5 and 30.6).
 Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int max_len) {
     Cut k;
     const int group = n_heads / s->n_kv_heads, rest = max_len - prefix;
     const long long rows = (long long)n * mc * group;
     k.stiles = (mc * group + 15) / 16;
-    const long long items = (long long)n * s->n_kv_heads * k.stiles;
-    long long parts = prefix == 0 ? 256 / items : ((s->type == MHIP_F32 ? 96 : 256) + items - 1) / items;
-    const int shortest = prefix > 0 && s->type == MHIP_F32 ? 512 : 256;
-    const int most = (rest + shortest - 1) / shortest, least = (rest + PART_MAX - 1) / PART_MAX;
-    if (parts > most) parts = most;
-    if (parts < least) parts = least;
-    if (parts < 1) parts = 1;
-    k.slen = rest > 0 ? (int)((rest + parts - 1) / parts + TILE - 1) / TILE * TILE : TILE;
-    k.ss = rest > 0 ? (rest + k.slen - 1) / k.slen : 1;
-
     k.wr = prefix == 0 ? 1 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
     k.rt = prefix > 0 && rows > 128 && s->head_dim <= 128 && s->type != MHIP_F32 ? 2 : 1;
     const int tile = k.wr * k.rt * 16;
     k.ptiles = prefix > 0 ? (int)((rows + tile - 1) / tile) : 0;
-    k.sp = 0;
-    k.plen = 0;
-    if (prefix > 0) {
+    const long long items = (long long)n * s->n_kv_heads * k.stiles;
+
+    auto cut = [&](long long parts) {  // `parts` for each slot
+        k.slen = rest > 0 ? (int)((rest + parts - 1) / parts + TILE - 1) / TILE * TILE : TILE;
+        k.ss = rest > 0 ? (rest + k.slen - 1) / k.slen : 1;
+        k.sp = 0;
+        k.plen = 0;
+        if (prefix == 0) return;
         const int padded = s->head_dim <= 64 ? 64 : s->head_dim <= 128 ? 128 : 256;
         const bool single = padded * mhip::type_bytes(s->type) > (tile > 16 ? 512 : 256);
         long long wgs = (single ? 256 : 512) - items * k.ss;
@@ -58,7 +56,17 @@ Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int 
         if (pp < pleast) pp = pleast;
         k.plen = (int)((prefix + pp - 1) / pp + TILE - 1) / TILE * TILE;
         k.sp = (prefix + k.plen - 1) / k.plen;
-    }
+    };
+    auto wgs = [&]() { return items * k.ss + (long long)s->n_kv_heads * k.ptiles * k.sp; };
+    const int most = (rest + 255) / 256, least = (rest + PART_MAX - 1) / PART_MAX;
+    long long parts = prefix == 0 ? 256 / items : (256 + items - 1) / items;
+    if (parts > most) parts = most;
+    if (parts < least) parts = least;
+    if (parts < 1) parts = 1;
+    cut(1);
+    const bool one = s->type == MHIP_F32 && prefix > 0 && rest <= 512 && wgs() <= 256;
+    if (parts > 1) cut(parts);
+    if (one && wgs() > 256) cut(1);
     return k;
 }
 
