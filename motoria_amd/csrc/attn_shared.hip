@@ -13,16 +13,16 @@ using mhip_shared::TILE;
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // How a call is cut. A part of the prefix serves up to 128 rows (16-bit heads up
-// to 128); tiles of 64 rows do better up to 128 rows in all (16 slots behind 16000
-// tokens, bf16: 22.6 us, with tiles of 128 rows 24.8; 64 slots behind 8000: 30.4
-// and 29.1). Every part's results pass through memory once more, so there are
+// to 128); tiles of 64 rows do better up to 256 rows in all (bf16, 8 rows a slot behind 8000
+// tokens: 24 slots 21.4 us, with tiles of 128 rows 24.5; 32 slots 24.0 and 25.6; 40 slots 30.9 and
+// 31.0; 56 slots 52.7 and 45.7). Every part's results pass through memory once more, so there are
 // only as many as keep the CUs busy: 256 workgroups for the prefix (64 slots
-// behind 8000: 8 parts 39 us, 16 parts 30, 32 parts 35) and 256 for the slots (32
-// unshared slots of up to 8000 tokens: 2 parts 77 us, 8 parts 85; 64 of 300
-// tokens: 1 part 9.8 us, 2 parts 14.7). Without a prefix one part needs no join, so the
-// number is rounded down (200 workgroups or 400: 13.3 and 17.0 us), else up (168 or 336:
-// 17.0 and 14.9). Where a CU holds one workgroup only the two together should not be more
-// than the CUs. fp32 tiles keep the matrix cores busy, so that two workgroups on a CU
+// behind 8000: 8 parts 45 us, 16 parts 32.6, 32 parts 41) and 256 for the slots (32
+// unshared slots of up to 8000 tokens: 2 parts 75 us, 8 parts 81; 64 of 300
+// tokens: 1 part 10.4 us, 2 parts 15.4). Without a prefix one part needs no join, so the
+// number is rounded down (200 workgroups or 400: 500 positions 12.7 and 16.6 us, 2000
+// positions 36.4 and 40.6), else up (fp16, 168 or 336: 20.1 and 17.1). Where a CU holds one
+// workgroup only the two together should not be more than the CUs. fp32 tiles keep the matrix cores busy, so that two workgroups on a CU
 // take twice as long: slots of up to 512 positions behind a prefix stay in one part each
 // where that keeps the launch at one a CU (64 slots' workgroups or 128 beside 160 of the
 // prefix: 300 positions 22.8 us and 26.9, 400 26.5 and 29.0, 500 29.0 and 29.3, 600 31.4 and
@@ -34,7 +34,7 @@ Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int 
     const long long rows = (long long)n * mc * group;
     k.stiles = (mc * group + 15) / 16;
     k.wr = prefix == 0 ? 1 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
-    k.rt = prefix > 0 && rows > 128 && s->head_dim <= 128 && s->type != MHIP_F32 ? 2 : 1;
+    k.rt = prefix > 0 && rows > 256 && s->head_dim <= 128 && s->type != MHIP_F32 ? 2 : 1;
     const int tile = k.wr * k.rt * 16;
     k.ptiles = prefix > 0 ? (int)((rows + tile - 1) / tile) : 0;
     const long long items = (long long)n * s->n_kv_heads * k.stiles;

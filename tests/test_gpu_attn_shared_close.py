@@ -75,6 +75,10 @@ LAYOUTS = [
     (8, 1, 48, 16, [77 + i for i in range(18)], 77, 1),
     (8, 1, 112, 32, [500 + 9 * i for i in range(9)], 500, 2),
     (16, 2, 128, 16, [3020] * 20, 3007, 1),
+    (16, 1, 64, 16, [310 + 3 * i for i in range(20)], 310, 1),
+    (16, 1, 48, 16, [77 + i for i in range(18)], 77, 1),
+    (16, 1, 128, 32, [500 + 9 * i for i in range(9)], 500, 2),
+    (20, 1, 80, 64, [1100 + 2 * i for i in range(14)], 1090, 1),
 ]
 
 
@@ -136,7 +140,7 @@ def test_scores_a_step_apart(g, scale, t):
 
 # heads, head size, slots
 TILES = [(8, 64, 20), (8, 128, 18), (8, 80, 17), (8, 32, 24), (10, 112, 4), (4, 256, 9), (8, 144, 3), (16, 208, 6),
-         (2, 96, 7)]
+         (2, 96, 7), (16, 64, 20), (16, 128, 17), (20, 80, 14)]
 
 
 @pytest.mark.parametrize("t", TYPES)
