@@ -472,7 +472,10 @@ int mhip_chain_f32(mhip_ctx *c, const float *d_v, int n, int mode, float thr, in
  * is fixed: the free pages of lowest index, in the order of the call's list.
  * An invalid call that the host sees returns -1; what only the device sees
  * (an index out of range, a slot twice in one list, no page left) sets bits
- * of mhip_pages_status and leaves memory outside the cache alone.
+ * of mhip_pages_status and leaves memory outside the cache alone. A slot of
+ * length l holds l / page pages, rounded up, and each counts in refs: a program
+ * that writes table or len by itself (these calls never shorten a slot but to
+ * nothing) keeps that so, or pages stay in use for good.
  */
 #define MHIP_F32 0 /* element types of the cache, and of rows in and out */
 #define MHIP_F16 1
@@ -504,11 +507,12 @@ int mhip_pages_clear(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p);
 int mhip_pages_extend(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
                       const int *d_seqs, const int *d_count, int n);
 /* The keys and values of one layer for the last d_count[i] tokens of each
- * slot (NULL: max_count each): token j < d_count[i] of entry i is row
+ * slot (0 to max_count; NULL: max_count each): token j < d_count[i] of entry i is row
  * i * max_count + j of d_k and d_v (rows of n_kv_heads * head_dim values, ld
  * values apart, 16-byte aligned as the rows' step is; rows past d_count[i] are
  * in the arrays, but not used). Less than 2^24 rows. A slot twice in the list
- * is not looked for: its positions get the rows of either entry. */
+ * is not looked for: its positions get the rows of either entry. What is
+ * written to a page that several slots share is every one's. */
 int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,
                      const int *d_seqs, const int *d_count, int n, int max_count,
                      const void *d_k, const void *d_v, int ld);
@@ -541,7 +545,7 @@ int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * rows are in the cache already (mhip_pages_extend and _write come first).
  * Row i * max_count + j of d_q ([n_heads][head_dim] values of the cache's
  * type, rows ldq values apart) is token j of slot d_seqs[i], at position
- * t = len - d_count[i] + j (d_count NULL: max_count each); it attends to its
+ * t = len - d_count[i] + j (0 <= d_count[i] <= max_count; NULL: max_count each); it attends to its
  * slot's positions 0 .. t: softmax(scale q.k) v per query head (scale from
  * 2^-64 to 2^64), n_heads a multiple of n_kv_heads, n * max_count * n_heads
  * less than 2^26 (than 2^26 - 3 behind a prefix or with a max_len above
@@ -557,7 +561,8 @@ int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
  * longer slot is an error bit and its row is NaN).
  * d_q and d_out are 16-byte aligned as their rows' steps are. d_ws:
  * mhip_attention_shared_ws_bytes() bytes, 256-byte aligned, of one call at a
- * time (0 for invalid arguments). Scores, softmax and sums are fp32; with a
+ * time (0 for invalid arguments). Scores, softmax and sums are fp32 (values of v
+ * from 2^90 on may leave its range before they are divided by the weights' sum); with a
  * 16-bit cache the softmax's weights meet v in two pieces of that type (2^-16 of
  * a weight or closer). Where a page of the table is out of range its tokens
  * count as zeros, with an error bit. */
@@ -584,10 +589,10 @@ int mhip_dequantize_q4(mhip_ctx *c, const void *d_codes, const void *d_scales, i
                        int group, float *d_w);
 /* out[t][r] = sum over c of w[r][c] x[t][c] for n tokens: x and out of `type`
  * (MHIP_F32, ...), rows ldx and ldo values apart (x 16-byte aligned as its
- * rows' step is), sums in fp32. fp32 x enters the products with 22 bits or
- * more of each value's (values 2^29 below the largest of 1024 columns lose
- * further bits); fp16 x enters whole, and so do bf16 values down to 2^-32 of
- * the largest of 1024 columns (smaller ones may lose bits). n <= 65535 * 64. d_ws:
+ * rows' step is), sums in fp32. fp32 x enters the products within 2^-23 of each
+ * value (values 2^27 and more below the largest of 1024 columns lose bits);
+ * fp16 x enters whole, and so do bf16 values down to 2^-31 of the largest of 1024
+ * columns (smaller ones may lose bits). n <= 65535 * 64. d_ws:
  * mhip_matvec_q4_ws_bytes() bytes, 256-byte aligned, of one call at a time (0
  * for invalid arguments). */
 size_t mhip_matvec_q4_ws_bytes(int type, int cols, int n);

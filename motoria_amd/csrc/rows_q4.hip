@@ -13,11 +13,11 @@
 //
 // x as fp16 operands (up to FEW tokens; fp32 x; 17 to 32 tokens of 16-bit x with many
 // rows): each token's segment of 1024 columns is scaled by a power of two that brings its largest value to [2^14,
-// 2^15). A bf16 value then is an fp16 value (8 bits; exact down to 2^-32 of the
+// 2^15). A bf16 value then is an fp16 value (8 bits; exact down to 2^-31 of the
 // largest). An fp32 value is split: hi = fp16(x'), lo = fp16((x' - hi) 2^11), together
-// within 2^-23 of x (a step of fp32's own rounding) down to 2^-29 of the
-// segment's largest value, as lo carries its own exponent; their products
-// are accumulated apart and joined in fp32. fp16 x is taken as it is; elsewhere
+// within 2^-23 of x (a step of fp32's own rounding) down to 2^-27 of the
+// segment's largest value (then fp16's least step counts, 2^-36 of x'), as lo carries its
+// own exponent; their products are accumulated apart and joined in fp32. fp16 x is taken as it is; elsewhere
 // 16-bit x of either type is (k_q4_wide).
 //
 // Measured (us; bytes of the weights at what a large copy reaches, 4.92 TB/s, in
