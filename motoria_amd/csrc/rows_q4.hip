@@ -12,20 +12,21 @@
 // which still is faster than the vector units (2.25 instructions a weight).
 //
 // x as fp16 operands (up to FEW tokens; fp32 x; 17 to 32 tokens of 16-bit x with many
-// rows): each token's segment of 1024 columns is scaled by a power of two that brings its largest value to [2^14,
-// 2^15). A bf16 value then is an fp16 value (8 bits; exact down to 2^-31 of the
-// largest). An fp32 value is split: hi = fp16(x'), lo = fp16((x' - hi) 2^11), together
-// within 2^-23 of x (a step of fp32's own rounding) down to 2^-27 of the
-// segment's largest value (then fp16's least step counts, 2^-36 of x'), as lo carries its
-// own exponent; their products are accumulated apart and joined in fp32. fp16 x is taken as it is; elsewhere
-// 16-bit x of either type is (k_q4_wide).
+// rows): each token's segment of 1024 columns is scaled by a power of two that
+// brings its largest value to [2^14, 2^15). A bf16 value then is an fp16 value (8 bits;
+// exact down to 2^-31 of the largest). An fp32 value is split: hi = fp16(x'), lo =
+// fp16((x' - hi) 2^11), together within 2^-23 of x (a step of fp32's own rounding)
+// down to 2^-27 of the segment's largest value (then fp16's least step counts, 2^-36
+// of x'), as lo carries its own exponent; their products are accumulated apart and
+// joined in fp32. fp16 x is taken as it is; elsewhere 16-bit x of either type is
+// (k_q4_wide).
 //
-// Measured (us; bytes of the weights at what a large copy reaches, 4.92 TB/s, in
-// brackets): a head of 151936 x 2048, fp32, groups of 32, one token 40 [36], fp16 with
-// groups of 128 33 [33]; 512 to 4096 x 2048, one token 5, a launch among others being
-// 3.6; 4096 x 2048 in bf16 with 16 tokens 4.5, with 64 tokens 7.0, where a workgroup
-// waits for 256 KB of operands from L2; the head with 16 tokens, fp32 81 [36], bf16,
-// groups of 128, 54 [33].
+// Measured (us, a call in a row of calls; bytes of the weights at what a large copy
+// reaches, 4.92 TB/s, in brackets): a head of 151936 x 2048, fp32, groups of 32, one token
+// 40 [36], fp16 with groups of 128 33 [33]; 512 to 4096 x 2048, one token 5, a launch among
+// others being 3.6; 4096 x 2048 in bf16 with 16 tokens 5.2, with 64 tokens 7.0, where a
+// workgroup waits for 256 KB of operands from L2; the head with 16 tokens, fp32 81 [36],
+// bf16, groups of 128, 57.5 [33], with 64 tokens 162.
 #include "mhip_internal.h"
 #include <type_traits>
 
@@ -701,8 +702,8 @@ template <class T, int G, bool WHOLE, int TT>
 int many_tokens(mhip_ctx *c, int type, T *out, int ldo, const void *w, const void *s, int rows,
                 int cols, int n, void *ws, const T *x, int ldx) {
     // 17 to 32 tokens of 16-bit x: from LDS where rows are many (bf16, 32 tokens of
-    // 2048 columns: 16384 rows 14.9 us, k_q4_wide 11.3; 32768 rows 18.4 and 20.6; 151936 rows
-    // 72 and 98)
+    // 2048 columns: 16384 rows 15.1 us, k_q4_wide 12.1; 32768 rows 18.3 and 21.9; 151936 rows
+    // 72 and 104)
     constexpr bool may = TT == 2 && sizeof(T) == 2;
     const bool many = may && rows >= 2 * MANY_ROWS;
     if (many || type == MHIP_F32) {
@@ -727,7 +728,7 @@ int many_tokens(mhip_ctx *c, int type, T *out, int ldo, const void *w, const voi
         }
     };
     // two tiles of rows a workgroup where one each would be more than one per CU (64
-    // tokens, bf16, 6144 x 2048: 12.2 us, two tiles 8.7; 16 tokens 5.3 and 5.0, fp32 9.9 and 8.3)
+    // tokens, bf16, 6144 x 2048: 12.5 us, two tiles 9.7; 16 tokens 5.5 and 5.3, fp32 10.0 and 8.5)
     if (rows > 256 * 16) wide(k_q4_wide<T, G, WHOLE, WT, 2>, 2);
     else wide(k_q4_wide<T, G, WHOLE, WT, 1>, 1);
     return mhip::check_launch(c, "matvec_q4");
