@@ -200,3 +200,63 @@ def test_values_that_are_not_finite(g, x, bad, t):
             c.v = was
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("prefix, lens", [(0, [21000]), (20000, [20000, 20007]), (17001, [17100, 17001, 40])])
+def test_more_parts_than_lanes(g, prefix, lens, t):
+    """One head over a long context: a row's results come from more than 64 parts."""
+    rng = np.random.default_rng(22)
+    blocks = -(-max(lens) // 256) + 1
+    c = Cache(g, type=t, n_layers=1, n_kv_heads=1, head_dim=48, page=256, max_blocks=blocks, max_seqs=len(lens) + 1,
+              n_pages=blocks + 4)
+    try:
+        fill(c, lens, prefix, rng)
+        if lens[-1] < prefix:  # a slot that holds the prefix's first tokens and no more
+            for mine in (c.k, c.v):
+                mine[:, c.table[len(lens) - 1][0]] = mine[:, c.table[0][0]]
+            c.load()
+        seqs = list(range(len(lens)))
+        q = rng.standard_normal((len(lens), 2 * 48)) * 2
+        check(c, q, 2, seqs, [1] * len(lens), 1, {prefix, 0}, max(lens), 0.15)
+    finally:
+        c.close()
+
+
+def test_many_slots(g):
+    """More slots than workgroups that run at once, behind a prefix and alone."""
+    rng = np.random.default_rng(23)
+    n = 700
+    c = Cache(g, type=M.MHIP_BF16, n_layers=1, n_kv_heads=2, head_dim=32, max_blocks=6, max_seqs=n, n_pages=6 * n)
+    try:
+        c.extend([0], [40])
+        c.fork([0] * (n - 1), list(range(1, n)))
+        c.extend(list(range(n)), [1 + i % 37 for i in range(n)])
+        seqs = rng.permutation(n).tolist()
+        q = rng.standard_normal((n, 4 * 32))
+        check(c, q, 4, seqs, [1] * n, 1, {40, 0}, 77, 0.2)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_prompt_chunks(g, t):
+    """Many tokens a slot, of different numbers: a prompt's first chunk, one behind a
+    prefix and one that begins inside it."""
+    rng = np.random.default_rng(24)
+    c = Cache(g, type=t, n_layers=1, n_kv_heads=2, head_dim=64, max_blocks=20, max_seqs=4, n_pages=60)
+    try:
+        c.extend([0], [150])
+        c.fork([0, 0], [1, 3])
+        c.extend([1, 2, 3], [77, 130, 1])
+        for mine in (c.k, c.v):  # slot 2 begins with the prefix's tokens
+            for b in range(9):
+                if b < len(c.table[2]) - 1:
+                    mine[:, c.table[2][b]] = mine[:, c.table[0][b]]
+        c.load()
+        seqs, counts, top = [1, 3, 0], [77, 1, 130], 133
+        q = rng.standard_normal((3 * top, 6 * 64))
+        check(c, q, 6, seqs, counts, top, {0, 150, 90}, 227, 0.125)
+        check(c, q, 6, [2, 1, 3], [130, 100, 0], top, {0, 112}, 227, 0.125)
+    finally:
+        c.close()

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import motoria_amd as M
-from shared_model import TYPES, q4_tolerance, q4_weights, rounded
+from shared_model import TYPES, q4_tolerance, q4_weights, rounded, values
 from test_gpu_rows_q4 import product, weights
 
 pytestmark = pytest.mark.gpu
@@ -118,3 +118,28 @@ def test_roundings_of_fp32_do_not_add_up(g, x):
     w, xv = q4_weights(codes, scales, group), rounded(v, M.MHIP_F32)[0]
     o = xv @ w.T
     assert np.linalg.norm(got - o) <= np.linalg.norm(np.abs(xv) @ np.abs(w).T) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows, cols, group, n", [(70, 1024, 32, 1), (12400, 256, 64, 2), (100, 512, 128, 12),
+                                                  (5000, 768, 32, 40), (24600, 256, 64, 20)])
+def test_pointers_aligned_as_their_types(g, rows, cols, group, n, t):
+    """Scales on 2 bytes and results on their own size, between other data."""
+    rng = np.random.default_rng(70)
+    codes, scales = weights(rng, rows, cols, group)
+    v, raw = rounded(rng.standard_normal((n, cols)), t)
+    dt, esz = raw.dtype, raw.dtype.itemsize
+    guard = np.full(n * rows + 2, 0x5a5a, dt)
+    mem = [g.upload(codes), g.upload(np.concatenate([np.full(1, np.nan, np.float16), scales.ravel()])),
+           g.upload(np.ascontiguousarray(raw.reshape(n, cols))), g.upload(guard), g.malloc(M.matvec_q4_ws_bytes(t, cols, n))]
+    try:
+        M.matvec_q4(g, t, mem[3] + esz, rows, mem[0], mem[1] + 2, group, mem[2], cols, rows, cols, n, mem[4])
+        got = g.download(mem[3], guard.shape, dt)
+    finally:
+        for p in mem:
+            g.free(p)
+    assert got[0] == guard[0] and got[-1] == guard[-1]
+    out = values(got[1:-1], t).reshape(n, rows)
+    w, xv = q4_weights(codes, scales, group), v.reshape(n, cols)
+    o = xv @ w.T
+    assert (np.abs(out - o) <= q4_tolerance(w, xv, o, t)).all()
