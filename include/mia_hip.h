@@ -480,8 +480,9 @@ int mhip_chain_f32(mhip_ctx *c, const float *d_v, int n, int mode, float thr, in
 #define MHIP_F32 0 /* element types of the cache, and of rows in and out */
 #define MHIP_F16 1
 #define MHIP_BF16 2
+#define MHIP_Q4 4  /* a cache in 4 bits (below): head_dim a multiple of 32 */
 typedef struct {
-    int type;                           /* MHIP_F32, MHIP_F16, MHIP_BF16 */
+    int type;                           /* MHIP_F32, MHIP_F16, MHIP_BF16, MHIP_Q4 */
     int n_layers, n_kv_heads, head_dim; /* head_dim a multiple of 16, <= 256; heads <= 256 */
     int page;                           /* tokens of a page: 16, 32, 64, 128 or 256 */
     int n_pages;                        /* <= 2^20 */
@@ -489,7 +490,8 @@ typedef struct {
     int max_blocks;                     /* pages of one slot; max_blocks * page <= 2^30 */
 } mhip_page_dims;
 typedef struct {
-    void *k, *v; /* [n_layers][n_pages][n_kv_heads][page][head_dim], 16-byte aligned */
+    void *k, *v; /* [n_layers][n_pages][n_kv_heads][page][head_dim], 16-byte aligned; in 4 bits
+                    [n_layers][n_pages][n_kv_heads][page * head_dim * 5 / 8 bytes] */
     int *table;  /* [max_seqs][max_blocks] page, or -1 */
     int *len;    /* [max_seqs] tokens */
     int *refs;   /* [n_pages] slots that hold the page, 0: free */
@@ -518,7 +520,8 @@ int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, 
                      const void *d_k, const void *d_v, int ld);
 /* The empty slot d_dst[i] becomes a copy of slot d_src[i] (which may repeat,
  * and be no d_dst): full pages are shared, the tokens of a page that is
- * not full are copied to a page of its own, in every layer. MHIP_PAGES_DEEP
+ * not full are copied to a page of its own, in every layer (in 4 bits: the whole
+ * page, as tokens share its words). MHIP_PAGES_DEEP
  * copies every page instead. All n, or (error bits) none. */
 #define MHIP_PAGES_DEEP 1
 int mhip_pages_fork(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, const int *d_src,
@@ -537,6 +540,7 @@ int mhip_pages_compact(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p
  * free pages. */
 #define MHIP_PAGES_NO_SPACE 1 /* too few free pages, or a slot longer than max_blocks */
 #define MHIP_PAGES_BAD 2      /* an index out of range, a slot twice, a d_dst in use */
+#define MHIP_PAGES_NOT_FINITE 4 /* a NaN, or a value beyond +-2^15, on its way into 4 bits */
 int mhip_pages_status(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int status[2]);
 
 /*
@@ -572,6 +576,74 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
                           int n_heads, const void *d_q, int ldq, void *d_out, int ldo,
                           const int *d_seqs, const int *d_count, int n, int max_count,
                           int prefix_seq, int prefix, int max_len, float scale, void *d_ws);
+
+/* ---- a key/value cache in 4 bits, and slots of bounded length ----------------
+ * No counterpart in the reference. A cache of type MHIP_Q4 has the pages, slots
+ * and calls above (all but mhip_pages_write and mhip_attention_shared, which
+ * refuse it) and holds a value as s c + m: a code c of 0 .. 15, and s and m in fp16
+ * for 32 values of a token and head, 5 bits a value in all. The order of a
+ * page's bytes is the library's (csrc/cache_q4.h): the calls here write and read
+ * them. s and m are finite; a program that fills pages by itself keeps them so.
+ *
+ * Rows into the cache, as mhip_pages_write takes them, of `type` (MHIP_F32,
+ * MHIP_F16 or MHIP_BF16): m is the least of 32 values rounded to fp16, s a
+ * fifteenth of what the greatest is above m (0 if it is not), rounded to fp32 and then to
+ * fp16, and c the nearest code (halves up). Values are kept within +-2^15, NaN as 0, with error
+ * bit MHIP_PAGES_NOT_FINITE. d_weights (NULL: none): the tokens' accumulated weights
+ * of this layer (below) become 0. */
+int mhip_pages_write_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,
+                        int type, const int *d_seqs, const int *d_count, int n, int max_count,
+                        const void *d_k, const void *d_v, int ld, float *d_weights);
+/* The way back: the values of the same tokens (the last d_count[i] of each
+ * slot) of one layer, rounded to `type`, into rows of the same form; rows
+ * past d_count[i] are left as they were. A slot twice in the list is no error. */
+int mhip_pages_read_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,
+                       int type, const int *d_seqs, const int *d_count, int n, int max_count,
+                       void *d_k, void *d_v, int ld);
+/*
+ * Attention of one layer over a cache in 4 bits: rows, entries, positions,
+ * limits and errors as of mhip_attention_shared without a prefix (d_q and d_out of
+ * `type`, n * max_count * n_heads at most 2^26 - 4; slots may share pages). Keys enter
+ * as they are; values are rounded once to fp16 for rows of 16 bits and are within 2^-22
+ * for fp32 rows. fp32 queries enter within 2^-22 of each value or 2^-34 of the largest of
+ * their row, 16-bit ones whole, but for what is below 2^-34 of that. Scores,
+ * softmax and sums are fp32; the softmax's weights meet the values within 2^-11 (bf16 rows)
+ * or 2^-22 (fp16, fp32) of their size, or 2^-31 of the largest one.
+ *
+ * d_weights (NULL: not added up): [n_layers][max_seqs][n_kv_heads][max_blocks *
+ * page] floats, mhip_weights_bytes() in all, 16-byte aligned: for each token of a slot
+ * the attention weights that it has got so far, in one layer and head. The call
+ * adds those of its rows, summed over the query heads of a key/value head and
+ * the slot's tokens; a slot is then at most once in the list (its
+ * weights else are those of either entry). Sums do not depend on the order in which
+ * workgroups run. Entries behind a slot's length are left as they were.
+ * d_ws: mhip_attention_q4_ws_bytes() bytes (`weights`: whether d_weights is given), 256-byte
+ * aligned, of one call at a time. */
+size_t mhip_weights_bytes(const mhip_page_dims *s);
+size_t mhip_attention_q4_ws_bytes(const mhip_page_dims *s, int type, int n_heads, int n,
+                                  int max_count, int max_len, int weights);
+int mhip_attention_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer, int type,
+                      int n_heads, const void *d_q, int ldq, void *d_out, int ldo,
+                      const int *d_seqs, const int *d_count, int n, int max_count, int max_len,
+                      float scale, float *d_weights, void *d_ws);
+/* mhip_pages_fork, with the accumulated weights of the copies as their sources'. */
+int mhip_pages_fork_weights(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
+                            float *d_weights, const int *d_src, const int *d_dst, int n, int flags);
+/* Eviction: each slot of the list that is longer than `keep` (1 or more) gets
+ * that length. In every layer and head by itself the last `recent` (<= keep) tokens stay and,
+ * of those before them, the keep - recent of the greatest accumulated weight (of equal ones
+ * the first; NaN counts as less than any), in their order, with their keys,
+ * values and weights, as tokens 0 .. keep - 1. So one token of the slot need not be the
+ * same one in two heads, and a token's place is no longer its position: what
+ * depends on that (rotations) is in the rows before they are written, and
+ * later tokens still attend to all that is left. Pages behind are given back; pages that other
+ * slots hold too are replaced by free ones (in the order of the list). All slots, or (error
+ * bits: a slot twice, one longer than max_len, no page left) none. d_ws:
+ * mhip_pages_evict_ws_bytes() bytes, 256-byte aligned, of one call at a time (0
+ * for invalid arguments). */
+size_t mhip_pages_evict_ws_bytes(const mhip_page_dims *s, int n, int keep, int max_len);
+int mhip_pages_evict(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, float *d_weights,
+                     const int *d_seqs, int n, int keep, int recent, int max_len, void *d_ws);
 
 /* ---- weights in 4 bits ------------------------------------------------------
  * No counterpart in the reference (Q8_0 and fp32 weights). A row of cols

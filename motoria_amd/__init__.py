@@ -31,9 +31,9 @@ MHIP_DECODE_CHAINS_FIRST = 32
 MHIP_ATTN_FORCE_ABORT = 64
 MHIP_CHAIN_SUM, MHIP_CHAIN_GE, MHIP_CHAIN_GT = 0, 1, 2
 MHIP_MODEL_PER_LAYER = 128
-MHIP_F32, MHIP_F16, MHIP_BF16 = 0, 1, 2
+MHIP_F32, MHIP_F16, MHIP_BF16, MHIP_Q4 = 0, 1, 2, 4
 MHIP_PAGES_DEEP = 1
-MHIP_PAGES_NO_SPACE, MHIP_PAGES_BAD = 1, 2
+MHIP_PAGES_NO_SPACE, MHIP_PAGES_BAD, MHIP_PAGES_NOT_FINITE = 1, 2, 4
 MHIP_DECODE_CERTIFIED = 256
 MHIP_FAST_DOWN = 512
 MHIP_MODEL_STACK_MAX_SEQ = 8192  # longest context of the model stack (mia_hip.h)
@@ -206,6 +206,19 @@ SIGNATURES = {
     "mhip_attention_shared_ws_bytes": (_sz, [ctypes.POINTER(PageDims), _i, _i, _i, _i, _i]),
     "mhip_attention_shared": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _i,
                                    _i, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i, _f, _p]),
+    "mhip_pages_write_q4": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _i, _i, _p,
+                                 _p, _i, _i, _p, _p, _i, _p]),
+    "mhip_pages_read_q4": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _i, _i, _p,
+                                _p, _i, _i, _p, _p, _i]),
+    "mhip_weights_bytes": (_sz, [ctypes.POINTER(PageDims)]),
+    "mhip_attention_q4_ws_bytes": (_sz, [ctypes.POINTER(PageDims), _i, _i, _i, _i, _i, _i]),
+    "mhip_attention_q4": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _i, _i, _i, _p,
+                               _i, _p, _i, _p, _p, _i, _i, _i, _f, _p, _p]),
+    "mhip_pages_fork_weights": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _p, _p,
+                                     _p, _i, _i]),
+    "mhip_pages_evict_ws_bytes": (_sz, [ctypes.POINTER(PageDims), _i, _i, _i]),
+    "mhip_pages_evict": (_i, [_p, ctypes.POINTER(PageDims), ctypes.POINTER(PageArrays), _p, _p, _i, _i,
+                              _i, _i, _p]),
     "mhip_quantize_q4": (_i, [_p, _p, _i, _i, _i, _p, _p]),
     "mhip_dequantize_q4": (_i, [_p, _p, _p, _i, _i, _i, _p]),
     "mhip_matvec_q4_ws_bytes": (_sz, [_i, _i, _i]),
@@ -630,6 +643,35 @@ class Pages:
                   prefix_seq, prefix, max_len, scale, d_ws):
         self._call("mhip_attention_shared", layer, n_heads, d_q, ldq, d_out, ldo, d_seqs, d_count, n,
                    max_count, prefix_seq, prefix, max_len, scale, d_ws)
+
+    # -- a cache of type MHIP_Q4
+    def write_q4(self, layer, type, d_seqs, d_count, n, max_count, d_k, d_v, ld, d_weights=None):
+        self._call("mhip_pages_write_q4", layer, type, d_seqs, d_count, n, max_count, d_k, d_v, ld,
+                   d_weights)
+
+    def read_q4(self, layer, type, d_seqs, d_count, n, max_count, d_k, d_v, ld):
+        self._call("mhip_pages_read_q4", layer, type, d_seqs, d_count, n, max_count, d_k, d_v, ld)
+
+    def weights_bytes(self):
+        return lib().mhip_weights_bytes(self._d)
+
+    def attention_q4_ws_bytes(self, type, n_heads, n, max_count, max_len, weights=False):
+        return lib().mhip_attention_q4_ws_bytes(self._d, type, n_heads, n, max_count, max_len,
+                                                int(weights))
+
+    def attention_q4(self, layer, type, n_heads, d_q, ldq, d_out, ldo, d_seqs, d_count, n, max_count,
+                     max_len, scale, d_weights, d_ws):
+        self._call("mhip_attention_q4", layer, type, n_heads, d_q, ldq, d_out, ldo, d_seqs, d_count, n,
+                   max_count, max_len, scale, d_weights, d_ws)
+
+    def fork_weights(self, d_weights, d_src, d_dst, n, flags=0):
+        self._call("mhip_pages_fork_weights", d_weights, d_src, d_dst, n, flags)
+
+    def evict_ws_bytes(self, n, keep, max_len):
+        return lib().mhip_pages_evict_ws_bytes(self._d, n, keep, max_len)
+
+    def evict(self, d_weights, d_seqs, n, keep, recent, max_len, d_ws):
+        self._call("mhip_pages_evict", d_weights, d_seqs, n, keep, recent, max_len, d_ws)
 
 
 def matvec_q4_ws_bytes(type, cols, n):

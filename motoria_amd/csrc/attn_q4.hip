@@ -1,0 +1,132 @@
+// The entry points of the attention over a cache in 4 bits
+// (include/mia_hip.h): arguments, workspace and how a call is cut; its kernels
+// are in attn_q4.inc.
+#include "attn_q4.h"
+
+namespace {
+
+using mhip_q4::Cut;
+using mhip_q4::Job;
+using mhip_q4::PART_MAX;
+using mhip_q4::Stat;
+using mhip_q4::SUM_MAX;
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+int up(long long n, int to) { return (int)((n + to - 1) / to * to); }
+
+// How a call is cut.
+Cut cut_of(const mhip_page_dims *s, int type, int n_heads, int n, int mc, int max_len) {
+    Cut k;
+    const int rows = mc * (n_heads / s->n_kv_heads), step = mhip_q4::WAVES * mhip_q4::TILE;
+    k.nq = rows <= 16 ? 1 : mhip_q4::wide_tiles(type == MHIP_F32, s->head_dim / 32);
+    k.tiles = (rows + 16 * k.nq - 1) / (16 * k.nq);
+    const long long items = (long long)n * s->n_kv_heads * k.tiles;
+    long long parts = (512 + items - 1) / items;
+    const long long most = (max_len + 255) / 256, least = (max_len + PART_MAX - 1) / PART_MAX;
+    if (parts > most) parts = most;
+    if (parts < least) parts = least;
+    if (parts < 1) parts = 1;
+    k.plen = max_len > 0 ? up((max_len + parts - 1) / parts, step) : step;
+    if (k.plen > PART_MAX) k.plen = PART_MAX;
+    k.parts = max_len > 0 ? (max_len + k.plen - 1) / k.plen : 1;
+    const long long each = (long long)max_len * n * s->n_kv_heads / 1024;
+    k.wlen = each < step ? step : each > SUM_MAX ? SUM_MAX : up(each, step);
+    k.wparts = max_len > 0 ? (max_len + k.wlen - 1) / k.wlen : 1;
+    return k;
+}
+
+bool shape_ok(const mhip_page_dims *s, int type, int n_heads, int n, int mc, int max_len) {
+    return s->type == MHIP_Q4 && type >= MHIP_F32 && type <= MHIP_BF16 && n_heads >= 1 && n_heads <= 65536 &&
+           n_heads % s->n_kv_heads == 0 && n >= 1 && n <= s->max_seqs && mc >= 1 &&
+           (long long)n * mc * n_heads <= (1 << 26) - 4 && max_len >= 0 &&
+           max_len <= (long long)s->max_blocks * s->page;
+}
+
+// A launch holds less than 2^32 threads: 2^24 workgroups of 256.
+bool fits(const mhip_page_dims *s, int n, const Cut &k) {
+    const long long items = (long long)n * s->n_kv_heads;
+    return items * k.tiles * k.parts < 1 << 24 && items * k.wparts < 1 << 24;
+}
+
+// The workspace: every part's results and what is kept of them, where there is more
+// than one, and what is kept of each row, where weights are added up.
+struct Work {
+    size_t o, part, row;
+};
+Work work_of(const mhip_page_dims *s, int n_heads, int n, int mc, const Cut &k, bool weights) {
+    const size_t rows = (size_t)n * mc * n_heads, parts = k.parts > 1 ? k.parts : 0;
+    return Work{align256(parts * rows * s->head_dim * 4), align256(parts * rows * sizeof(Stat)),
+                weights ? align256(rows * sizeof(Stat)) : 0};
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mhip_attention_q4_ws_bytes(const mhip_page_dims *s, int type, int n_heads, int n, int max_count, int max_len,
+                                  int weights) {
+    if (!mhip_pages_plan_bytes(s) || !shape_ok(s, type, n_heads, n, max_count, max_len)) return 0;
+    const Cut k = cut_of(s, type, n_heads, n, max_count, max_len);
+    if (!fits(s, n, k)) return 0;
+    const Work w = work_of(s, n_heads, n, max_count, k, weights != 0);
+    return w.o + w.part + w.row + 256;
+}
+
+int mhip_attention_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer, int type, int n_heads,
+                      const void *d_q, int ldq, void *d_out, int ldo, const int *d_seqs, const int *d_count, int n,
+                      int max_count, int max_len, float scale, float *d_weights, void *d_ws) {
+    const char *what = "attention q4";
+    if (mhip::check_pages(c, s, p, what)) return -1;
+    if (s->type != MHIP_Q4) return mhip::fail(c, "%s: a cache of type %d is not in 4 bits", what, s->type);
+    if (type < MHIP_F32 || type > MHIP_BF16) return mhip::fail(c, "%s: rows of type %d", what, type);
+    if (layer < 0 || layer >= s->n_layers) return mhip::fail(c, "%s: layer %d of %d", what, layer, s->n_layers);
+    if (n == 0 || max_count == 0) return 0;
+    if (!shape_ok(s, type, n_heads, n, max_count, max_len))
+        return mhip::fail(c, "%s: %d heads over %d, %d x %d tokens, %d positions", what, n_heads, s->n_kv_heads, n,
+                          max_count, max_len);
+    const int esz = mhip::type_bytes(type);
+    if (ldq < n_heads * s->head_dim || ldo < n_heads * s->head_dim)
+        return mhip::fail(c, "%s: rows %d and %d apart (width %d)", what, ldq, ldo, n_heads * s->head_dim);
+    if (!(scale >= 0x1p-64f && scale <= 0x1p64f))
+        return mhip::fail(c, "%s: scale %g outside [2^-64, 2^64]", what, scale);
+    if (!d_q || !d_out || !d_seqs || !d_ws) return mhip::fail(c, "%s: a null argument", what);
+    if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_weights) % 16 || (size_t)ldq * esz % 16 ||
+        (size_t)ldo * esz % 16 || (uintptr_t)d_ws % 256)
+        return mhip::fail(c, "%s: rows and weights must start on 16 bytes, the workspace on 256", what);
+    const Cut k = cut_of(s, type, n_heads, n, max_count, max_len);
+    if (!fits(s, n, k)) return mhip::fail(c, "%s: too many rows or parts in one call", what);
+    if (mhip::use_device(c)) return -1;
+    const Work w = work_of(s, n_heads, n, max_count, k, d_weights != nullptr);
+    Job a;
+    a.s = *s;
+    a.p = *p;
+    a.layer = layer;
+    a.nh = n_heads;
+    a.group = n_heads / s->n_kv_heads;
+    a.q = d_q;
+    a.ldq = ldq;
+    a.out = d_out;
+    a.ldo = ldo;
+    a.seqs = d_seqs;
+    a.count = d_count;
+    a.n = n;
+    a.mc = max_count;
+    a.max_len = max_len;
+    a.c = scale * 1.44269504088896341f;
+    a.lp = __builtin_ctz(s->page);
+    a.parts = k.parts;
+    a.plen = k.plen;
+    a.tiles = k.tiles;
+    a.o = (float *)d_ws;
+    a.part = (Stat *)((uint8_t *)d_ws + w.o);
+    a.row = (Stat *)((uint8_t *)d_ws + w.o + w.part);
+    a.weights = d_weights;
+    a.wparts = k.wparts;
+    a.wlen = k.wlen;
+    if (type == MHIP_F32) return mhip_q4::launch_f32(c, a, k);
+    if (type == MHIP_F16) return mhip_q4::launch_f16(c, a, k);
+    return mhip_q4::launch_bf16(c, a, k);
+}
+
+}  // extern "C"

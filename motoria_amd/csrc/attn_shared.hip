@@ -71,7 +71,7 @@ Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int 
 }
 
 bool shape_ok(const mhip_page_dims *s, int n_heads, int n, int mc, int prefix, int max_len) {
-    return n_heads >= 1 && n_heads <= 65536 && n_heads % s->n_kv_heads == 0 && n >= 1 &&
+    return s->type != MHIP_Q4 && n_heads >= 1 && n_heads <= 65536 && n_heads % s->n_kv_heads == 0 && n >= 1 &&
            n <= s->max_seqs && mc >= 1 && (long long)n * mc * n_heads < 1 << 26 && prefix >= 0 &&
            max_len >= prefix && max_len <= (long long)s->max_blocks * s->page;
 }
@@ -101,6 +101,7 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
                           int prefix_seq, int prefix, int max_len, float scale, void *d_ws) {
     const char *what = "attention shared";
     if (mhip::check_pages(c, s, p, what)) return -1;
+    if (s->type == MHIP_Q4) return mhip::fail(c, "%s: a cache in 4 bits is read by mhip_attention_q4", what);
     if (layer < 0 || layer >= s->n_layers) return mhip::fail(c, "%s: layer %d of %d", what, layer, s->n_layers);
     if (n == 0 || max_count == 0) return 0;
     if (!shape_ok(s, n_heads, n, max_count, prefix, max_len))

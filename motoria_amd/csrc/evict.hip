@@ -1,0 +1,432 @@
+// Eviction from a cache in 4 bits by accumulated attention weight
+// (include/mia_hip.h). For a slot longer than `keep`, and in each layer and head by
+// itself, the last `recent` tokens and the keep - recent others of the greatest weight stay,
+// in their order, as tokens 0 .. keep - 1.
+//
+//   k_evict_select  a workgroup per slot, layer and head: the least weight that
+//                   stays by three rounds of counting (11, 11 and 10 bits of the weight as a
+//                   whole number), then the positions that stay, in order
+//   k_evict_plan    one workgroup: pages for those that other slots hold too
+//   k_evict_books   tables, lengths and counts; the old and the new pages into the workspace
+//   k_evict_move    a workgroup per slot, layer, head and array moves what stays
+//
+// Tokens only move towards the front, so within a page they move in place: a
+// workgroup takes its tokens in order, 128 at a time, and writes where it has read.
+#include "cache_q4.h"
+#include "pages_plan.h"
+
+namespace {
+
+using mhip_q4::Shape;
+
+constexpr int SEL = 512;        // threads that select
+constexpr int BINS = 2048;
+constexpr int CHUNK = 128;      // tokens that move at a time
+constexpr int MOVE = 256;       // threads that move them
+
+// The workspace of a call.
+struct Work {
+    int *stay;       // [n][layers][heads][keep] positions
+    int *from, *to;  // [n][blocks of max_len], [n][blocks of keep] pages
+    int *need;       // [n] pages shared with others; -1: none moves, -2: a page out of range
+    uint8_t *shared; // [n][blocks of keep]
+    int fb, tb;
+    size_t bytes;
+};
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+Work work_of(const mhip_page_dims *s, int n, int keep, int max_len, void *d_ws) {
+    Work w;
+    const int most = keep < max_len ? keep : max_len;
+    w.fb = (max_len + s->page - 1) / s->page;
+    w.tb = (most + s->page - 1) / s->page;
+    uint8_t *b = (uint8_t *)d_ws;
+    w.bytes = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t *r = b + w.bytes;
+        w.bytes += align256(bytes);
+        return r;
+    };
+    w.need = (int *)take((size_t)n * 4);
+    w.from = (int *)take((size_t)n * w.fb * 4);
+    w.to = (int *)take((size_t)n * w.tb * 4);
+    w.shared = take((size_t)n * w.tb);
+    w.stay = (int *)take((size_t)n * s->n_layers * s->n_kv_heads * most * 4);
+    return w;
+}
+
+// A weight as a whole number of the same order (-0 as 0, NaN below all).
+__device__ __forceinline__ unsigned key_of(float w) {
+    const unsigned u = __float_as_uint(w + 0.0f);
+    return w != w ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ inline int slot_length(const mhip_page_dims &s, const mhip_pages &p, int q, int max_len) {
+    if ((unsigned)q >= (unsigned)s.max_seqs) return -1;
+    const int l = p.len[q];
+    return l > max_len ? -1 : l;
+}
+
+// The pages that entry i's first tokens are in: which of them others hold too.
+__device__ void look_at_pages(const mhip_page_dims &s, const mhip_pages &p, const Work &w, int i, int q, int len,
+                              int *lds) {
+    if (threadIdx.x == 0) lds[0] = lds[1] = 0;
+    __syncthreads();
+    const int have = blocks_of(len, s.page);
+    int bad = 0, held = 0;
+    for (int b = threadIdx.x; b < have; b += SEL) {
+        const int g = p.table[(size_t)q * s.max_blocks + b];
+        if ((unsigned)g >= (unsigned)s.n_pages) {
+            bad = 1;
+        } else if (b < w.tb) {
+            const int is = p.refs[g] > 1;
+            w.shared[(size_t)i * w.tb + b] = (uint8_t)is;
+            held += is;
+        }
+    }
+    if (bad) atomicOr(&lds[1], 1);
+    if (held) atomicAdd(&lds[0], held);
+    __syncthreads();
+    if (threadIdx.x == 0) w.need[i] = lds[1] ? -2 : lds[0];
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(SEL) void k_evict_select(mhip_page_dims s, mhip_pages p, const float *weights,
+                                                      const int *seqs, int n, int keep, int recent, int max_len,
+                                                      Work w) {
+    __shared__ int bins[BINS];
+    __shared__ long long sums[SEL / 64];
+    __shared__ int found[2];
+    const int tid = threadIdx.x;
+    const long long items = (long long)n * s.n_layers * s.n_kv_heads;
+    for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+        const int h = (int)(it % s.n_kv_heads), layer = (int)(it / s.n_kv_heads % s.n_layers);
+        const int i = (int)(it / s.n_kv_heads / s.n_layers), q = seqs[i];
+        const int len = slot_length(s, p, q, max_len);
+        const bool first = h == 0 && layer == 0;
+        if (len <= keep) {
+            if (first && tid == 0) w.need[i] = -1;
+            continue;
+        }
+        if (first) look_at_pages(s, p, w, i, q, len, bins);
+        const float *row = weights + mhip_q4::weights_row(s, layer, q, h);
+        int *stay = w.stay + (size_t)it * keep;
+        const int nc = len - recent, kc = keep - recent;  // candidates, and how many of them stay
+        unsigned least = 0;                               // the least key that stays
+        int equal = kc;                                   // how many of that very key do
+        int taken = 0;                                    // bits of `least` that are known
+        while (kc > 0 && taken < 32) {
+            const int width = taken < 22 ? 11 : 10, shift = 32 - taken - width;
+            for (int b = tid; b < BINS; b += SEL) bins[b] = 0;
+            __syncthreads();
+            for (int x = tid * 4; x < nc; x += SEL * 4) {  // (a row is whole fours of floats)
+                const float4 v = *(const float4 *)(row + x);
+                const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const unsigned k = key_of(f[e]);
+                    if (x + e < nc && (taken == 0 || k >> (32 - taken) == least >> (32 - taken)))
+                        atomicAdd(&bins[k >> shift & ((1u << width) - 1)], 1);
+                }
+            }
+            __syncthreads();
+            // from the highest bin down: the one in which the count reaches `equal`
+            constexpr int EACH = BINS / SEL;
+            const int top = BINS - 1 - tid * EACH;
+            int mine = 0;
+#pragma unroll
+            for (int e = 0; e < EACH; e++) mine += bins[top - e];
+            long long all;
+            int above = (int)scan<SEL>(mine, &all, sums);
+            if (above < equal && above + mine >= equal) {
+                int b = top;
+                while (above + bins[b] < equal) above += bins[b--];
+                found[0] = b;
+                found[1] = equal - above;
+            }
+            __syncthreads();
+            least |= (unsigned)found[0] << shift;
+            equal = found[1];
+            taken += width;
+            __syncthreads();
+        }
+        // the candidates that stay, each thread a run of positions
+        if (kc > 0) {
+            const int run = ((nc + SEL - 1) / SEL + 3) & ~3, x0 = min(nc, tid * run), x1 = min(nc, x0 + run);
+            int more = 0, same = 0;
+            for (int x = x0; x < x1; x += 4) {
+                const float4 v = *(const float4 *)(row + x);
+                const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const unsigned k = key_of(f[e]);
+                    more += x + e < x1 && k > least;
+                    same += x + e < x1 && k == least;
+                }
+            }
+            long long all;
+            const long long before = scan<SEL>((long long)more << 32 | same, &all, sums);
+            more = (int)(before >> 32);
+            same = (int)(before & 0xffffffff);
+            for (int x = x0; x < x1; x += 4) {
+                const float4 v = *(const float4 *)(row + x);
+                const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (x + e >= x1) break;
+                    const unsigned k = key_of(f[e]);
+                    if (k > least || (k == least && same < equal)) stay[more + min(same, equal)] = x + e;
+                    more += k > least;
+                    same += k == least;
+                }
+            }
+        }
+        for (int x = tid; x < recent; x += SEL) stay[kc + x] = nc + x;
+    }
+}
+
+__global__ __launch_bounds__(NT) void k_evict_plan(mhip_page_dims s, mhip_pages p, const int *seqs, int n, int keep,
+                                                   int max_len, Work w) {
+    __shared__ Desk d;
+    const Plan pl = plan_of(p.plan, s.n_pages);
+    int *first, *list;
+    const int want = decide(s, p, d, n, first, list, [&](int i, int &bad) {
+        const int q = seqs[i];
+        if ((unsigned)q >= (unsigned)s.max_seqs || mark(d, q) || p.len[q] < 0 || p.len[q] > max_len ||
+            w.need[i] == -2) {
+            bad = MHIP_PAGES_BAD;
+            return 0LL;
+        }
+        return (long long)max(w.need[i], 0);
+    }, [](int) { return false; });
+    if (threadIdx.x == 0) {
+        pl.head[PL_PAIRS] = 0;
+        pl.head[PL_OK] = want >= 0;
+    }
+    if (want < 0) return;
+    for (int i = threadIdx.x; i < n; i += NT)
+        if (first != pl.first) pl.first[i] = first[i];
+    for (int x = threadIdx.x; x < want; x += NT) {
+        const int g = list[x];
+        if (list != pl.dst) pl.dst[x] = g;
+        p.refs[g] = 1;
+        if (x == want - 1) p.state[ST_HINT] = g + 1;
+    }
+}
+
+__global__ __launch_bounds__(NT) void k_evict_books(mhip_page_dims s, mhip_pages p, const int *seqs, int keep, Work w) {
+    __shared__ long long sums[NT / 64];
+    const Plan pl = plan_of(p.plan, s.n_pages);
+    const int i = blockIdx.x;
+    if (!pl.head[PL_OK] || w.need[i] < 0) return;
+    const int q = seqs[i], have = blocks_of(p.len[q], s.page);
+    int *row = p.table + (size_t)q * s.max_blocks;
+    int next = pl.first[i];
+    for (int b0 = 0; b0 < have; b0 += NT) {
+        const int b = b0 + threadIdx.x;
+        const int g = b < have ? row[b] : -1;
+        const bool front = b < w.tb, swap = front && w.shared[(size_t)i * w.tb + b];
+        long long all;
+        const int at = next + (int)scan<NT>(swap, &all, sums);
+        next += (int)all;
+        if (b >= have) continue;
+        w.from[(size_t)i * w.fb + b] = g;
+        int to = g;
+        if (swap) to = pl.dst[at];
+        if (front) w.to[(size_t)i * w.tb + b] = to;
+        if (swap || !front) {
+            row[b] = front ? to : -1;
+            if (atomicSub(&p.refs[g], 1) == 1) atomicMin(&p.state[ST_HINT], g);
+        }
+    }
+    __syncthreads();  // every thread has read the length
+    if (threadIdx.x == 0) p.len[q] = keep;
+}
+
+// What this thread has read is here, and so is what the others have.
+__device__ __forceinline__ void all_read() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Tokens of a chunk: the block in which each is, and its number there.
+struct Desk2 {
+    const uint8_t *from[CHUNK];
+    uint8_t *to[CHUNK];
+    int a[CHUNK];
+    int moves;
+};
+
+template <int G>
+__global__ __launch_bounds__(MOVE) void k_evict_move(mhip_page_dims s, mhip_pages p, float *weights,
+                                                     const int *seqs, int n, int keep, Work w) {
+    __shared__ Desk2 d;
+    const Shape f = mhip_q4::shape_of(s);
+    if (!plan_of(p.plan, s.n_pages).head[PL_OK]) return;
+    const int tid = threadIdx.x, lp = __builtin_ctz(s.page);
+    const long long items = 2LL * n * s.n_layers * s.n_kv_heads;
+    for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+        const bool keys = it % 2 == 0;
+        const long long list = it / 2;
+        const int h = (int)(list % s.n_kv_heads), layer = (int)(list / s.n_kv_heads % s.n_layers);
+        const int i = (int)(list / s.n_kv_heads / s.n_layers);
+        if (w.need[i] < 0) continue;
+        const int *stay = w.stay + (size_t)list * keep;
+        const int *from = w.from + (size_t)i * w.fb, *to = w.to + (size_t)i * w.tb;
+        uint8_t *base = (uint8_t *)(keys ? p.k : p.v) + ((size_t)layer * s.n_pages * s.n_kv_heads + h) * f.block;
+        const size_t page = s.n_kv_heads * f.block;
+        float *wrow = weights + mhip_q4::weights_row(s, layer, seqs[i], h);
+        for (int r0 = 0; r0 < keep; r0 += CHUNK) {
+            const int m = min(CHUNK, keep - r0);
+            if (tid == 0) d.moves = 0;
+            __syncthreads();
+            if (tid < CHUNK) {
+                // (past the end, in a four that is not whole: the token that is there)
+                const int r = r0 + tid;
+                if (r < keep || (r >> lp < w.tb && r < ((keep + 3) & ~3))) {
+                    const int a = r < keep ? stay[r] : r, g = r < keep ? from[a >> lp] : to[r >> lp];
+                    d.from[tid] = base + (size_t)g * page;
+                    d.to[tid] = base + (size_t)to[r >> lp] * page;
+                    d.a[tid] = a & (s.page - 1);
+                    if (a != r || g != to[r >> lp]) d.moves = 1;
+                }
+            }
+            __syncthreads();
+            if (!d.moves) {
+                __syncthreads();
+                continue;
+            }
+            if (keys) {
+                constexpr int P = (CHUNK * G + MOVE - 1) / MOVE;
+                uint4 code[P];
+                _Float16 sc[P], lo[P];
+                float wt = 0.0f;
+#pragma unroll
+                for (int e = 0; e < P; e++) {
+                    const int x = tid + e * MOVE, t = x / G, j = x % G;
+                    if (t < m) {
+                        const uint8_t *b = d.from[t];
+                        code[e] = *(const uint4 *)(b + mhip_q4::key_word(f, d.a[t], 0, 0) + j * 16);
+                        sc[e] = *(const _Float16 *)(b + mhip_q4::scale_at(f, d.a[t], j));
+                        lo[e] = *(const _Float16 *)(b + mhip_q4::low_at(f, true, d.a[t], j));
+                    }
+                }
+                if (tid < m) wt = wrow[stay[r0 + tid]];
+                all_read();
+#pragma unroll
+                for (int e = 0; e < P; e++) {
+                    const int x = tid + e * MOVE, t = x / G, j = x % G;
+                    if (t < m) {
+                        uint8_t *b = d.to[t];
+                        const int at = (r0 + t) & (s.page - 1);
+                        *(uint4 *)(b + mhip_q4::key_word(f, at, 0, 0) + j * 16) = code[e];
+                        *(_Float16 *)(b + mhip_q4::scale_at(f, at, j)) = sc[e];
+                        *(_Float16 *)(b + mhip_q4::low_at(f, true, at, j)) = lo[e];
+                    }
+                }
+                if (tid < m) wrow[r0 + tid] = wt;
+            } else {
+                constexpr int P = (CHUNK * G + MOVE - 1) / MOVE, W = (CHUNK / 4 * 16 * G + MOVE - 1) / MOVE;
+                _Float16 sc[P], lo[P];
+                unsigned word[W];
+#pragma unroll
+                for (int e = 0; e < W; e++) {
+                    const int x = tid + e * MOVE, four = x / (16 * G), cj = x % (16 * G);
+                    word[e] = 0;
+                    if (four * 4 < m) {
+                        unsigned b[4];
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            const int t = four * 4 + y;
+                            b[y] = d.from[t][mhip_q4::value_byte(f, d.a[t], cj / G, cj % G)];
+                        }
+                        word[e] = b[0] | b[2] << 8 | b[1] << 16 | b[3] << 24;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < P; e++) {
+                    const int x = tid + e * MOVE, t = x / G, j = x % G;
+                    if (t < m) {
+                        sc[e] = *(const _Float16 *)(d.from[t] + mhip_q4::scale_at(f, d.a[t], j));
+                        lo[e] = *(const _Float16 *)(d.from[t] + mhip_q4::low_at(f, false, d.a[t], j));
+                    }
+                }
+                all_read();
+#pragma unroll
+                for (int e = 0; e < W; e++) {
+                    const int x = tid + e * MOVE, four = x / (16 * G), cj = x % (16 * G);
+                    if (four * 4 < m) {
+                        const int at = (r0 + four * 4) & (s.page - 1);
+                        *(unsigned *)(d.to[four * 4] + mhip_q4::value_byte(f, at, cj / G, cj % G)) = word[e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < P; e++) {
+                    const int x = tid + e * MOVE, t = x / G, j = x % G;
+                    if (t < m) {
+                        const int at = (r0 + t) & (s.page - 1);
+                        *(_Float16 *)(d.to[t] + mhip_q4::scale_at(f, at, j)) = sc[e];
+                        *(_Float16 *)(d.to[t] + mhip_q4::low_at(f, false, at, j)) = lo[e];
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+bool shape_ok(const mhip_page_dims *s, int n, int keep, int recent, int max_len) {
+    return s->type == MHIP_Q4 && n >= 1 && n <= s->max_seqs && keep >= 1 && recent >= 0 && recent <= keep &&
+           max_len >= 0 && max_len <= (long long)s->max_blocks * s->page &&
+           (double)n * s->n_layers * s->n_kv_heads * keep < 0x1p58;  // (a workspace of less than 2^60 bytes)
+}
+
+template <int G>
+void move(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, float *weights, const int *seqs, int n, int keep,
+          const Work &w) {
+    const long long items = 2LL * n * s->n_layers * s->n_kv_heads;
+    k_evict_move<G><<<(unsigned)(items < 1 << 20 ? items : 1 << 20), MOVE, 0, c->stream>>>(*s, *p, weights, seqs, n,
+                                                                                         keep, w);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mhip_pages_evict_ws_bytes(const mhip_page_dims *s, int n, int keep, int max_len) {
+    if (!mhip_pages_plan_bytes(s) || !shape_ok(s, n, keep, 0, max_len)) return 0;
+    return work_of(s, n, keep, max_len, nullptr).bytes;
+}
+
+int mhip_pages_evict(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, float *d_weights, const int *d_seqs,
+                     int n, int keep, int recent, int max_len, void *d_ws) {
+    const char *what = "pages evict";
+    if (mhip::check_pages(c, s, p, what) || mhip::check_list(c, s, d_seqs, n, what)) return -1;
+    if (s->type != MHIP_Q4) return mhip::fail(c, "%s: a cache of type %d is not in 4 bits", what, s->type);
+    if (!shape_ok(s, n ? n : 1, keep, recent, max_len))
+        return mhip::fail(c, "%s: %d tokens stay, %d of them the last, slots of up to %d", what, keep, recent, max_len);
+    if (!n) return 0;
+    if (!d_weights || !d_ws) return mhip::fail(c, "%s: a null argument", what);
+    if ((uintptr_t)d_weights % 16 || (uintptr_t)d_ws % 256)
+        return mhip::fail(c, "%s: the weights must start on 16 bytes, the workspace on 256", what);
+    if (mhip::use_device(c)) return -1;
+    const Work w = work_of(s, n, keep, max_len, d_ws);
+    const long long items = (long long)n * s->n_layers * s->n_kv_heads;
+    k_evict_select<<<(unsigned)(items < 1 << 20 ? items : 1 << 20), SEL, 0, c->stream>>>(*s, *p, d_weights, d_seqs, n,
+                                                                                        keep, recent, max_len, w);
+    k_evict_plan<<<1, NT, 0, c->stream>>>(*s, *p, d_seqs, n, keep, max_len, w);
+    k_evict_books<<<n, NT, 0, c->stream>>>(*s, *p, d_seqs, keep, w);
+    switch (s->head_dim / 32) {
+        case 1: move<1>(c, s, p, d_weights, d_seqs, n, keep, w); break;
+        case 2: move<2>(c, s, p, d_weights, d_seqs, n, keep, w); break;
+        case 3: move<3>(c, s, p, d_weights, d_seqs, n, keep, w); break;
+        case 4: move<4>(c, s, p, d_weights, d_seqs, n, keep, w); break;
+        case 5: move<5>(c, s, p, d_weights, d_seqs, n, keep, w); break;
+        case 6: move<6>(c, s, p, d_weights, d_seqs, n, keep, w); break;
+        case 7: move<7>(c, s, p, d_weights, d_seqs, n, keep, w); break;
+        default: move<8>(c, s, p, d_weights, d_seqs, n, keep, w); break;
+    }
+    return mhip::check_launch(c, what);
+}
+
+}  // extern "C"

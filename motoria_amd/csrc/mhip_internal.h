@@ -92,7 +92,14 @@ int launch_down_mfma(hipStream_t st, const mhip_dims *s, const mhip_layout *lay,
 
 // Arguments of the paged cache (pages.hip): 0 or fail().
 int check_pages(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, const char *what);
+int check_list(mhip_ctx *c, const mhip_page_dims *s, const void *list, int n, const char *what);
 inline int type_bytes(int type) { return type == MHIP_F32 ? 4 : 2; }
+constexpr int PLAN_OK = 1;  // the word of mhip_pages.plan that is not 0 once a fork has been decided on
+// Bytes of one page's keys (or values) of one layer and head in 4 bits: half a
+// byte each, and four for every 32 (csrc/cache_q4.h).
+__host__ __device__ inline size_t q4_block(const mhip_page_dims &s) {
+    return (size_t)s.page * s.head_dim / 8 * 5;
+}
 
 }  // namespace mhip
 

@@ -13,151 +13,11 @@
 // 238 MB read and written, 57 us (4.2 TB/s; a large copy reaches 4.92) after a plan
 // of 5.5; 48 forks, 73 MB, 23 us after 6; extend 5.6, a layer's rows of 64 tokens 3.0
 // (each alone; small launches one after another take 3.6).
-#include "mhip_internal.h"
+#include "pages_plan.h"
 
 namespace {
 
-constexpr int NT = 256;                  // a deciding workgroup: barriers of four wavefronts cost
-                                         // 1.5 us less than those of sixteen (extend 7.2 -> 5.6)
-constexpr int WIDE = 1024;               // ... one that goes over every page
-constexpr int PER = 8;                   // pages a thread looks at per round of a scan
-constexpr int SEQ_WORDS = 65536 / 32;    // one bit per slot
-enum { ST_BITS = 0, ST_HINT = 1, ST_FREE = 2 };  // words of mhip_pages.state
-enum { PL_PAIRS = 0, PL_OK = 1, PL_HEAD = 16 };  // words of mhip_pages.plan
-
-// The plan: [PL_HEAD] words, then per page the source, destination and rows of
-// a copy and the page's new index, then per list entry the pages before its own.
-struct Plan {
-    int *head, *src, *dst, *rows, *map, *first;
-};
-__host__ __device__ inline Plan plan_of(int *p, int n_pages) {
-    Plan r;
-    r.head = p;
-    r.src = p + PL_HEAD;
-    r.dst = r.src + n_pages;
-    r.rows = r.dst + n_pages;
-    r.map = r.rows + n_pages;
-    r.first = r.map + n_pages;
-    return r;
-}
-
-// Exclusive prefix sum of v over the workgroup; total in every thread.
-// (Sums of at most n_pages or max_seqs * max_blocks: 64 bits for the latter.)
-template <int N>
-__device__ long long scan(long long v, long long *total, long long *lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    long long s = v;
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long o = __shfl_up(s, d);
-        if (lane >= d) s += o;
-    }
-    if (lane == 63) lds[wave] = s;
-    __syncthreads();
-    long long before = 0, all = 0;
-    for (int w = 0; w < N / 64; w++) {
-        const long long x = lds[w];
-        before += w < wave ? x : 0;
-        all += x;
-    }
-    __syncthreads();
-    *total = all;
-    return before + s - v;
-}
-
-__device__ inline int blocks_of(int tokens, int page) { return (tokens + page - 1) / page; }
-
-// LDS of a workgroup that decides. Its loads depend on each other (entry,
-// length, pages), at about 0.7 us a level, so what can be asked for early is, and
-// lists of up to NT entries and pages stay here.
-struct Desk {
-    unsigned seen[SEQ_WORDS];
-    long long sums[NT / 64];
-    int first[NT], list[NT], slot[NT], len[NT];
-    int bad;
-};
-
-// Which of this thread's PER pages from `base` on are free.
-__device__ unsigned free_mask(const mhip_page_dims &s, const mhip_pages &p, int base) {
-    const int at = base + threadIdx.x * PER;
-    unsigned is = 0;
-#pragma unroll
-    for (int j = 0; j < PER; j++)
-        if (at + j < s.n_pages && p.refs[at + j] <= 0) is |= 1u << j;
-    return is;
-}
-
-// The first `want` free pages in ascending order into out[]; whether there
-// are as many. Every page below `from` (the hint) is in use; is: free_mask there.
-__device__ bool take_free(const mhip_page_dims &s, const mhip_pages &p, int want, int *out, int from,
-                          unsigned is, long long *sums) {
-    int got = 0;
-    for (int base = from; base < s.n_pages && got < want; base += NT * PER) {
-        const int at = base + threadIdx.x * PER;
-        if (base != from) is = free_mask(s, p, base);
-        long long all;
-        int r = got + (int)scan<NT>(__popc(is), &all, sums);
-        for (int j = 0; j < PER; j++)
-            if (is >> j & 1) {
-                if (r < want) out[r] = at + j;
-                r++;
-            }
-        got = min(want, got + (int)all);
-    }
-    __syncthreads();  // out[] is written
-    return got == want;
-}
-
-// The entry whose pages page number x of the call belongs to.
-__device__ inline int entry_of(const int *first, int n, int x) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int m = (lo + hi + 1) >> 1;
-        if (first[m] <= x) lo = m;
-        else hi = m - 1;
-    }
-    return lo;
-}
-
-// What a call over n entries needs: need(i, bad) pages for entry i (and error
-// bits). Takes the pages (list[]) if nothing is wrong, with the prefix sums of the
-// needs in first[]. Returns their number, or -1 with the error bits set.
-// late(i): whether entry i is wrong now that all have been looked at.
-template <class F, class L>
-__device__ int decide(const mhip_page_dims &s, const mhip_pages &p, Desk &d, int n, int *&first,
-                      int *&list, F need, L late) {
-    const Plan pl = plan_of(p.plan, s.n_pages);
-    const int from = max(0, min(p.state[ST_HINT], s.n_pages));
-    const unsigned is = free_mask(s, p, from);
-    for (int i = threadIdx.x; i < (s.max_seqs + 31) / 32; i += NT) d.seen[i] = 0;
-    if (threadIdx.x == 0) d.bad = 0;
-    __syncthreads();
-    first = n <= NT ? d.first : pl.first;
-    long long run = 0;
-    for (int base = 0; base < n; base += NT) {
-        const int i = base + threadIdx.x;
-        long long all;
-        int bad = 0;
-        const long long mine = i < n ? need(i, bad) : 0;
-        if (bad) atomicOr(&d.bad, bad);
-        const long long x = scan<NT>(bad ? 0 : mine, &all, d.sums);
-        if (i < n) first[i] = (int)min(run + x, (long long)1 << 30);
-        run += all;
-    }
-    for (int i = threadIdx.x; i < n; i += NT)
-        if (late(i)) atomicOr(&d.bad, MHIP_PAGES_BAD);
-    __syncthreads();
-    int err = d.bad;
-    list = run <= NT ? d.list : pl.dst;
-    if (!err && (run > s.n_pages || !take_free(s, p, (int)run, list, from, is, d.sums)))
-        err = MHIP_PAGES_NO_SPACE;
-    if (err && threadIdx.x == 0) atomicOr(&p.state[ST_BITS], err);
-    return err ? -1 : (int)run;
-}
-
-// Marks slot q as named by the list; whether it was already.
-__device__ inline bool mark(Desk &d, int q) {
-    return atomicOr(&d.seen[q >> 5], 1u << (q & 31)) >> (q & 31) & 1;
-}
+constexpr int WIDE = 1024;               // a deciding workgroup that goes over every page
 
 __global__ __launch_bounds__(NT) void k_extend(mhip_page_dims s, mhip_pages p, const int *seqs,
                                                const int *count, int n) {
@@ -280,11 +140,13 @@ __global__ __launch_bounds__(WIDE) void k_compact_plan(mhip_page_dims s, mhip_pa
 }
 
 // The plan's copies: an item is one page in one layer of one array, its
-// rows one run per head; 256 threads with four 16-byte pieces each in flight.
+// rows one run per head (in 4 bits the whole page: tokens share its words); 256 threads
+// with four 16-byte pieces each in flight.
 __device__ void copy_pages(const mhip_page_dims &s, const mhip_pages &p, const Plan &pl, int block,
                            int blocks) {
+    const bool whole = s.type == MHIP_Q4;
     const int esz = s.type == MHIP_F32 ? 4 : 2, unit = s.head_dim * esz / 16;  // pieces of a row
-    const size_t head = (size_t)s.page * unit, page = head * s.n_kv_heads;
+    const size_t head = whole ? mhip::q4_block(s) / 16 : (size_t)s.page * unit, page = head * s.n_kv_heads;
     const long long items = (long long)pl.head[PL_PAIRS] * s.n_layers * 2;
     for (long long it = block; it < items; it += blocks) {
         const int x = (int)(it / (2 * s.n_layers)), y = (int)(it % (2 * s.n_layers));
@@ -296,7 +158,7 @@ __device__ void copy_pages(const mhip_page_dims &s, const mhip_pages &p, const P
         uint4 *base = (uint4 *)(y & 1 ? p.v : p.k) + (size_t)(y >> 1) * s.n_pages * page;
         const uint4 *from = base + a * page;
         uint4 *to = base + b * page;
-        const unsigned run = (unsigned)pl.rows[x] * unit, all = run * s.n_kv_heads;
+        const unsigned run = whole ? (unsigned)head : (unsigned)pl.rows[x] * unit, all = run * s.n_kv_heads;
         for (unsigned i = threadIdx.x; i < all; i += 4 * blockDim.x) {
             uint4 r[4];
             size_t o[4];
@@ -442,8 +304,9 @@ __global__ __launch_bounds__(WIDE) void k_status(mhip_page_dims s, mhip_pages p)
 }
 
 bool dims_ok(const mhip_page_dims *s) {
-    return s && s->type >= MHIP_F32 && s->type <= MHIP_BF16 && s->n_layers >= 1 &&
-           s->n_layers <= 65536 && s->n_kv_heads >= 1 && s->n_kv_heads <= 256 && s->head_dim >= 16 &&
+    return s && ((s->type >= MHIP_F32 && s->type <= MHIP_BF16) ||
+                 (s->type == MHIP_Q4 && s->head_dim % 32 == 0)) &&
+           s->n_layers >= 1 && s->n_layers <= 65536 && s->n_kv_heads >= 1 && s->n_kv_heads <= 256 && s->head_dim >= 16 &&
            s->head_dim <= 256 && s->head_dim % 16 == 0 && s->page >= 16 && s->page <= 256 &&
            (s->page & (s->page - 1)) == 0 && s->n_pages >= 1 && s->n_pages <= 1 << 20 &&
            s->max_seqs >= 1 && s->max_seqs <= 65536 && s->max_blocks >= 1 &&
@@ -453,8 +316,9 @@ bool dims_ok(const mhip_page_dims *s) {
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 size_t pool_bytes(const mhip_page_dims *s) {
-    return (size_t)s->n_layers * s->n_pages * s->n_kv_heads * s->page * s->head_dim *
-           mhip::type_bytes(s->type);
+    const size_t blocks = (size_t)s->n_layers * s->n_pages * s->n_kv_heads;
+    if (s->type == MHIP_Q4) return blocks * mhip::q4_block(*s);
+    return blocks * s->page * s->head_dim * mhip::type_bytes(s->type);
 }
 
 // Workgroups for copies of at most `pairs` pages: an item each, at most
@@ -464,16 +328,18 @@ unsigned copy_grid(const mhip_page_dims *s, long long pairs) {
     return (unsigned)(items < 2048 ? items : 2048);
 }
 
-int check_list(mhip_ctx *c, const mhip_page_dims *s, const void *list, int n, const char *what) {
-    if (n < 0 || n > s->max_seqs)
-        return mhip::fail(c, "%s: %d entries, the cache has %d slots", what, n, s->max_seqs);
-    if (n && !list) return mhip::fail(c, "%s: a null argument", what);
-    return 0;
-}
+using mhip::check_list;
 
 }  // namespace
 
 namespace mhip {
+
+int check_list(mhip_ctx *c, const mhip_page_dims *s, const void *list, int n, const char *what) {
+    if (n < 0 || n > s->max_seqs)
+        return fail(c, "%s: %d entries, the cache has %d slots", what, n, s->max_seqs);
+    if (n && !list) return fail(c, "%s: a null argument", what);
+    return 0;
+}
 
 int check_pages(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, const char *what) {
     if (!s || !p) return fail(c, "%s: a null argument", what);
@@ -542,6 +408,7 @@ int mhip_pages_write(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, 
                      const void *d_k, const void *d_v, int ld) {
     if (mhip::check_pages(c, s, p, "pages write") || check_list(c, s, d_seqs, n, "pages write"))
         return -1;
+    if (s->type == MHIP_Q4) return mhip::fail(c, "pages write: a cache in 4 bits takes its rows by mhip_pages_write_q4");
     const int esz = mhip::type_bytes(s->type), width = s->n_kv_heads * s->head_dim;
     if (layer < 0 || layer >= s->n_layers)
         return mhip::fail(c, "pages write: layer %d of %d", layer, s->n_layers);
