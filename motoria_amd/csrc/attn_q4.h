@@ -9,14 +9,17 @@ namespace mhip_q4 {
 
 constexpr int NT = 256, WAVES = 4;
 constexpr int TILE = 32;                 // positions that a wavefront works on at a time
-constexpr int PART_MAX = 4096;           // positions of a part
+constexpr int PART_MAX = 4096;           // positions whose pages are in LDS at a time
 constexpr int PART_PAGES = PART_MAX / 16 + 2;
+constexpr int ITEMS_MAX = 512;           // items of a call that is cut into parts
 constexpr int SUM_MAX = 1024;            // positions of a workgroup that adds weights up
 
-// What is kept of a row and part: the reference of its weights, their sum, and the factor
-// of its scores (scale * log2(e), less the power of two that its queries were taken by).
+// What is kept of a row and part: the reference of its weights, their sum as they enter the
+// products and in fp32 (of a whole row: one over it), the factor of its scores (scale * log2(e), less the
+// powers of two that its queries were taken by), and the positions that it sees.
 struct Stat {
-    float m, l, c, none;
+    float m, l, sum, c;
+    int sees;
 };
 
 // The arguments of one call.
@@ -32,21 +35,26 @@ struct Job {
     int n, mc, max_len;                  // entries, tokens of each at most, positions
     float c;                             // scale * log2(e)
     int lp;                              // log2(page)
-    int parts, plen, tiles;              // parts of a slot, positions of each, row tiles of a slot
-    float *o;                            // partial results [part][row][hd]
-    Stat *part;                          // [part][row]
+    int tiles;                           // row tiles of an entry (each an item)
+    int wgs, least;                      // parts wanted (0: a workgroup an item), steps of one at least
+    float *o;                            // partial results [part][head][row of the tile][hd]
+    Stat *part;                          // [part][head][row of the tile]
     Stat *row;                           // [row]: of all parts
+    int *start;                          // the parts before each item, and all of them
     float *weights;
-    int wparts, wlen;                    // the same for the weights
+    int wparts, wlen;                    // workgroups of a slot and head that add them up, positions of each
+    float *kept;                         // scores of a call with up to 16 rows a slot and head, or null
+    size_t keep_step;                    // of one slot and head
 };
 
 // How a call is cut; nq: tiles of 16 rows of a workgroup.
 struct Cut {
-    int nq, tiles, parts, plen, wparts, wlen;
+    int nq, tiles, wgs, wparts, wlen;
 };
 
-// Tiles of 16 rows of a workgroup that has more than one.
-constexpr int wide_tiles(bool f32, int groups) { return f32 ? (groups > 4 ? 1 : 2) : groups > 4 ? 2 : 4; }
+// Tiles of 16 rows of a workgroup that has more than one (fp32 rows of more than 128 elements leave
+// no registers for a second).
+constexpr int wide_tiles(bool f32, int groups) { return f32 && groups > 4 ? 1 : 2; }
 
 int launch_f32(mhip_ctx *c, const Job &a, const Cut &k);
 int launch_f16(mhip_ctx *c, const Job &a, const Cut &k);

@@ -7,7 +7,6 @@ namespace {
 
 using mhip_q4::Cut;
 using mhip_q4::Job;
-using mhip_q4::PART_MAX;
 using mhip_q4::Stat;
 using mhip_q4::SUM_MAX;
 
@@ -15,23 +14,24 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 int up(long long n, int to) { return (int)((n + to - 1) / to * to); }
 
-// How a call is cut.
+// How a call is cut. Up to 512 positions a workgroup takes an item whole, which saves the join
+// (5 us with its launch). Longer ones are cut into parts for all workgroups to be on their CUs at
+// once, with some to spare, as an item's last part is shorter (two on a CU, one with heads of more than
+// 192 elements, whose stages are large): 32 slots of up to 8000 positions 34.6 us with 448 parts in
+// all, 37.5 with 640, and 40 to 46 where some had to wait for others to end; 16 slots of up to 2900
+// 18.2, 19.2 with 640.
+constexpr int WHOLE = 512, PARTS = 448, PARTS_LARGE = 224, LEAST = 2;
 Cut cut_of(const mhip_page_dims *s, int type, int n_heads, int n, int mc, int max_len) {
     Cut k;
     const int rows = mc * (n_heads / s->n_kv_heads), step = mhip_q4::WAVES * mhip_q4::TILE;
     k.nq = rows <= 16 ? 1 : mhip_q4::wide_tiles(type == MHIP_F32, s->head_dim / 32);
     k.tiles = (rows + 16 * k.nq - 1) / (16 * k.nq);
-    const long long items = (long long)n * s->n_kv_heads * k.tiles;
-    long long parts = (512 + items - 1) / items;
-    const long long most = (max_len + 255) / 256, least = (max_len + PART_MAX - 1) / PART_MAX;
-    if (parts > most) parts = most;
-    if (parts < least) parts = least;
-    if (parts < 1) parts = 1;
-    k.plen = max_len > 0 ? up((max_len + parts - 1) / parts, step) : step;
-    if (k.plen > PART_MAX) k.plen = PART_MAX;
-    k.parts = max_len > 0 ? (max_len + k.plen - 1) / k.plen : 1;
-    const long long each = (long long)max_len * n * s->n_kv_heads / 1024;
-    k.wlen = each < step ? step : each > SUM_MAX ? SUM_MAX : up(each, step);
+    const long long items = (long long)n * k.tiles;
+    const int parts = s->head_dim > 192 ? PARTS_LARGE : PARTS;
+    const bool cut = items <= mhip_q4::ITEMS_MAX && max_len > WHOLE && items * s->n_kv_heads < 4 * parts;
+    k.wgs = cut ? (parts + s->n_kv_heads - 1) / s->n_kv_heads : 0;
+    const long long each = (long long)max_len * n * s->n_kv_heads / (k.nq == 1 ? 2048 : 1024);
+    k.wlen = each < 2 * step ? 2 * step : each > SUM_MAX ? SUM_MAX : up(each, 2 * step);
     k.wparts = max_len > 0 ? (max_len + k.wlen - 1) / k.wlen : 1;
     return k;
 }
@@ -46,18 +46,25 @@ bool shape_ok(const mhip_page_dims *s, int type, int n_heads, int n, int mc, int
 // A launch holds less than 2^32 threads: 2^24 workgroups of 256.
 bool fits(const mhip_page_dims *s, int n, const Cut &k) {
     const long long items = (long long)n * s->n_kv_heads;
-    return items * k.tiles * k.parts < 1 << 24 && items * k.wparts < 1 << 24;
+    return items * k.tiles < 1 << 24 && items * k.wparts < 1 << 24;
 }
 
-// The workspace: every part's results and what is kept of them, where there is more
-// than one, and what is kept of each row, where weights are added up.
+// The workspace: where items are cut, the results of the parts, what is kept of them and
+// where each item's begin; what is kept of each row, where weights are added up.
 struct Work {
-    size_t o, part, row;
+    size_t o, part, row, start, kept, step;
 };
-Work work_of(const mhip_page_dims *s, int n_heads, int n, int mc, const Cut &k, bool weights) {
-    const size_t rows = (size_t)n * mc * n_heads, parts = k.parts > 1 ? k.parts : 0;
-    return Work{align256(parts * rows * s->head_dim * 4), align256(parts * rows * sizeof(Stat)),
-                weights ? align256(rows * sizeof(Stat)) : 0};
+Work work_of(const mhip_page_dims *s, int n_heads, int n, int mc, int max_len, const Cut &k, bool weights) {
+    const size_t parts = k.wgs ? ((size_t)k.wgs + (size_t)n * k.tiles) * s->n_kv_heads * 16 * k.nq : 0;
+    Work w;
+    w.o = align256(parts * s->head_dim * 4);
+    w.part = align256(parts * sizeof(Stat));
+    w.row = weights ? align256((size_t)n * mc * n_heads * sizeof(Stat)) : 0;
+    w.start = k.wgs ? align256(((size_t)n * k.tiles + 1) * 4) : 0;
+    // (whole tiles of 32 positions)
+    w.step = weights && k.nq == 1 && k.tiles == 1 ? (size_t)up(max_len, 32) * mc * (n_heads / s->n_kv_heads) : 0;
+    w.kept = align256(w.step * n * s->n_kv_heads * 4);
+    return w;
 }
 
 }  // namespace
@@ -69,8 +76,8 @@ size_t mhip_attention_q4_ws_bytes(const mhip_page_dims *s, int type, int n_heads
     if (!mhip_pages_plan_bytes(s) || !shape_ok(s, type, n_heads, n, max_count, max_len)) return 0;
     const Cut k = cut_of(s, type, n_heads, n, max_count, max_len);
     if (!fits(s, n, k)) return 0;
-    const Work w = work_of(s, n_heads, n, max_count, k, weights != 0);
-    return w.o + w.part + w.row + 256;
+    const Work w = work_of(s, n_heads, n, max_count, max_len, k, weights != 0);
+    return w.o + w.part + w.row + w.start + w.kept + 256;
 }
 
 int mhip_attention_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer, int type, int n_heads,
@@ -97,7 +104,7 @@ int mhip_attention_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
     const Cut k = cut_of(s, type, n_heads, n, max_count, max_len);
     if (!fits(s, n, k)) return mhip::fail(c, "%s: too many rows or parts in one call", what);
     if (mhip::use_device(c)) return -1;
-    const Work w = work_of(s, n_heads, n, max_count, k, d_weights != nullptr);
+    const Work w = work_of(s, n_heads, n, max_count, max_len, k, d_weights != nullptr);
     Job a;
     a.s = *s;
     a.p = *p;
@@ -115,12 +122,16 @@ int mhip_attention_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
     a.max_len = max_len;
     a.c = scale * 1.44269504088896341f;
     a.lp = __builtin_ctz(s->page);
-    a.parts = k.parts;
-    a.plen = k.plen;
     a.tiles = k.tiles;
-    a.o = (float *)d_ws;
-    a.part = (Stat *)((uint8_t *)d_ws + w.o);
-    a.row = (Stat *)((uint8_t *)d_ws + w.o + w.part);
+    a.wgs = k.wgs;
+    a.least = LEAST;
+    uint8_t *ws = (uint8_t *)d_ws;
+    a.o = (float *)ws;
+    a.part = (Stat *)(ws + w.o);
+    a.row = (Stat *)(ws + w.o + w.part);
+    a.start = (int *)(ws + w.o + w.part + w.row);
+    a.kept = w.kept ? (float *)(ws + w.o + w.part + w.row + w.start) : nullptr;
+    a.keep_step = w.step;
     a.weights = d_weights;
     a.wparts = k.wparts;
     a.wlen = k.wlen;

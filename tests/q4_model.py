@@ -206,35 +206,43 @@ class CacheQ4(Cache):
 
 def attend(q, k, v, scale):
     """A token's heads in 64 bits: q [heads][hd]; k, v as parts() gives them, cut to what it
-    sees. Output, weights [tokens][kv], and how large the sums are that give them."""
+    sees. Output, weights [tokens][kv], the sums of the weights with the sizes of v, of s c and of s c and m
+    apart, and how large the sums are that give the scores."""
     (ks, km), (vs, vm) = k, v
     n, kv, hd = ks.shape
     g = q.shape[0] // kv
-    out, w, size = np.zeros(q.shape), np.zeros((n, kv)), np.zeros(q.shape)
+    out, w, sizes = np.zeros(q.shape), np.zeros((n, kv)), np.zeros((3,) + q.shape)
     err = 0.0
     if n == 0:
-        return out, w, size, err
+        return out, w, sizes, err
     for h in range(q.shape[0]):
-        kk, vv = (ks + km)[:, h // g], (vs + vm)[:, h // g]
+        kk, sc, mm = (ks + km)[:, h // g], vs[:, h // g], vm[:, h // g]
         s = scale * (kk @ q[h])
         e = np.exp(s - s.max())
         e /= e.sum()
-        out[h], size[h] = e @ vv, e @ np.abs(vv)
+        out[h] = e @ (sc + mm)
+        for x, a in zip(sizes, (np.abs(sc + mm), sc, sc + np.abs(mm))):
+            x[h] = e @ a
         w[:, h // g] += e
         err = max(err, scale * ((np.abs(ks) + np.abs(km))[:, h // g] @ np.abs(q[h])).max())
-    return out, w, size, err
+    return out, w, sizes, err
 
 
-def tolerances(t, n, hd, err):
-    """How far results may be off, as factors of the sums of sizes: of an output (before its
-    own rounding) and of a weight. u = 2^-24. A score is a sum of hd products and G of
-    the m, each of them cut or rounded in fp32 (2^-23), G products with s; fp32 queries enter within
+def tolerances(t, n, hd, sizes, err):
+    """How far an output (before its own rounding) may be off, and a weight as a factor of
+    itself. u = 2^-24. A score is a sum of hd products and G of
+    the m, each of them cut or rounded in fp32 (2^-23, and sixteen times that where codes of 16-bit rows are
+    lined up as larger than they are), G products with s; fp32 queries enter within
     2^-22. A weight's relative error is that of its score and of the row's reference, two exponentials'
-    (2^-21) and the sums'. It meets the values within 2^-11 (bf16 rows; fp16's half step)
-    or 2^-22; values are rounded once to fp16 (2^-11), or to 2^-22 for fp32 rows."""
+    (2^-21) and the sums'. A weight enters within half a step of fp16 (2^-11, bf16 rows) or 2^-22 (two
+    pieces) and is the same one for s c and m, so that is an error of it times v; its product with s is rounded by
+    as much again, which is an error of s c alone; and the sums of s c and of m are apart in fp32, a
+    rounding a product (sixteen times that for s c, as above), of their own sizes. fp16's least
+    step adds 2^-30 a weight."""
     u = 2.0 ** -24
-    e = err * ((hd + 16) * 2 * u + (4 * u if t == M.MHIP_F32 else 0))
+    v, sc, both = sizes
+    cut = 1 if t == M.MHIP_F32 else 16
+    e = err * ((hd * cut + 16) * 2 * u + (4 * u if t == M.MHIP_F32 else 0))
     weight = 2 * e + 2.0 ** -21 + (n + 80) * u
-    out = weight + {M.MHIP_F32: 2.0 ** -21, M.MHIP_F16: 2.0 ** -11 + 2.0 ** -22,
-                    M.MHIP_BF16: 2.0 ** -10}[t] + (n + 80) * u
-    return out, weight
+    once = 2.0 ** -11 if t == M.MHIP_BF16 else 2.0 ** -21
+    return (weight + once) * v + once * sc + (n + 80) * u * both + (n / 32 + 8) * cut * 2 * u * sc + n * 2.0 ** -30 * sc, weight

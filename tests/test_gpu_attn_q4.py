@@ -51,13 +51,13 @@ def check(c, layer, t, n_heads, q, seqs, counts, top, max_len, scale, weights=Tr
         k, v = c.parts(0, layer, s), c.parts(1, layer, s)
         for j in range(top):
             see = max(0, c.len[s] - n + j + 1) if j < n else 0
-            o, w, size, err = attend(x[i * top + j], [a[:see] for a in k], [a[:see] for a in v], scale)
-            fo, fw = tolerances(t, see, d.head_dim, err)
+            o, w, sizes, err = attend(x[i * top + j], [a[:see] for a in k], [a[:see] for a in v], scale)
+            off, fw = tolerances(t, see, d.head_dim, sizes, err)
             row = got[i * top + j]
             if see == 0:
                 assert (row == 0).all(), (s, j)
                 continue
-            tol = fo * size + eps / 2 * np.abs(o) * (1 + fo) + 2.0 ** -25
+            tol = off + eps / 2 * (np.abs(o) + off) + 2.0 ** -25
             assert (np.abs(row - o) <= tol).all(), (s, j, np.abs(row - o).max(), (np.abs(row - o) / tol).max())
             want_w[layer, s, :, :see] += w.T
             tol_w[layer, s, :, :see] += fw * w.T
@@ -177,6 +177,29 @@ def test_scores_of_every_size(g, t, spread):
         c.close()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("order", ["up", "down", "spikes"])
+def test_values_of_every_size(g, t, order):
+    """Values that grow or shrink by 2^20 along a slot, so that what a wavefront sees first says nothing about
+    the rest, and single tokens that are far larger than all others; more rows than a tile too."""
+    c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=64, page=16, n_pages=60, max_blocks=50, max_seqs=2)
+    rng = np.random.default_rng(11)
+    n = 780
+    try:
+        size = np.exp2(np.linspace(-8, 12, n))
+        if order == "down":
+            size = size[::-1]
+        elif order == "spikes":
+            size = np.where(np.arange(n) % 97 == 60, 3000.0, 0.01)
+        c.extend([0], [n])
+        k, v = (rng.standard_normal((n, 64)) for _ in (0, 1))
+        c.write_q4(0, t, [0], [n], k, v * size[:, None], n)
+        check(c, 0, t, 4, queries(rng, 3, 4, 64, 0.125), [0], [3], 3, 800, 0.125)
+        check(c, 0, t, 4, queries(rng, 20, 4, 64, 0.125), [0], [20], 20, 800, 0.125)
+    finally:
+        c.close()
+
+
 @pytest.mark.parametrize("scale", [2.0 ** -64, 2.0 ** -20, 2.0 ** 64])
 @pytest.mark.parametrize("t", [M.MHIP_F32, M.MHIP_BF16])
 def test_scales(g, t, scale):
@@ -233,8 +256,9 @@ def test_a_page_out_of_range_counts_as_zeros(g, t):
             k, v = c.parts(0, 0, 0), c.parts(1, 0, 0)
             for a in (*k, *v):
                 a[32:48] = 0
-            o, _, size, err = attend(x, k, v, 0.125)
-            tol = tolerances(t, 70, 64, err)[0] * size + torch.finfo(TORCH[t]).eps * np.abs(o) + 2.0 ** -25
+            o, _, sizes, err = attend(x, k, v, 0.125)
+            off = tolerances(t, 70, 64, sizes, err)[0]
+            tol = off + torch.finfo(TORCH[t]).eps / 2 * (np.abs(o) + off) + 2.0 ** -25
             assert (np.abs(got[0] - o) <= tol).all()
     finally:
         c.close()
@@ -395,9 +419,11 @@ def test_a_pool_behind_32_bits(g):
         ws = up(np.zeros(p.attention_q4_ws_bytes(M.MHIP_F32, 8, 1, 1, 300)), np.uint8)
         p.attention_q4(8, M.MHIP_F32, 8, up(q, np.float32), width, out, width, up([1]), None, 1, 1, 300, 1 / 16, None, ws)
         got = g.download(out, (8, 256), np.float32)
-        o, _, size, err = attend(q.astype(np.float64).reshape(8, 256), (k, 0 * k), (v, 0 * v), 1 / 16)
-        # (s c and m are not apart here: their sizes are at most eight times the sums')
-        tol = tolerances(M.MHIP_F32, 300, 256, 8 * err + 8)[0] * (size + 1) + 2.0 ** -24 * np.abs(o)
+        o, _, sizes, err = attend(q.astype(np.float64).reshape(8, 256), (k, 0 * k), (v, 0 * v), 1 / 16)
+        # (s c and m are not apart here: neither is larger than 16, as no value is beyond +-8)
+        assert np.abs(v).max() < 8 and np.abs(k).max() < 8
+        err += 16 * np.abs(q).sum() / 16
+        tol = tolerances(M.MHIP_F32, 300, 256, np.abs(sizes) + 16, err)[0] + 2.0 ** -24 * np.abs(o)
         assert (np.abs(got - o) <= tol).all()
         assert p.status()[0] == 0
     finally:
