@@ -8,7 +8,7 @@
 //                   whole number), then the positions that stay, in order
 //   k_evict_plan    one workgroup: pages for those that other slots hold too
 //   k_evict_books   tables, lengths and counts; the old and the new pages into the workspace
-//   k_evict_move    a workgroup per slot, layer, head and array moves what stays
+//   k_evict_move    workgroups per slot, layer, head and array move what stays
 //
 // Tokens only move towards the front, so within a page they move in place: a
 // workgroup takes its tokens in order, 128 at a time, and writes where it has read.
@@ -21,8 +21,8 @@ using mhip_q4::Shape;
 
 constexpr int SEL = 512;        // threads that select
 constexpr int BINS = 2048;
-constexpr int CHUNK = 128;      // tokens that move at a time
-constexpr int MOVE = 256;       // threads that move them
+constexpr int CHUNK = 512;      // tokens that move at a time
+constexpr int MOVE = 512;       // threads that move them
 
 // The workspace of a call.
 struct Work {
@@ -249,25 +249,32 @@ __device__ __forceinline__ void all_read() {
     asm volatile("" ::: "memory");
 }
 
-// Tokens of a chunk: the block in which each is, and its number there.
-struct Desk2 {
-    const uint8_t *from[CHUNK];
-    uint8_t *to[CHUNK];
-    int a[CHUNK];
-    int moves;
+// Workgroups that share a head's keys (or values): each moves its part of every token.
+__host__ __device__ constexpr int sides(int groups) { return groups >= 4 ? 4 : groups >= 2 ? 2 : 1; }
+
+// Tokens of a chunk: the page in which each is and will be (of this layer and head), and its number there.
+struct Chunk {
+    unsigned from[CHUNK], to[CHUNK];
+    uint8_t at[CHUNK];
+    int moves[MOVE / 64];
 };
+static_assert(CHUNK <= MOVE, "a thread looks at one token of a chunk");
 
 template <int G>
 __global__ __launch_bounds__(MOVE) void k_evict_move(mhip_page_dims s, mhip_pages p, float *weights,
                                                      const int *seqs, int n, int keep, Work w) {
-    __shared__ Desk2 d;
+    __shared__ Chunk d[3];
     const Shape f = mhip_q4::shape_of(s);
     if (!plan_of(p.plan, s.n_pages).head[PL_OK]) return;
-    const int tid = threadIdx.x, lp = __builtin_ctz(s.page);
-    const long long items = 2LL * n * s.n_layers * s.n_kv_heads;
-    for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    constexpr int SIDES = sides(G), PJ = (G + SIDES - 1) / SIDES, COLS = 16 / SIDES;
+    const int tid = threadIdx.x, lp = __builtin_ctz(s.page), mask = s.page - 1;
+    const long long items = 2LL * n * s.n_layers * s.n_kv_heads, all = (items + 7) / 8 * 8 * SIDES;
+    for (long long b = blockIdx.x; b < all; b += gridDim.x) {
+        // (workgroups that share lines are eight apart, on one XCD)
+        const int side = (int)(b / 8 % SIDES);
+        const long long it = b / (8 * SIDES) * 8 + b % 8, list = it / 2;
         const bool keys = it % 2 == 0;
-        const long long list = it / 2;
+        if (it >= items) continue;
         const int h = (int)(list % s.n_kv_heads), layer = (int)(list / s.n_kv_heads % s.n_layers);
         const int i = (int)(list / s.n_kv_heads / s.n_layers);
         if (w.need[i] < 0) continue;
@@ -276,102 +283,119 @@ __global__ __launch_bounds__(MOVE) void k_evict_move(mhip_page_dims s, mhip_page
         uint8_t *base = (uint8_t *)(keys ? p.k : p.v) + ((size_t)layer * s.n_pages * s.n_kv_heads + h) * f.block;
         const size_t page = s.n_kv_heads * f.block;
         float *wrow = weights + mhip_q4::weights_row(s, layer, seqs[i], h);
+        const int whole = (keep + 3) & ~3;  // (past the end, in a four that is not whole: the token that is there)
+        auto look = [&](Chunk &c, int r0) {
+            bool moves = false;
+            if (tid < CHUNK && r0 + tid < whole) {
+                const int r = r0 + tid, a = r < keep ? stay[r] : r, will = to[r >> lp];
+                const int is = r < keep ? from[a >> lp] : will;
+                c.from[tid] = is;
+                c.to[tid] = will;
+                c.at[tid] = a & mask;
+                moves = a != r || is != will;
+            }
+            moves = __any(moves);
+            if ((tid & 63) == 0) c.moves[tid >> 6] = moves;
+        };
+        int now = 0;
+        look(d[0], 0);
+        __syncthreads();
+        // A turn reads a chunk and finds out what the next one is while that is on its way. Behind the
+        // barrier everyone has read this chunk, so it can be written; the next one's
+        // tokens are all behind it. (Three descriptions, as this one's is still in use then.)
         for (int r0 = 0; r0 < keep; r0 += CHUNK) {
+            const Chunk &c = d[now];
+            now = now == 2 ? 0 : now + 1;
             const int m = min(CHUNK, keep - r0);
-            if (tid == 0) d.moves = 0;
-            __syncthreads();
-            if (tid < CHUNK) {
-                // (past the end, in a four that is not whole: the token that is there)
-                const int r = r0 + tid;
-                if (r < keep || (r >> lp < w.tb && r < ((keep + 3) & ~3))) {
-                    const int a = r < keep ? stay[r] : r, g = r < keep ? from[a >> lp] : to[r >> lp];
-                    d.from[tid] = base + (size_t)g * page;
-                    d.to[tid] = base + (size_t)to[r >> lp] * page;
-                    d.a[tid] = a & (s.page - 1);
-                    if (a != r || g != to[r >> lp]) d.moves = 1;
-                }
-            }
-            __syncthreads();
-            if (!d.moves) {
-                __syncthreads();
-                continue;
-            }
+            bool moves = false;
+#pragma unroll
+            for (int e = 0; e < MOVE / 64; e++) moves |= c.moves[e] != 0;
+            constexpr int P = (CHUNK * PJ + MOVE - 1) / MOVE, W = (CHUNK / 4 * COLS * G + MOVE - 1) / MOVE;
+            _Float16 sc[P], lo[P];
+            float wt = 0.0f;
             if (keys) {
-                constexpr int P = (CHUNK * G + MOVE - 1) / MOVE;
                 uint4 code[P];
-                _Float16 sc[P], lo[P];
-                float wt = 0.0f;
+                if (moves) {
 #pragma unroll
-                for (int e = 0; e < P; e++) {
-                    const int x = tid + e * MOVE, t = x / G, j = x % G;
-                    if (t < m) {
-                        const uint8_t *b = d.from[t];
-                        code[e] = *(const uint4 *)(b + mhip_q4::key_word(f, d.a[t], 0, 0) + j * 16);
-                        sc[e] = *(const _Float16 *)(b + mhip_q4::scale_at(f, d.a[t], j));
-                        lo[e] = *(const _Float16 *)(b + mhip_q4::low_at(f, true, d.a[t], j));
-                    }
-                }
-                if (tid < m) wt = wrow[stay[r0 + tid]];
-                all_read();
-#pragma unroll
-                for (int e = 0; e < P; e++) {
-                    const int x = tid + e * MOVE, t = x / G, j = x % G;
-                    if (t < m) {
-                        uint8_t *b = d.to[t];
-                        const int at = (r0 + t) & (s.page - 1);
-                        *(uint4 *)(b + mhip_q4::key_word(f, at, 0, 0) + j * 16) = code[e];
-                        *(_Float16 *)(b + mhip_q4::scale_at(f, at, j)) = sc[e];
-                        *(_Float16 *)(b + mhip_q4::low_at(f, true, at, j)) = lo[e];
-                    }
-                }
-                if (tid < m) wrow[r0 + tid] = wt;
-            } else {
-                constexpr int P = (CHUNK * G + MOVE - 1) / MOVE, W = (CHUNK / 4 * 16 * G + MOVE - 1) / MOVE;
-                _Float16 sc[P], lo[P];
-                unsigned word[W];
-#pragma unroll
-                for (int e = 0; e < W; e++) {
-                    const int x = tid + e * MOVE, four = x / (16 * G), cj = x % (16 * G);
-                    word[e] = 0;
-                    if (four * 4 < m) {
-                        unsigned b[4];
-#pragma unroll
-                        for (int y = 0; y < 4; y++) {
-                            const int t = four * 4 + y;
-                            b[y] = d.from[t][mhip_q4::value_byte(f, d.a[t], cj / G, cj % G)];
+                    for (int e = 0; e < P; e++) {
+                        const int x = tid + e * MOVE, t = x / PJ, j = x % PJ * SIDES + side;
+                        if (t < m && j < G) {
+                            const uint8_t *b = base + c.from[t] * page;
+                            const int at = c.at[t];
+                            code[e] = *(const uint4 *)(b + mhip_q4::key_word(f, at, 0, 0) + j * 16);
+                            sc[e] = *(const _Float16 *)(b + mhip_q4::scale_at(f, at, j));
+                            lo[e] = *(const _Float16 *)(b + mhip_q4::low_at(f, true, at, j));
                         }
-                        word[e] = b[0] | b[2] << 8 | b[1] << 16 | b[3] << 24;
                     }
+                    if (side == 0 && tid < m) wt = wrow[stay[r0 + tid]];
                 }
-#pragma unroll
-                for (int e = 0; e < P; e++) {
-                    const int x = tid + e * MOVE, t = x / G, j = x % G;
-                    if (t < m) {
-                        sc[e] = *(const _Float16 *)(d.from[t] + mhip_q4::scale_at(f, d.a[t], j));
-                        lo[e] = *(const _Float16 *)(d.from[t] + mhip_q4::low_at(f, false, d.a[t], j));
-                    }
-                }
+                look(d[now], r0 + CHUNK);
                 all_read();
+                if (moves) {
 #pragma unroll
-                for (int e = 0; e < W; e++) {
-                    const int x = tid + e * MOVE, four = x / (16 * G), cj = x % (16 * G);
-                    if (four * 4 < m) {
-                        const int at = (r0 + four * 4) & (s.page - 1);
-                        *(unsigned *)(d.to[four * 4] + mhip_q4::value_byte(f, at, cj / G, cj % G)) = word[e];
+                    for (int e = 0; e < P; e++) {
+                        const int x = tid + e * MOVE, t = x / PJ, j = x % PJ * SIDES + side;
+                        if (t < m && j < G) {
+                            uint8_t *b = base + c.to[t] * page;
+                            const int at = (r0 + t) & mask;
+                            *(uint4 *)(b + mhip_q4::key_word(f, at, 0, 0) + j * 16) = code[e];
+                            *(_Float16 *)(b + mhip_q4::scale_at(f, at, j)) = sc[e];
+                            *(_Float16 *)(b + mhip_q4::low_at(f, true, at, j)) = lo[e];
+                        }
+                    }
+                    if (side == 0 && tid < m) wrow[r0 + tid] = wt;
+                }
+            } else {
+                uint8_t code[W][4];  // (of a word of the destination: a byte of each of its four tokens)
+                if (moves) {
+#pragma unroll
+                    for (int e = 0; e < W; e++) {
+                        const int x = tid + e * MOVE, four = x / (COLS * G), cj = x % (COLS * G) + side * COLS * G;
+                        if (four * 4 < m) {
+#pragma unroll
+                            for (int y = 0; y < 4; y++) {
+                                const int t = four * 4 + y;
+                                code[e][y] = base[c.from[t] * page + mhip_q4::value_byte(f, c.at[t], cj / G, cj % G)];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < P; e++) {
+                        const int x = tid + e * MOVE, t = x / PJ, j = x % PJ * SIDES + side;
+                        if (t < m && j < G) {
+                            const uint8_t *b = base + c.from[t] * page;
+                            sc[e] = *(const _Float16 *)(b + mhip_q4::scale_at(f, c.at[t], j));
+                            lo[e] = *(const _Float16 *)(b + mhip_q4::low_at(f, false, c.at[t], j));
+                        }
                     }
                 }
+                look(d[now], r0 + CHUNK);
+                all_read();
+                if (moves) {
 #pragma unroll
-                for (int e = 0; e < P; e++) {
-                    const int x = tid + e * MOVE, t = x / G, j = x % G;
-                    if (t < m) {
-                        const int at = (r0 + t) & (s.page - 1);
-                        *(_Float16 *)(d.to[t] + mhip_q4::scale_at(f, at, j)) = sc[e];
-                        *(_Float16 *)(d.to[t] + mhip_q4::low_at(f, false, at, j)) = lo[e];
+                    for (int e = 0; e < W; e++) {
+                        const int x = tid + e * MOVE, four = x / (COLS * G), cj = x % (COLS * G) + side * COLS * G;
+                        if (four * 4 < m) {
+                            const int at = (r0 + four * 4) & mask;
+                            // (tokens 0, 2, 1, 3: cache_q4.h)
+                            const unsigned word = code[e][0] | code[e][2] << 8 | code[e][1] << 16 | (unsigned)code[e][3] << 24;
+                            *(unsigned *)(base + c.to[four * 4] * page + mhip_q4::value_byte(f, at, cj / G, cj % G)) = word;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < P; e++) {
+                        const int x = tid + e * MOVE, t = x / PJ, j = x % PJ * SIDES + side;
+                        if (t < m && j < G) {
+                            uint8_t *b = base + c.to[t] * page;
+                            const int at = (r0 + t) & mask;
+                            *(_Float16 *)(b + mhip_q4::scale_at(f, at, j)) = sc[e];
+                            *(_Float16 *)(b + mhip_q4::low_at(f, false, at, j)) = lo[e];
+                        }
                     }
                 }
             }
-            __syncthreads();
         }
+        __syncthreads();  // (the descriptions, for the next item)
     }
 }
 
@@ -384,8 +408,8 @@ bool shape_ok(const mhip_page_dims *s, int n, int keep, int recent, int max_len)
 template <int G>
 void move(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, float *weights, const int *seqs, int n, int keep,
           const Work &w) {
-    const long long items = 2LL * n * s->n_layers * s->n_kv_heads;
-    k_evict_move<G><<<(unsigned)(items < 1 << 20 ? items : 1 << 20), MOVE, 0, c->stream>>>(*s, *p, weights, seqs, n,
+    const long long all = (2LL * n * s->n_layers * s->n_kv_heads + 7) / 8 * 8 * sides(G);
+    k_evict_move<G><<<(unsigned)(all < 1 << 20 ? all : 1 << 20), MOVE, 0, c->stream>>>(*s, *p, weights, seqs, n,
                                                                                          keep, w);
 }
 
