@@ -12,7 +12,8 @@ constexpr int TILE = 32;                 // positions that a wavefront works on 
 constexpr int PART_MAX = 4096;           // positions whose pages are in LDS at a time
 constexpr int PART_PAGES = PART_MAX / 16 + 2;
 constexpr int ITEMS_MAX = 512;           // items of a call that is cut into parts
-constexpr int SUM_MAX = 1024;            // positions of a workgroup that adds weights up
+constexpr int SUM_EACH = 4;              // tiles of a wavefront that adds weights up from new scores
+constexpr int SUM_TILES = SUM_EACH * WAVES;
 
 // What is kept of a row and part: the reference of its weights, their sum as they enter the
 // products and in fp32 (of a whole row: one over it), the factor of its scores (scale * log2(e), less the
@@ -43,18 +44,21 @@ struct Job {
     int *start;                          // the parts before each item, and all of them
     float *weights;
     int wparts, wlen;                    // workgroups of a slot and head that add them up, positions of each
+    int wsides;                          // wavefronts of one that share its positions and take rows in turn
     float *kept;                         // scores of a call with up to 16 rows a slot and head, or null
     size_t keep_step;                    // of one slot and head
 };
 
 // How a call is cut; nq: tiles of 16 rows of a workgroup.
 struct Cut {
-    int nq, tiles, wgs, wparts, wlen;
+    int nq, tiles, wgs, wparts, wlen, wsides;
 };
 
-// Tiles of 16 rows of a workgroup that has more than one (fp32 rows of more than 128 elements leave
-// no registers for a second).
-constexpr int wide_tiles(bool f32, int groups) { return f32 && groups > 4 ? 1 : 2; }
+
+// Tiles of 16 rows of a workgroup that has more than one: two share a tile's codes and s. Heads of more
+// than 128 elements leave no registers for them (a chunk of 500 tokens over 6000, heads of 256: 79 us
+// with one, 84 with two; heads of 128 in fp32 193 with two, 200 with one).
+constexpr int wide_tiles(int groups) { return groups > 4 ? 1 : 2; }
 
 int launch_f32(mhip_ctx *c, const Job &a, const Cut &k);
 int launch_f16(mhip_ctx *c, const Job &a, const Cut &k);

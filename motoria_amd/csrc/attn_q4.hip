@@ -8,7 +8,9 @@ namespace {
 using mhip_q4::Cut;
 using mhip_q4::Job;
 using mhip_q4::Stat;
-using mhip_q4::SUM_MAX;
+using mhip_q4::SUM_EACH;
+using mhip_q4::TILE;
+using mhip_q4::WAVES;
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -21,17 +23,35 @@ int up(long long n, int to) { return (int)((n + to - 1) / to * to); }
 // all, 37.5 with 640, and 40 to 46 where some had to wait for others to end; 16 slots of up to 2900
 // 18.2, 19.2 with 640.
 constexpr int WHOLE = 512, PARTS = 448, PARTS_LARGE = 224, LEAST = 2;
-Cut cut_of(const mhip_page_dims *s, int type, int n_heads, int n, int mc, int max_len) {
+
+// Weights are added up from kept scores where a slot and head have one tile of up to 16 rows, some
+// 2048 workgroups of 256 positions at least (memory is what they wait for). Else they are from
+// new scores, by wavefronts that share positions where there are enough rows for them, with more
+// positions for each once 256 workgroups have some (a chunk of 500 tokens over 6000: 283 us with its
+// attention, 295 with 512 workgroups; 8 drafted tokens of 8 slots of up to 1000, fp32: 34 both).
+constexpr int SUM_WGS = 256;
+bool kept(const Cut &k) { return k.nq == 1 && k.tiles == 1; }
+
+Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int max_len) {
     Cut k;
-    const int rows = mc * (n_heads / s->n_kv_heads), step = mhip_q4::WAVES * mhip_q4::TILE;
-    k.nq = rows <= 16 ? 1 : mhip_q4::wide_tiles(type == MHIP_F32, s->head_dim / 32);
+    const int rows = mc * (n_heads / s->n_kv_heads);
+    k.nq = rows <= 16 ? 1 : mhip_q4::wide_tiles(s->head_dim / 32);
     k.tiles = (rows + 16 * k.nq - 1) / (16 * k.nq);
     const long long items = (long long)n * k.tiles;
     const int parts = s->head_dim > 192 ? PARTS_LARGE : PARTS;
     const bool cut = items <= mhip_q4::ITEMS_MAX && max_len > WHOLE && items * s->n_kv_heads < 4 * parts;
     k.wgs = cut ? (parts + s->n_kv_heads - 1) / s->n_kv_heads : 0;
-    const long long each = (long long)max_len * n * s->n_kv_heads / (k.nq == 1 ? 2048 : 1024);
-    k.wlen = each < 2 * step ? 2 * step : each > SUM_MAX ? SUM_MAX : up(each, 2 * step);
+    const long long heads = (long long)n * s->n_kv_heads;
+    if (kept(k)) {
+        const long long each = max_len * heads / 2048;
+        k.wsides = 1;
+        k.wlen = each < 256 ? 256 : each > 1024 ? 1024 : up(each, 256);
+    } else {
+        k.wsides = k.tiles >= 3 ? 4 : k.tiles;
+        const int side = WAVES / k.wsides;
+        const long long each = (max_len + TILE - 1) / TILE * heads / (SUM_WGS * side);
+        k.wlen = (each < 1 ? 1 : each > SUM_EACH ? SUM_EACH : (int)each) * side * TILE;
+    }
     k.wparts = max_len > 0 ? (max_len + k.wlen - 1) / k.wlen : 1;
     return k;
 }
@@ -62,7 +82,7 @@ Work work_of(const mhip_page_dims *s, int n_heads, int n, int mc, int max_len, c
     w.row = weights ? align256((size_t)n * mc * n_heads * sizeof(Stat)) : 0;
     w.start = k.wgs ? align256(((size_t)n * k.tiles + 1) * 4) : 0;
     // (whole tiles of 32 positions)
-    w.step = weights && k.nq == 1 && k.tiles == 1 ? (size_t)up(max_len, 32) * mc * (n_heads / s->n_kv_heads) : 0;
+    w.step = weights && kept(k) ? (size_t)up(max_len, 32) * mc * (n_heads / s->n_kv_heads) : 0;
     w.kept = align256(w.step * n * s->n_kv_heads * 4);
     return w;
 }
@@ -74,7 +94,7 @@ extern "C" {
 size_t mhip_attention_q4_ws_bytes(const mhip_page_dims *s, int type, int n_heads, int n, int max_count, int max_len,
                                   int weights) {
     if (!mhip_pages_plan_bytes(s) || !shape_ok(s, type, n_heads, n, max_count, max_len)) return 0;
-    const Cut k = cut_of(s, type, n_heads, n, max_count, max_len);
+    const Cut k = cut_of(s, n_heads, n, max_count, max_len);
     if (!fits(s, n, k)) return 0;
     const Work w = work_of(s, n_heads, n, max_count, max_len, k, weights != 0);
     return w.o + w.part + w.row + w.start + w.kept + 256;
@@ -101,7 +121,7 @@ int mhip_attention_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
     if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_weights) % 16 || (size_t)ldq * esz % 16 ||
         (size_t)ldo * esz % 16 || (uintptr_t)d_ws % 256)
         return mhip::fail(c, "%s: rows and weights must start on 16 bytes, the workspace on 256", what);
-    const Cut k = cut_of(s, type, n_heads, n, max_count, max_len);
+    const Cut k = cut_of(s, n_heads, n, max_count, max_len);
     if (!fits(s, n, k)) return mhip::fail(c, "%s: too many rows or parts in one call", what);
     if (mhip::use_device(c)) return -1;
     const Work w = work_of(s, n_heads, n, max_count, max_len, k, d_weights != nullptr);
@@ -135,6 +155,7 @@ int mhip_attention_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p,
     a.weights = d_weights;
     a.wparts = k.wparts;
     a.wlen = k.wlen;
+    a.wsides = k.wsides;
     if (type == MHIP_F32) return mhip_q4::launch_f32(c, a, k);
     if (type == MHIP_F16) return mhip_q4::launch_f16(c, a, k);
     return mhip_q4::launch_bf16(c, a, k);

@@ -127,6 +127,23 @@ def test_lengths(g, t, length):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("count", [12, 30, 70])
+@pytest.mark.parametrize("max_len", [3000, 8000])
+def test_weights_of_many_rows(g, t, count, max_len):
+    """Rows of one, two and more turns, and wavefronts with one to four tiles of positions (as many as
+    max_len gives them), of which slots fill some."""
+    print("test_weights_of_many_rows", t, count, max_len, flush=True)
+    c = CacheQ4(g, n_layers=1, n_kv_heads=8, head_dim=32, page=256, n_pages=8, max_blocks=32, max_seqs=2)
+    rng = np.random.default_rng(count + max_len + t)
+    scale = 32 ** -0.5
+    try:
+        c.fill([0, 1], [645, 75], rng, t)
+        check(c, 0, t, 16, queries(rng, 2 * count, 16, 32, scale), [1, 0], [count - 3, count], count, max_len, scale)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_long_slots_in_parts(g, t):
     """Slots of several parts, of very different lengths; parts that a slot or a row does not reach."""
     c = CacheQ4(g, n_layers=1, n_kv_heads=2, head_dim=32, page=64, n_pages=330, max_blocks=150, max_seqs=4)
