@@ -69,6 +69,37 @@ def test_write_and_read(g, shape, t):
         c.close()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("count", [4, 5, 6, 7, 8, 9, 17])
+def test_tokens_in_fours(g, count, t):
+    """Calls that begin and end anywhere in a four of tokens, and what was there beside them."""
+    print("test_tokens_in_fours", count, t, flush=True)
+    c = CacheQ4(g, n_layers=2, n_kv_heads=2, head_dim=96, page=16, max_seqs=4, max_blocks=4, n_pages=16)
+    rng = np.random.default_rng(10 * count + t)
+    width = 2 * 96
+    try:
+        seqs = [2, 0, 3, 1]
+        for counts in ([0, 1, 2, 3], [count, 3, count - 1, count], [1] * 4, [2, count, count, 1]):
+            c.extend(seqs, counts)
+            k, v = rows(rng, 4 * count, width)
+            for layer in (0, 1):
+                c.write_q4(layer, t, seqs, counts, k, v, count, weights=layer == 0)
+            c.check()
+            blank = np.zeros((4 * count, width * (4 if t == M.MHIP_F32 else 2)), np.uint8)
+            dk, dv = c.up(blank, np.uint8), c.up(blank, np.uint8)
+            c.gpu.read_q4(1, t, c.up(seqs), c.up(counts), 4, count, dk, dv, width)
+            for which, at in ((0, dk), (1, dv)):
+                got = torch.from_numpy(g.download(at, blank.shape, np.uint8)).view(TORCH[t])
+                want = torch.zeros((4 * count, width), dtype=TORCH[t])
+                for i, s in enumerate(seqs):
+                    if counts[i]:
+                        a, b = c.parts(which, 1, s)
+                        want[i * count:i * count + counts[i]] = torch.from_numpy((a + b)[-counts[i]:].reshape(counts[i], -1)).float().to(TORCH[t])
+                assert torch.equal(got, want), (counts, which)
+    finally:
+        c.close()
+
+
 def test_borders_between_codes(g):
     """Values on and next to every border, groups of one value, of the least steps and of large ones."""
     c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=128, n_pages=64, max_seqs=2, max_blocks=60)
