@@ -3,15 +3,15 @@
 // itself, the last `recent` tokens and the keep - recent others of the greatest weight stay,
 // in their order, as tokens 0 .. keep - 1.
 //
-//   k_evict_select  a workgroup per slot, layer and head: the least weight that
-//                   stays by three rounds of counting (11, 11 and 10 bits of the weight as a
-//                   whole number), then the positions that stay, in order
-//   k_evict_plan    one workgroup: pages for those that other slots hold too
-//   k_evict_books   tables, lengths and counts; the old and the new pages into the workspace
-//   k_evict_move    workgroups per slot, layer, head and array move what stays
+//   k_evict_begin  a workgroup per slot, layer and head: the least weight that
+//                  stays by three rounds of counting (11, 11 and 10 bits of the weight as a
+//                  whole number), then the positions that stay, in order; one more keeps the
+//                  books meanwhile (4 short slots 14.9 us in all, with a launch for the plan
+//                  and one for the books 24.9)
+//   k_evict_move   workgroups per slot, layer, head and array move what stays
 //
 // Tokens only move towards the front, so within a page they move in place: a
-// workgroup takes its tokens in order, 128 at a time, and writes where it has read.
+// workgroup takes its tokens in order, 512 at a time, and writes where it has read.
 #include "cache_q4.h"
 #include "pages_plan.h"
 
@@ -66,48 +66,102 @@ __device__ inline int slot_length(const mhip_page_dims &s, const mhip_pages &p, 
     return l > max_len ? -1 : l;
 }
 
-// The pages that entry i's first tokens are in: which of them others hold too.
-__device__ void look_at_pages(const mhip_page_dims &s, const mhip_pages &p, const Work &w, int i, int q, int len,
-                              int *lds) {
-    if (threadIdx.x == 0) lds[0] = lds[1] = 0;
+// The books of a call, by one workgroup beside those that select: pages for those that other
+// slots hold too, tables and counts of references, the old and the new pages into the workspace. A
+// wavefront takes an entry at a time. (Lengths change with the moves: selecting reads them.)
+__device__ void keep_books(const mhip_page_dims &s, const mhip_pages &p, Desk &d, const int *seqs, int n, int keep,
+                           int max_len, const Work &w) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = wave; i < n; i += SEL / 64) {
+        const int q = seqs[i], len = slot_length(s, p, q, max_len);
+        int need = -1;
+        if (len > keep) {
+            const int have = blocks_of(len, s.page);
+            need = 0;
+            for (int b0 = 0; b0 < have; b0 += 64) {
+                const int b = b0 + lane;
+                const int g = b < have ? p.table[(size_t)q * s.max_blocks + b] : 0;
+                const bool bad = (unsigned)g >= (unsigned)s.n_pages, held = !bad && b < have && b < w.tb && p.refs[g] > 1;
+                if (b < have && b < w.tb) w.shared[(size_t)i * w.tb + b] = (uint8_t)held;
+                if (__any(bad)) {
+                    need = -2;
+                    break;
+                }
+                need += __popcll(__ballot(held));
+            }
+        }
+        if (lane == 0) w.need[i] = need;
+    }
     __syncthreads();
-    const int have = blocks_of(len, s.page);
-    int bad = 0, held = 0;
-    for (int b = threadIdx.x; b < have; b += SEL) {
-        const int g = p.table[(size_t)q * s.max_blocks + b];
-        if ((unsigned)g >= (unsigned)s.n_pages) {
-            bad = 1;
-        } else if (b < w.tb) {
-            const int is = p.refs[g] > 1;
-            w.shared[(size_t)i * w.tb + b] = (uint8_t)is;
-            held += is;
+    const Plan pl = plan_of(p.plan, s.n_pages);
+    int *first, *list;
+    const int want = decide<SEL>(s, p, d, n, first, list, [&](int i, int &bad) {
+        const int q = seqs[i];
+        if ((unsigned)q >= (unsigned)s.max_seqs || mark(d, q) || p.len[q] < 0 || p.len[q] > max_len ||
+            w.need[i] == -2) {
+            bad = MHIP_PAGES_BAD;
+            return 0LL;
+        }
+        return (long long)max(w.need[i], 0);
+    }, [](int) { return false; });
+    if (threadIdx.x == 0) {
+        pl.head[PL_PAIRS] = 0;
+        pl.head[PL_OK] = want >= 0;
+    }
+    if (want < 0) return;
+    for (int x = threadIdx.x; x < want; x += SEL) {
+        const int g = list[x];
+        p.refs[g] = 1;
+        if (x == want - 1) p.state[ST_HINT] = g + 1;
+    }
+    __syncthreads();
+    for (int i = wave; i < n; i += SEL / 64) {
+        if (w.need[i] < 0) continue;
+        const int q = seqs[i], have = blocks_of(p.len[q], s.page);
+        int *row = p.table + (size_t)q * s.max_blocks;
+        int next = first[i];
+        for (int b0 = 0; b0 < have; b0 += 64) {
+            const int b = b0 + lane;
+            const bool front = b < w.tb, swap = b < have && front && w.shared[(size_t)i * w.tb + b];
+            const unsigned long long swaps = __ballot(swap);
+            const int at = next + __popcll(swaps & ((1ull << lane) - 1));
+            next += __popcll(swaps);
+            if (b >= have) continue;
+            const int g = row[b], to = swap ? list[at] : g;
+            w.from[(size_t)i * w.fb + b] = g;
+            if (front) w.to[(size_t)i * w.tb + b] = to;
+            if (swap || !front) {
+                row[b] = front ? to : -1;
+                if (atomicSub(&p.refs[g], 1) == 1) atomicMin(&p.state[ST_HINT], g);
+            }
         }
     }
-    if (bad) atomicOr(&lds[1], 1);
-    if (held) atomicAdd(&lds[0], held);
-    __syncthreads();
-    if (threadIdx.x == 0) w.need[i] = lds[1] ? -2 : lds[0];
-    __syncthreads();
 }
 
-__global__ __launch_bounds__(SEL) void k_evict_select(mhip_page_dims s, mhip_pages p, const float *weights,
+__global__ __launch_bounds__(SEL) void k_evict_begin(mhip_page_dims s, mhip_pages p, const float *weights,
                                                       const int *seqs, int n, int keep, int recent, int max_len,
                                                       Work w) {
-    __shared__ int bins[BINS];
-    __shared__ long long sums[SEL / 64];
-    __shared__ int found[2];
+    __shared__ union {
+        Desk desk;
+        struct {
+            int bins[BINS];
+            long long sums[SEL / 64];
+            int found[2];
+        } of;
+    } lds;
+    if (blockIdx.x == 0) {
+        keep_books(s, p, lds.desk, seqs, n, keep, max_len, w);
+        return;
+    }
+    int *bins = lds.of.bins, *found = lds.of.found;
+    long long *sums = lds.of.sums;
     const int tid = threadIdx.x;
     const long long items = (long long)n * s.n_layers * s.n_kv_heads;
-    for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    for (long long it = blockIdx.x - 1; it < items; it += gridDim.x - 1) {
         const int h = (int)(it % s.n_kv_heads), layer = (int)(it / s.n_kv_heads % s.n_layers);
         const int i = (int)(it / s.n_kv_heads / s.n_layers), q = seqs[i];
         const int len = slot_length(s, p, q, max_len);
-        const bool first = h == 0 && layer == 0;
-        if (len <= keep) {
-            if (first && tid == 0) w.need[i] = -1;
-            continue;
-        }
-        if (first) look_at_pages(s, p, w, i, q, len, bins);
+        if (len <= keep) continue;
         const float *row = weights + mhip_q4::weights_row(s, layer, q, h);
         int *stay = w.stay + (size_t)it * keep;
         const int nc = len - recent, kc = keep - recent;  // candidates, and how many of them stay
@@ -184,64 +238,6 @@ __global__ __launch_bounds__(SEL) void k_evict_select(mhip_page_dims s, mhip_pag
     }
 }
 
-__global__ __launch_bounds__(NT) void k_evict_plan(mhip_page_dims s, mhip_pages p, const int *seqs, int n, int keep,
-                                                   int max_len, Work w) {
-    __shared__ Desk d;
-    const Plan pl = plan_of(p.plan, s.n_pages);
-    int *first, *list;
-    const int want = decide(s, p, d, n, first, list, [&](int i, int &bad) {
-        const int q = seqs[i];
-        if ((unsigned)q >= (unsigned)s.max_seqs || mark(d, q) || p.len[q] < 0 || p.len[q] > max_len ||
-            w.need[i] == -2) {
-            bad = MHIP_PAGES_BAD;
-            return 0LL;
-        }
-        return (long long)max(w.need[i], 0);
-    }, [](int) { return false; });
-    if (threadIdx.x == 0) {
-        pl.head[PL_PAIRS] = 0;
-        pl.head[PL_OK] = want >= 0;
-    }
-    if (want < 0) return;
-    for (int i = threadIdx.x; i < n; i += NT)
-        if (first != pl.first) pl.first[i] = first[i];
-    for (int x = threadIdx.x; x < want; x += NT) {
-        const int g = list[x];
-        if (list != pl.dst) pl.dst[x] = g;
-        p.refs[g] = 1;
-        if (x == want - 1) p.state[ST_HINT] = g + 1;
-    }
-}
-
-__global__ __launch_bounds__(NT) void k_evict_books(mhip_page_dims s, mhip_pages p, const int *seqs, int keep, Work w) {
-    __shared__ long long sums[NT / 64];
-    const Plan pl = plan_of(p.plan, s.n_pages);
-    const int i = blockIdx.x;
-    if (!pl.head[PL_OK] || w.need[i] < 0) return;
-    const int q = seqs[i], have = blocks_of(p.len[q], s.page);
-    int *row = p.table + (size_t)q * s.max_blocks;
-    int next = pl.first[i];
-    for (int b0 = 0; b0 < have; b0 += NT) {
-        const int b = b0 + threadIdx.x;
-        const int g = b < have ? row[b] : -1;
-        const bool front = b < w.tb, swap = front && w.shared[(size_t)i * w.tb + b];
-        long long all;
-        const int at = next + (int)scan<NT>(swap, &all, sums);
-        next += (int)all;
-        if (b >= have) continue;
-        w.from[(size_t)i * w.fb + b] = g;
-        int to = g;
-        if (swap) to = pl.dst[at];
-        if (front) w.to[(size_t)i * w.tb + b] = to;
-        if (swap || !front) {
-            row[b] = front ? to : -1;
-            if (atomicSub(&p.refs[g], 1) == 1) atomicMin(&p.state[ST_HINT], g);
-        }
-    }
-    __syncthreads();  // every thread has read the length
-    if (threadIdx.x == 0) p.len[q] = keep;
-}
-
 // What this thread has read is here, and so is what the others have.
 __device__ __forceinline__ void all_read() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -282,7 +278,9 @@ __global__ __launch_bounds__(MOVE) void k_evict_move(mhip_page_dims s, mhip_page
         const int *from = w.from + (size_t)i * w.fb, *to = w.to + (size_t)i * w.tb;
         uint8_t *base = (uint8_t *)(keys ? p.k : p.v) + ((size_t)layer * s.n_pages * s.n_kv_heads + h) * f.block;
         const size_t page = s.n_kv_heads * f.block;
-        float *wrow = weights + mhip_q4::weights_row(s, layer, seqs[i], h);
+        const int q = seqs[i];
+        float *wrow = weights + mhip_q4::weights_row(s, layer, q, h);
+        if (keys && h == 0 && layer == 0 && side == 0 && tid == 0) p.len[q] = keep;
         const int whole = (keep + 3) & ~3;  // (past the end, in a four that is not whole: the token that is there)
         auto look = [&](Chunk &c, int r0) {
             bool moves = false;
@@ -436,10 +434,8 @@ int mhip_pages_evict(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, 
     if (mhip::use_device(c)) return -1;
     const Work w = work_of(s, n, keep, max_len, d_ws);
     const long long items = (long long)n * s->n_layers * s->n_kv_heads;
-    k_evict_select<<<(unsigned)(items < 1 << 20 ? items : 1 << 20), SEL, 0, c->stream>>>(*s, *p, d_weights, d_seqs, n,
-                                                                                        keep, recent, max_len, w);
-    k_evict_plan<<<1, NT, 0, c->stream>>>(*s, *p, d_seqs, n, keep, max_len, w);
-    k_evict_books<<<n, NT, 0, c->stream>>>(*s, *p, d_seqs, keep, w);
+    k_evict_begin<<<(unsigned)(items < 1 << 20 ? items : 1 << 20) + 1, SEL, 0, c->stream>>>(
+        *s, *p, d_weights, d_seqs, n, keep, recent, max_len, w);
     switch (s->head_dim / 32) {
         case 1: move<1>(c, s, p, d_weights, d_seqs, n, keep, w); break;
         case 2: move<2>(c, s, p, d_weights, d_seqs, n, keep, w); break;

@@ -9,6 +9,7 @@ namespace {
 
 constexpr int NT = 256;                  // a deciding workgroup: barriers of four wavefronts cost
                                          // 1.5 us less than those of sixteen (extend 7.2 -> 5.6)
+constexpr int MOST_THREADS = 512;        // of a workgroup that decides beside others' work (evict.hip)
 constexpr int PER = 8;                   // pages a thread looks at per round of a scan
 constexpr int SEQ_WORDS = 65536 / 32;    // one bit per slot
 enum { ST_BITS = 0, ST_HINT = 1, ST_FREE = 2 };  // words of mhip_pages.state
@@ -60,7 +61,7 @@ __device__ inline int blocks_of(int tokens, int page) { return (tokens + page - 
 // lists of up to NT entries and pages stay here.
 struct Desk {
     unsigned seen[SEQ_WORDS];
-    long long sums[NT / 64];
+    long long sums[MOST_THREADS / 64];
     int first[NT], list[NT], slot[NT], len[NT];
     int bad;
 };
@@ -77,14 +78,15 @@ __device__ unsigned free_mask(const mhip_page_dims &s, const mhip_pages &p, int 
 
 // The first `want` free pages in ascending order into out[]; whether there
 // are as many. Every page below `from` (the hint) is in use; is: free_mask there.
+template <int N>
 __device__ bool take_free(const mhip_page_dims &s, const mhip_pages &p, int want, int *out, int from,
                           unsigned is, long long *sums) {
     int got = 0;
-    for (int base = from; base < s.n_pages && got < want; base += NT * PER) {
+    for (int base = from; base < s.n_pages && got < want; base += N * PER) {
         const int at = base + threadIdx.x * PER;
         if (base != from) is = free_mask(s, p, base);
         long long all;
-        int r = got + (int)scan<NT>(__popc(is), &all, sums);
+        int r = got + (int)scan<N>(__popc(is), &all, sums);
         for (int j = 0; j < PER; j++)
             if (is >> j & 1) {
                 if (r < want) out[r] = at + j;
@@ -111,33 +113,33 @@ __device__ inline int entry_of(const int *first, int n, int x) {
 // bits). Takes the pages (list[]) if nothing is wrong, with the prefix sums of the
 // needs in first[]. Returns their number, or -1 with the error bits set.
 // late(i): whether entry i is wrong now that all have been looked at.
-template <class F, class L>
+template <int N = NT, class F, class L>
 __device__ int decide(const mhip_page_dims &s, const mhip_pages &p, Desk &d, int n, int *&first,
                       int *&list, F need, L late) {
     const Plan pl = plan_of(p.plan, s.n_pages);
     const int from = max(0, min(p.state[ST_HINT], s.n_pages));
     const unsigned is = free_mask(s, p, from);
-    for (int i = threadIdx.x; i < (s.max_seqs + 31) / 32; i += NT) d.seen[i] = 0;
+    for (int i = threadIdx.x; i < (s.max_seqs + 31) / 32; i += N) d.seen[i] = 0;
     if (threadIdx.x == 0) d.bad = 0;
     __syncthreads();
     first = n <= NT ? d.first : pl.first;
     long long run = 0;
-    for (int base = 0; base < n; base += NT) {
+    for (int base = 0; base < n; base += N) {
         const int i = base + threadIdx.x;
         long long all;
         int bad = 0;
         const long long mine = i < n ? need(i, bad) : 0;
         if (bad) atomicOr(&d.bad, bad);
-        const long long x = scan<NT>(bad ? 0 : mine, &all, d.sums);
+        const long long x = scan<N>(bad ? 0 : mine, &all, d.sums);
         if (i < n) first[i] = (int)min(run + x, (long long)1 << 30);
         run += all;
     }
-    for (int i = threadIdx.x; i < n; i += NT)
+    for (int i = threadIdx.x; i < n; i += N)
         if (late(i)) atomicOr(&d.bad, MHIP_PAGES_BAD);
     __syncthreads();
     int err = d.bad;
     list = run <= NT ? d.list : pl.dst;
-    if (!err && (run > s.n_pages || !take_free(s, p, (int)run, list, from, is, d.sums)))
+    if (!err && (run > s.n_pages || !take_free<N>(s, p, (int)run, list, from, is, d.sums)))
         err = MHIP_PAGES_NO_SPACE;
     if (err && threadIdx.x == 0) atomicOr(&p.state[ST_BITS], err);
     return err ? -1 : (int)run;
