@@ -157,6 +157,84 @@ def test_long_slots_in_parts(g, t):
         c.close()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,kv,hd", [(12, 4, 64), (5, 1, 96), (16, 2, 160), (8, 2, 256), (20, 1, 256), (40, 8, 128)])
+def test_parts_of_every_layout(g, t, heads, kv, hd):
+    print("test_parts_of_every_layout", t, heads, kv, hd, flush=True)
+    c = CacheQ4(g, n_layers=1, n_kv_heads=kv, head_dim=hd, page=64, n_pages=60, max_blocks=25, max_seqs=3)
+    rng = np.random.default_rng(heads + hd + t)
+    scale = hd ** -0.5
+    try:
+        c.fill([0, 1, 2], [1500, 650, 1101], rng, t)
+        check(c, 0, t, heads, queries(rng, 3, heads, hd, scale), [1, 0, 2], None, 1, 1600, scale)
+        check(c, 0, t, heads, queries(rng, 9, heads, hd, scale), [2, 1, 0], [3, 0, 2], 3, 1500, scale)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_slots_longer_than_a_window_of_pages(g, t):
+    """Where there are many items a workgroup goes through a long slot by itself, 4096 positions' pages at a
+    time: tiles of many rows, and one token of many slots, whose scores are kept for the weights. As the values
+    grow it goes through it twice."""
+    print("test_slots_longer_than_a_window_of_pages", t, flush=True)
+    scale = 32 ** -0.5
+    for n, kv, heads, top, seqs in ((8, 1, 32, 65, [5, 0, 1, 2, 3, 4, 6, 7]), (230, 8, 16, 1, list(range(230)))):
+        c = CacheQ4(g, n_layers=1, n_kv_heads=kv, head_dim=32, page=64, n_pages=n + 80, max_blocks=75, max_seqs=n)
+        rng = np.random.default_rng(n + t)
+        try:
+            lens = [4700 if s == 5 else 1 + s % 60 for s in range(n)]
+            others = [s for s in range(n) if s != 5]
+            c.fill(others, [lens[s] for s in others], rng, t)
+            c.extend([5], [4700])
+            k, v = (rng.standard_normal((4700, kv * 32)) for _ in (0, 1))
+            v *= np.exp2(np.linspace(-8, 12, 4700))[:, None]
+            c.write_q4(0, t, [5], [4700], k, v, 4700)
+            sizes = M.lib().mhip_attention_q4_ws_bytes(ctypes.byref(c.d), t, heads, n, top, 4800, 0)
+            assert sizes == 256  # not cut into parts
+            counts = None if top == 1 else [min(top, lens[s]) for s in seqs]
+            check(c, 0, t, heads, queries(rng, n * top, heads, 32, scale), seqs, counts, top, 4800, scale)
+        finally:
+            c.close()
+
+
+def test_two_contexts_at_once(g):
+    """Two contexts (streams), each with a cache, weights and a workspace of its own and calls queued in turn
+    without a wait, give what each gives alone."""
+    rng = np.random.default_rng(17)
+    other = M.Gpu()
+    caches = []
+    try:
+        for gpu in (g, other):
+            c = CacheQ4(gpu, n_layers=1, n_kv_heads=2, head_dim=128, page=32, max_blocks=40, max_seqs=6, n_pages=220)
+            caches.append(c)
+            c.fill(list(range(6)), [900 + 30 * i for i in range(6)], rng, M.MHIP_F16)
+            c.dq = c.up(c.rows_of(rng.standard_normal((6, 8 * 128)), 0, M.MHIP_F16)[0], np.uint8)
+            c.out = c.up(np.zeros((6, 2048)), np.uint8)
+            c.ws = c.up(np.zeros(c.gpu.attention_q4_ws_bytes(M.MHIP_F16, 8, 6, 1, 1200, True)), np.uint8)
+            c.seqs = c.up(np.arange(6))
+
+        def step(c):
+            c.gpu.attention_q4(0, M.MHIP_F16, 8, c.dq, 1024, c.out, 1024, c.seqs, None, 6, 1, 1200, 0.09, c.d_w, c.ws)
+        alone = []
+        for c in caches:
+            c.set_weights(np.zeros_like(c.w))
+            for _ in range(20):
+                step(c)
+            alone.append((c.g.download(c.out, (6, 2048), np.uint8), c.g.download(c.d_w, c.w.shape, np.float32)))
+            c.set_weights(np.zeros_like(c.w))
+        for _ in range(20):
+            for c in caches:
+                step(c)
+        for c, (out, w) in zip(caches, alone):
+            assert np.array_equal(c.g.download(c.out, (6, 2048), np.uint8), out) and out.any()
+            assert np.array_equal(c.g.download(c.d_w, c.w.shape, np.float32).view(np.uint32), w.view(np.uint32))
+    finally:
+        for c in caches:
+            c.close()
+        other.close()
+
+
 def test_parts_are_as_planned():
     """The long slots of the test above are cut: their workspace holds parts."""
     d = M.PageDims(M.MHIP_Q4, 1, 2, 32, 64, 330, 4, 150)
