@@ -66,10 +66,11 @@ bool shape_ok(const mhip_page_dims *s, int type, int n_heads, int n, int mc, int
            max_len <= (long long)s->max_blocks * s->page;
 }
 
-// A launch holds less than 2^32 threads: 2^24 workgroups of 256.
+// A launch holds less than 2^32 threads: 2^24 workgroups of 256 (those that add weights up have up to 2^19
+// more beside them, which join parts).
 bool fits(const mhip_page_dims *s, int n, const Cut &k) {
     const long long items = (long long)n * s->n_kv_heads;
-    return items * k.tiles < 1 << 24 && items * k.wparts < 1 << 24;
+    return items * k.tiles < 1 << 24 && items * k.wparts < (1 << 24) - (1 << 19);
 }
 
 // The workspace: where items are cut, the results of the parts, what is kept of them and
