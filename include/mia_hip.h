@@ -619,7 +619,8 @@ int mhip_pages_read_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p
  * weights else are those of either entry). Sums do not depend on the order in which
  * workgroups run. Entries behind a slot's length are left as they were.
  * d_ws: mhip_attention_q4_ws_bytes() bytes (`weights`: whether d_weights is given), 256-byte
- * aligned, of one call at a time. */
+ * aligned, of one call at a time. (With weights and up to 16 rows a slot and key/value head
+ * it holds their scores: 4 bytes for each row and each position up to max_len.) */
 size_t mhip_weights_bytes(const mhip_page_dims *s);
 size_t mhip_attention_q4_ws_bytes(const mhip_page_dims *s, int type, int n_heads, int n,
                                   int max_count, int max_len, int weights);
