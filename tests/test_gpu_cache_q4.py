@@ -223,6 +223,22 @@ def test_evict_many_tokens(g):
         c.close()
 
 
+def test_evict_forks_of_many_pages(g):
+    """More entries than wavefronts keep books, more pages of each than lanes, most of them shared: with each other,
+    with a slot that is not in the list, or with none."""
+    c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=32, page=16, n_pages=1300, max_blocks=100, max_seqs=14)
+    rng = np.random.default_rng(6)
+    try:
+        c.fill([3, 9, 0, 5], [1490, 1300, 40, 1184], rng)
+        c.fork_weights([3, 3, 3, 3, 9, 9, 5, 5, 0], [1, 2, 4, 6, 7, 8, 10, 11, 12])
+        c.set_weights(rng.random(c.w.shape).astype(np.float32))
+        c.check()
+        c.evict([4, 1, 7, 9, 12, 10, 2, 6, 8, 0, 11, 5], 1100, 100)   # (slot 3 keeps its pages)
+        c.check()
+    finally:
+        c.close()
+
+
 def test_evict_refuses_whole_calls(g):
     """A slot twice, out of range or too long, and too few pages: nothing changes but the error bits."""
     c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=32, page=16, n_pages=12, max_blocks=8, max_seqs=4)
