@@ -16,8 +16,8 @@
 // 8000 tokens to 4000 in 48 layers of 4 heads of 128: selecting 17 us (a row of weights is read five
 // times, from the cache after the first), moving 126, where a copy of the bytes would take 51: a
 // value's code is a byte of a word of four tokens, and the chunks of a head have to follow each
-// other. (Chunks of 128: 258 us. A chunk asked for while the one before is written: the same 126,
-// in twice the registers.)
+// other. (Chunks of 128 whose places are looked up in turn: 258 us. A chunk asked for while the one
+// before is written: the same 126, in twice the registers.)
 #include "cache_q4.h"
 #include "pages_plan.h"
 
