@@ -606,10 +606,9 @@ int mhip_pages_read_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p
  * `type`, n * max_count * n_heads at most 2^26 - 4; slots may share pages). Keys and
  * values enter as they are. fp32 queries enter within 2^-22 of each value or 2^-34 of the
  * largest of their row, 16-bit ones whole, but for what is below 2^-34 of that.
- * Scores, softmax and sums are fp32; a weight enters the sum over the values within 2^-11 (bf16
- * rows) or 2^-22 (fp16, fp32) of its size, its product with s within as much again, or both
- * within 2^-30 of the row's largest weight. The weights' own sums are of unrounded ones
- * (fp16 and fp32 rows: within 2^-22).
+ * Scores, softmax and sums are fp32; a weight enters the sums over the values and over the weights
+ * within 2^-22 of its size, its product with s within as much again, or both
+ * within 2^-30 of the row's largest weight.
  *
  * d_weights (NULL: not added up): [n_layers][max_seqs][n_kv_heads][max_blocks *
  * page] floats, mhip_weights_bytes() in all, 16-byte aligned: for each token of a slot

@@ -15,11 +15,11 @@ constexpr int ITEMS_MAX = 512;           // items of a call that is cut into par
 constexpr int SUM_EACH = 4;              // tiles of a wavefront that adds weights up from new scores
 constexpr int SUM_TILES = SUM_EACH * WAVES;
 
-// What is kept of a row and part: the reference of its weights, their sum as they enter the
-// products and in fp32 (of a whole row: one over it), the factor of its scores (scale * log2(e), less the
+// What is kept of a row and part: the reference of its weights, their sum (of a whole
+// row: one over it), the factor of its scores (scale * log2(e), less the
 // powers of two that its queries were taken by), and the positions that it sees.
-struct Stat {
-    float m, l, sum, c;
+struct alignas(16) Stat {
+    float m, l, c;
     int sees;
 };
 
