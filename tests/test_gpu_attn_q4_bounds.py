@@ -83,3 +83,40 @@ def test_one_rounding(g, t, heads, kv, hd, length, count):
         check(c, t, heads, q.reshape(count, -1), [0], [count], count, length, 1.0, length // 128 + 1)
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [32, 128])
+def test_scores_of_queries_of_far_apart_sizes(g, t, hd):
+    """A query with one element of 512 at a code of 1, one at a code of 0 and the others of about 2^-14 at codes
+    of 15: all that is small has to reach the score. Seen by the weights, which are fp32. A score is off by 33 cuts
+    of 2^-23 of its largest product (34 with the product with s); what is small is 2^-14 of it in all."""
+    print("test_scores_of_queries_of_far_apart_sizes", t, hd, flush=True)
+    n = 60
+    c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=hd, page=16, max_seqs=2)
+    try:
+        step = np.linspace(2.0 ** -10, 1, n).astype(np.float16).astype(np.float32)  # a token's s, 15 of which are fp16's too
+        code = np.full(hd, 15.0, np.float32)
+        code[0], code[1] = 1, 0
+        code[32::32] = 0  # (a least value of 0 in every group)
+        c.extend([0], [n])
+        k = step[:, None] * code
+        c.write_q4(0, t, [0], [n], k, np.zeros_like(k), n)
+        q = np.full((1, hd), 2.0 ** -14 * 1.5, np.float32)
+        q[0, 0], q[0, 1], q[0, 32::32] = 512, 0, 0
+        scale = 2.0 ** -6
+        x = c.rows_of(q, 0, t)[1].astype(np.float64).reshape(1, hd)
+        ks, km = c.parts(0, 0, 0)
+        assert (km == 0).all() and (ks[:, 0, 0] > 0).all()
+        start = np.zeros_like(c.w)
+        c.set_weights(start)
+        call(c, 0, t, 1, q, [0], None, 1, 144, scale)
+        got = g.download(c.d_w, c.w.shape, np.float32)[0, 0, 0, :n].astype(np.float64)
+        _, w, _, err = attend(x, (ks, km), c.parts(1, 0, 0), scale)
+        less = np.abs(ks[:, 0, 2:] @ x[0, 2:] * scale).max()
+        e = err * (34 * 2.0 ** -23 + (2.0 ** -22 if t == M.MHIP_F32 else 0))
+        tol = 2 * e + 2.0 ** -21 + 2.0 ** -20
+        assert less > 3 * tol  # (a score without them is seen)
+        assert (np.abs(got / w[:, 0] - 1) <= tol).all(), np.abs(got / w[:, 0] - 1).max() / tol
+    finally:
+        c.close()
