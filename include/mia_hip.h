@@ -607,8 +607,11 @@ int mhip_pages_read_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p
  * values enter as they are. fp32 queries enter within 2^-22 of each value or 2^-34 of the
  * largest of their row, 16-bit ones whole, but for what is below 2^-34 of that.
  * Scores, softmax and sums are fp32; a weight enters the sums over the values and over the weights
- * within 2^-22 of its size, its product with s within as much again, or both
- * within 2^-30 of the row's largest weight.
+ * within 2^-22 of its size or 2^-34 of the row's largest; its product with s within 2^-21 of its
+ * size, or the products of a row and 32 values are, all together, within 2^-20 (16-bit rows 2^-16) of
+ * the sum of weight x 15 s over the tokens that the row sees. (Values whose sizes are so far apart that
+ * the fast way would be off by more are worked on twice.) Sums over an m below 2^-14 are within
+ * 2^-14 of their size.
  *
  * d_weights (NULL: not added up): [n_layers][max_seqs][n_kv_heads][max_blocks *
  * page] floats, mhip_weights_bytes() in all, 16-byte aligned: for each token of a slot

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import motoria_amd as M
-from q4_model import CacheQ4, attend
+from q4_model import CacheQ4
 from shared_model import TYPES
 from test_gpu_attn_q4 import call
 
@@ -27,43 +27,72 @@ def half_step(t, x):
     return np.exp2(np.maximum(np.floor(np.log2(np.abs(x) + 1e-300)), least)) * half
 
 
-def bound(t, see, sizes, err, tiles):
-    """How far an output may be off before its own rounding.
-    A score: products of 32 elements, each summed by the matrix cores within 32 cuts of 2^-23 of the largest
-    size, then a product with s and a sum (2^-23), and the m in one more; fp32 queries enter within 2^-22. Its
+def rows_of(q, k, v, scale):
+    """A token's heads in 64 bits, as q4_model.attend: output, weights [heads][tokens] and how large the sums
+    are that give the scores."""
+    (ks, km), (vs, vm) = k, v
+    g = q.shape[0] // ks.shape[1]
+    at = np.arange(q.shape[0]) // g
+    s = scale * np.einsum("hd,thd->ht", q, (ks + km)[:, at])
+    w = np.exp(s - s.max(1, keepdims=True))
+    w /= w.sum(1, keepdims=True)
+    err = scale * np.einsum("hd,thd->ht", np.abs(q), (np.abs(ks) + np.abs(km))[:, at]).max()
+    return np.einsum("ht,thd->hd", w, (vs + vm)[:, at]), w, err
+
+
+def bound(t, w, v, err, tiles, products=32):
+    """How far an output may be off before its own rounding, and a weight as a factor of itself.
+    A score: `products` of queries and codes that are not 0, each cut at 2^-23 of the largest by the matrix cores, a
+    product with s and a sum (2^-23 each), and the m in one more; fp32 queries enter within 2^-22. Its
     weight is off by twice that (its own and the reference's), two exponentials' 2^-21 and the sums'. Weights enter
-    within 2^-22 of their size or 2^-36 of the row's largest, their products with s as well or, all of them, within
-    2^-20 (16-bit rows 2^-16) of the sum they belong to. Sums over the tokens: a wavefront adds
-    32 at a time (2^-22 of the sum so far each), then wavefronts and parts are joined (2^-20)."""
-    v, sc, both = sizes
-    e = err * (34 * 2.0 ** -23 + (2.0 ** -22 if t == M.MHIP_F32 else 0))
-    weight = 2 * e + 2.0 ** -21 + 2.0 ** -22
-    sums = tiles * 2.0 ** -22 + 2.0 ** -20
-    group = np.repeat(sc.reshape(*sc.shape[:-1], -1, 32).max(-1), 32, -1)
+    within 2^-23 of their size or 2^-34 of the row's largest (or as nothing), their products with s within 3 2^-23 or, all
+    of them, within 2^-20 (16-bit rows 2^-16) of the group's largest sum of weight x s x code, which is no more than that
+    of weight x 15 s. Sums over the tokens: a wavefront adds 32 at a time (2^-22 of the sum so far each),
+    then wavefronts and parts are joined (2^-20)."""
+    (vs, vm), g = v, w.shape[0] // v[0].shape[1]
+    at = np.arange(w.shape[0]) // g
+    e = err * ((products + 2) * 2.0 ** -23 + (2.0 ** -22 if t == M.MHIP_F32 else 0))
+    weight = 2 * e + 2.0 ** -21 + 2.0 ** -22 + tiles * 2.0 ** -22 + 2.0 ** -20
     few = 2.0 ** -20 if t == M.MHIP_F32 else 2.0 ** -16
-    # (the greatest of a group's sums is 7 / 15 of the sum of 15 s w at least: its codes are 0 and 14 or 15 in each token,
-    # and those of these tests are spread evenly)
-    return weight * v + sums * both + few * 15 / 7 * group + 2.0 ** -21 * both
+    n = vs.shape[0]
+    most = vs.reshape(n, vs.shape[1], -1, 32).max(-1) * (15 / 14)  # (of 32 codes the greatest is 14 or 15)
+    group = np.repeat(np.einsum("ht,thg->hg", w, most[:, at]), 32, -1)
+    both = np.einsum("ht,thd->hd", w, (vs + np.abs(vm))[:, at])
+    off = weight * both + few * group
+    lost = np.einsum("ht,thd->hd", np.minimum(w, 2.0 ** -34 * w.max(1, keepdims=True)), (vs + np.abs(vm))[:, at])
+    return off + 2.0 ** -22 * both + lost, weight
 
 
-def check(c, t, heads, q, seqs, counts, top, max_len, scale, tiles):
-    """Rows held to the bound and one rounding. Returns how far they are off in units of the tolerance."""
+def check(c, t, heads, q, seqs, counts, top, max_len, scale, tiles, products=32, weights=False):
+    """Rows held to the bound and one rounding, and the weights added up to theirs; prints how far they are off in
+    units of that."""
     d = c.d
-    got = call(c, 0, t, heads, q, seqs, counts, top, max_len, scale, weights=False)
+    if weights:
+        c.set_weights(np.zeros_like(c.w))
+    got = call(c, 0, t, heads, q, seqs, counts, top, max_len, scale, weights=weights)
     x = c.rows_of(q, 0, t)[1].astype(np.float64).reshape(len(seqs) * top, heads, d.head_dim)
+    want, tol_w = np.zeros(c.w.shape), np.zeros(c.w.shape)
     for i, s in enumerate(seqs):
         n = top if counts is None else counts[i]
         k, v = c.parts(0, 0, s), c.parts(1, 0, s)
         for j in range(n):
             see = c.len[s] - n + j + 1
-            o, w, sizes, err = attend(x[i * top + j], [a[:see] for a in k], [a[:see] for a in v], scale)
-            largest = np.abs((v[0] + v[1])[:see]).max() if see else 0.0
-            off = bound(t, see, sizes, err, tiles) + see * 2.0 ** -36 * largest
+            seen = [a[:see] for a in v]
+            o, w, err = rows_of(x[i * top + j], [a[:see] for a in k], seen, scale)
+            off, fw = bound(t, w, seen, err, tiles, products)
             row = got[i * top + j]
-            tol = off + half_step(t, np.abs(o) + off) + 2.0 ** -25
-            over = np.abs(row - o) / tol
+            tol = off + half_step(t, np.abs(o) + off)
+            over = np.abs(row - o) / (tol + 1e-300)
             print("row", s, j, "of", see, "worst", over.max(), "of the tolerance", flush=True)
             assert (over <= 1).all(), (s, j, np.abs(row - o).max(), over.max(), (over > 1).mean())
+            sums = w.reshape(d.n_kv_heads, -1, see).sum(1)
+            want[0, s, :, :see] += sums
+            # (a weight of less than fp32's least is nothing)
+            tol_w[0, s, :, :see] += (fw + see * 2.0 ** -34) * sums + 2.0 ** -120
+    if weights:
+        got_w = c.g.download(c.d_w, c.w.shape, np.float32).astype(np.float64)
+        tol_w += (heads * top + 8) * 2.0 ** -24 * want
+        assert (np.abs(got_w - want) <= tol_w).all(), (np.abs(got_w - want) / (tol_w + 1e-300)).max()
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -112,11 +141,126 @@ def test_scores_of_queries_of_far_apart_sizes(g, t, hd):
         c.set_weights(start)
         call(c, 0, t, 1, q, [0], None, 1, 144, scale)
         got = g.download(c.d_w, c.w.shape, np.float32)[0, 0, 0, :n].astype(np.float64)
-        _, w, _, err = attend(x, (ks, km), c.parts(1, 0, 0), scale)
+        _, w, err = rows_of(x, (ks, km), c.parts(1, 0, 0), scale)
         less = np.abs(ks[:, 0, 2:] @ x[0, 2:] * scale).max()
         e = err * (34 * 2.0 ** -23 + (2.0 ** -22 if t == M.MHIP_F32 else 0))
         tol = 2 * e + 2.0 ** -21 + 2.0 ** -20
         assert less > 3 * tol  # (a score without them is seen)
-        assert (np.abs(got / w[:, 0] - 1) <= tol).all(), np.abs(got / w[:, 0] - 1).max() / tol
+        assert (np.abs(got / w[0] - 1) <= tol).all(), np.abs(got / w[0] - 1).max() / tol
+    finally:
+        c.close()
+
+
+def one_far_ahead(c, t, n, heads, gap, values, seq=0):
+    """A slot of n tokens of which the first gets a score that is `gap` powers of two above the others', which are
+    all 0; its own values are 0. Returns the query: one element, so that scores are one product."""
+    d = c.d
+    c.extend([seq], [n])
+    k = np.zeros((n, d.n_kv_heads, d.head_dim), np.float32)
+    k[0, :, 0] = 15
+    c.write_q4(0, t, [seq], [n], k.reshape(n, -1), values, n)
+    q = np.zeros((1, heads, d.head_dim))
+    q[:, :, 0] = gap * np.log(2) / 15
+    return q.reshape(1, -1)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [32, 160])
+@pytest.mark.parametrize("size,gap", [(1.0, 20.6), (750.0, 23.2), (7500.0, 22.2), (32000.0, 20.6), (7500.0, 30.0), (0.01, 25.0)])
+def test_small_weights_of_large_values(g, t, hd, size, gap):
+    """One weight of 1, at values of 0, and all others 2^-20 and less, at values of one size: what is small is all
+    that there is. In one launch, in parts, and with weights added up in both ways."""
+    print("test_small_weights_of_large_values", t, hd, size, gap, flush=True)
+    rng = np.random.default_rng(int(gap * 10) + hd)
+    for n, heads, top_len in ((500, 2, 500), (1500, 2, 1600), (500, 40, 500)):
+        c = CacheQ4(g, n_layers=1, n_kv_heads=2, head_dim=hd, page=64, n_pages=30, max_blocks=25, max_seqs=2)
+        try:
+            v = size * (0.5 + 0.5 * rng.random((n, 2 * hd))) * np.where(np.arange(2 * hd) % 3 == 0, -1, 1)
+            v[0] = 0
+            q = one_far_ahead(c, t, n, heads, gap, v)
+            check(c, t, heads, q, [0], None, 1, top_len, 1.0, n // 128 + 1, 1, weights=True)
+        finally:
+            c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_values_that_a_row_does_not_see(g, t):
+    """Tokens of 2^15 within the first tile that the first rows do not see: they change nothing of those."""
+    c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=64, page=16, n_pages=30, max_blocks=5, max_seqs=2)
+    rng = np.random.default_rng(3)
+    try:
+        for seq, (n, count) in enumerate(((30, 20), (70, 50))):
+            c.extend([seq], [n])
+            k, v = (rng.standard_normal((n, 64)) for _ in (0, 1))
+            v *= np.where(np.arange(n) < n - count + 3, 0.01, 30000)[:, None]
+            c.write_q4(0, t, [seq], [n], k, np.clip(v, -32768, 32768), n)
+            q = np.zeros((count, 4, 64))
+            q[:, np.arange(4), rng.integers(0, 64, 4)] = 1.5
+            check(c, t, 4, q.reshape(count, -1), [seq], [count], count, n, 1.0, 1, 1)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_large_values_of_no_weight(g, t):
+    """Tokens of 2^15, the first of a slot or some of each tile, whose weights are 2^-60: what they add is far
+    below what the others', of 0.01 and less, come to."""
+    rng = np.random.default_rng(4)
+    for n, top_len, which in ((300, 300, "first"), (300, 300, "some"), (1200, 1300, "some")):
+        c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=64, page=16, n_pages=90, max_blocks=85, max_seqs=1)
+        try:
+            large = np.arange(n) < 20 if which == "first" else np.arange(n) % 31 == 7
+            c.extend([0], [n])
+            k = np.zeros((n, 64), np.float32)
+            k[large, 0] = -15
+            v = rng.standard_normal((n, 64)) * np.where(large, 1e5, 0.01 if which == "first" else 0.0005)[:, None]
+            c.write_q4(0, t, [0], [n], k, np.clip(v, -32768, 32768), n)
+            q = np.zeros((1, 4, 64))
+            q[:, :, 0] = 60 * np.log(2) / 15
+            check(c, t, 4, q.reshape(1, -1), [0], None, 1, top_len, 1.0, n // 128 + 1, 1)
+        finally:
+            c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,hd", [(4, 96), (20, 256)])
+def test_groups_of_far_apart_sizes(g, t, heads, hd):
+    """Groups of 32 channels from 2^15 down to 2^-13, one of zeros, in every token."""
+    c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=hd, page=16, n_pages=20, max_blocks=13, max_seqs=1)
+    rng = np.random.default_rng(5)
+    n = 200
+    try:
+        c.extend([0], [n])
+        k, v = (rng.standard_normal((n, hd)) for _ in (0, 1))
+        size = np.exp2(np.linspace(13, -13, hd // 32))
+        size[1] = 0
+        c.write_q4(0, t, [0], [n], k, np.clip(v * np.repeat(size, 32), -32768, 32768), n)
+        q = np.zeros((1, heads, hd))
+        q[:, np.arange(heads), rng.integers(0, hd, heads)] = 1.5
+        got = call(c, 0, t, heads, q.reshape(1, -1), [0], None, 1, n, 1.0, weights=False)
+        assert (got[0, :, 32:64] == 0).all()
+        check(c, t, heads, q.reshape(1, -1), [0], None, 1, n, 1.0, 2, 1)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("t", [M.MHIP_F32, M.MHIP_BF16])
+def test_the_largest_s(g, t):
+    """Pages that a program fills by itself: any s and m that are finite."""
+    c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=64, page=16, n_pages=8, max_blocks=5, max_seqs=1)
+    rng = np.random.default_rng(6)
+    try:
+        c.fill([0], [77], rng, t)
+        _, _, scale, low = c.at[1]
+        for i, p in enumerate(c.table[0]):
+            for r in range(16):
+                for j in range(0, 64, 32):
+                    s, m = np.float16(65504 if r % 3 else 9000), np.float16((-1) ** r * 65504)
+                    c.v[0, p, 0, scale[r, j]:scale[r, j] + 2] = np.array([s]).view(np.uint8)
+                    c.v[0, p, 0, low[r, j]:low[r, j] + 2] = np.array([m]).view(np.uint8)
+        g.check(M.lib().mhip_h2d(g.h, c.gpu.arrays.v, c.v.ctypes.data, c.v.nbytes), "h2d")
+        q = np.zeros((1, 3, 64))
+        q[:, np.arange(3), [5, 40, 63]] = 2.0
+        check(c, t, 3, q.reshape(1, -1), [0], None, 1, 77, 1.0, 1, 1)
     finally:
         c.close()
