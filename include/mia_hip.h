@@ -619,7 +619,8 @@ int mhip_pages_read_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p
  * adds those of its rows, summed over the query heads of a key/value head and
  * the slot's tokens; a slot is then at most once in the list (its
  * weights else are those of either entry). Sums do not depend on the order in which
- * workgroups run. Entries behind a slot's length are left as they were.
+ * workgroups run. Entries behind a slot's length are left as they were. A row whose query
+ * is not finite gives NaN, and makes NaN of the weights of all that it sees, in its key/value head.
  * d_ws: mhip_attention_q4_ws_bytes() bytes (`weights`: whether d_weights is given), 256-byte
  * aligned, of one call at a time. (With weights and up to 16 rows a slot and key/value head
  * it holds their scores: 4 bytes for each row and each position up to max_len.) */

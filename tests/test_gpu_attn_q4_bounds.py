@@ -264,3 +264,35 @@ def test_the_largest_s(g, t):
         check(c, t, 3, q.reshape(1, -1), [0], None, 1, 77, 1.0, 1, 1)
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,lens", [(4, (100, 40)), (4, (1500, 700)), (40, (100, 40))])
+def test_weights_of_queries_that_are_not_finite(g, t, heads, lens):
+    """A row whose query is not finite makes NaN of the weights of the positions that it sees, in its key/value
+    head and slot, and of no others: scores kept and formed again, in one launch and in parts."""
+    print("test_weights_of_queries_that_are_not_finite", t, heads, lens, flush=True)
+    c = CacheQ4(g, n_layers=1, n_kv_heads=2, head_dim=64, page=64, n_pages=50, max_blocks=25, max_seqs=3)
+    rng = np.random.default_rng(heads)
+    try:
+        c.fill([0, 2], list(lens), rng, t)
+        q = rng.standard_normal((6, heads * 64))
+        start = np.zeros_like(c.w)
+        c.set_weights(start)
+        good = call(c, 0, t, heads, q, [0, 2], [3, 3], 3, lens[0], 0.125)
+        well = g.download(c.d_w, c.w.shape, np.float32)
+        q[1, 5] = np.nan              # slot 0, its second new token, head 0 of the first key/value head
+        q[3, 64 * heads - 7] = -np.inf  # slot 2, the first one, the last head
+        c.set_weights(start)
+        got = call(c, 0, t, heads, q, [0, 2], [3, 3], 3, lens[0], 0.125)
+        w = g.download(c.d_w, c.w.shape, np.float32)
+        bad = np.zeros((6, heads), bool)
+        bad[1, 0] = bad[3, heads - 1] = True
+        assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], good[~bad])
+        spoiled = np.zeros(w.shape, bool)
+        spoiled[0, 0, 0, :lens[0] - 1] = spoiled[0, 2, 1, :lens[1] - 2] = True
+        assert np.isnan(w[spoiled]).all()
+        assert np.array_equal(w[~spoiled], well[~spoiled])
+        assert c.gpu.status()[0] == 0
+    finally:
+        c.close()
