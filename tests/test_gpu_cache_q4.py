@@ -424,3 +424,28 @@ def test_pages_behind_32_bits(g):
         for h in held:
             g.free(h)
         p.close()
+
+
+def test_calls_of_more_entries_than_a_workgroup(g):
+    """Forks with weights and evictions of more slots than the deciding workgroup keeps in LDS (256) and than it
+    has threads (512): short slots, most of which share their first page."""
+    c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=32, page=16, n_pages=2000, max_seqs=640, max_blocks=3)
+    rng = np.random.default_rng(12)
+    try:
+        c.fill(list(range(40)), [17 + i % 20 for i in range(40)], rng)
+        c.set_weights(rng.integers(0, 9, c.w.shape).astype(np.float32) / 8)
+        dst = rng.permutation(np.arange(40, 640)).tolist()
+        c.fork_weights([i % 40 for i in range(300)], dst[:300])
+        c.check()
+        c.fork_weights([(7 * i) % 40 for i in range(300)], dst[300:])
+        c.check()
+        c.evict(rng.permutation(640)[:300].tolist(), 20, 5)
+        c.check()
+        c.evict(rng.permutation(640).tolist(), 9, 3)  # every slot, in one page each
+        c.check()
+        c.evict(rng.permutation(640).tolist() , 9, 3)  # none is longer
+        c.check()
+        c.evict(dst[:299] + [dst[0]], 4, 0, max_len=48, model=False)  # a slot twice, the last of many
+        c.check(M.MHIP_PAGES_BAD)
+    finally:
+        c.close()
