@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import motoria_amd as M
-from q4_model import CacheQ4
+from q4_model import CacheQ4, codes_of
 from shared_model import TYPES
 from test_gpu_attn_q4 import call
 
@@ -296,3 +296,95 @@ def test_weights_of_queries_that_are_not_finite(g, t, heads, lens):
         assert c.gpu.status()[0] == 0
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("order", ["up", "down", "mixed"])
+@pytest.mark.parametrize("heads,top", [(4, 3), (40, 3)])
+def test_scores_of_thousands(g, t, order, heads, top):
+    """Scores up to 20000, at least 30 apart: a row is the values of the greatest it sees, rounded, with a weight
+    of 1 (of the two pieces of a weight 2^-21, of its product with s 2^-20 or 2^-16, of the reference that
+    is the score itself nothing), and the others add less than 2^-40."""
+    print("test_scores_of_thousands", t, order, heads, top, flush=True)
+    n = 290
+    c = CacheQ4(g, n_layers=1, n_kv_heads=2, head_dim=64, page=16, n_pages=40, max_blocks=20, max_seqs=2)
+    rng = np.random.default_rng(8)
+    try:
+        size = {"up": np.arange(1, n + 1), "down": np.arange(n, 0, -1), "mixed": rng.permutation(n) + 1}[order] * 1.5
+        k = np.zeros((n, 2, 64))
+        k[:, :, 7] = size[:, None]
+        v = rng.standard_normal((n, 128))
+        c.extend([1], [n])
+        c.write_q4(0, M.MHIP_F32, [1], [n], k.reshape(n, -1), v, n)
+        q = np.zeros((top, heads, 64))
+        q[:, :, 7] = 400
+        (ks, km), (vs, vm) = c.parts(0, 0, 1), c.parts(1, 0, 1)
+        score = (ks + km)[:, 0, 7] * 400 / 8
+        assert np.diff(np.sort(score)).min() > 30 and score.max() > 20000
+        c.set_weights(np.zeros_like(c.w))
+        got = call(c, 0, t, heads, q.reshape(top, -1), [1], [top], top, n, 0.125)
+        w = g.download(c.d_w, c.w.shape, np.float32)[0, 1, :, :n]
+        want = np.zeros(n)
+        few = 2.0 ** -20 if t == M.MHIP_F32 else 2.0 ** -16
+        for j in range(top):
+            see = n - top + j + 1
+            at = int(score[:see].argmax())
+            want[at] += heads // 2
+            o = np.repeat((vs + vm)[at], heads // 2, 0)
+            size15 = np.repeat(np.repeat(vs[at].reshape(2, 2, 32).max(-1), 32, -1) * 15 / 14, heads // 2, 0)
+            off = 2.0 ** -20 * np.repeat((vs + np.abs(vm))[at], heads // 2, 0) + few * size15 + 2.0 ** -34
+            tol = off + half_step(t, np.abs(o) + off)
+            assert (np.abs(got[j] - o) <= tol).all(), (j, (np.abs(got[j] - o) / tol).max())
+        assert (np.abs(w - want) <= 2.0 ** -20 * want + 2.0 ** -40).all()
+    finally:
+        c.close()
+
+
+def test_pages_behind_32_bits_hold_what_is_attended_to(g):
+    """Pages beyond 2^32 bytes of both arrays, by the s c and m that were written there: the bound is so small that
+    zeros, or the tokens in another order of pages, would not pass."""
+    d = M.PageDims(M.MHIP_Q4, 9, 8, 256, 128, 4 * 1024, 2, 4)
+    p = M.Pages(g, d)
+    rng = np.random.default_rng(10)
+    held = []
+
+    def up(x, dt=np.int32):
+        held.append(g.upload(np.ascontiguousarray(x, dt)))
+        return held[-1]
+    L = M.lib()
+    try:
+        table = np.full((2, 4), -1, np.int32)
+        table[1, :3] = [d.n_pages - 1, 0, d.n_pages - 2]
+        lens = np.array([0, 300], np.int32)
+        for at, x in ((p.arrays.table, table), (p.arrays.len, lens)):
+            g.check(L.mhip_h2d(g.h, at, x.ctypes.data, x.nbytes), "h2d")
+        width = 8 * 256
+        rows = [rng.standard_normal((300, width)).astype(np.float32) for _ in (0, 1)]
+        p.write_q4(8, M.MHIP_F32, up([1]), up([300]), 1, 300, *(up(x, np.float32) for x in rows), width)
+        k, v = ([x.astype(np.float64) for x in (s[..., None] * code.astype(np.float64), m[..., None] + 0.0 * code)]
+                for code, s, m in (codes_of(x.reshape(300, 8, -1, 32)) for x in rows))
+        k, v = ([x.reshape(300, 8, 256) for x in y] for y in (k, v))
+        q = rng.standard_normal((1, width)).astype(np.float32) * 2
+        out = up(np.zeros((1, width)), np.float32)
+        ws = up(np.zeros(p.attention_q4_ws_bytes(M.MHIP_F32, 8, 1, 1, 300, True)), np.uint8)
+        sums = np.zeros(p.weights_bytes() // 4, np.float32)
+        dw = up(sums, np.float32)
+        p.attention_q4(8, M.MHIP_F32, 8, up(q, np.float32), width, out, width, up([1]), None, 1, 1, 300, 1 / 16, dw, ws)
+        got = g.download(out, (8, 256), np.float32)
+        x = q.astype(np.float64).reshape(8, 256)
+        o, w, err = rows_of(x, k, v, 1 / 16)
+        off, fw = bound(M.MHIP_F32, w, v, err, 3)
+        tol = off + half_step(M.MHIP_F32, np.abs(o) + off)
+        assert tol.max() < 0.02 and np.abs(o).max() > 0.5
+        other = np.r_[128:256, 0:128, 256:300]
+        for wrong in (0 * o, rows_of(x, k, [a[other] for a in v], 1 / 16)[0], rows_of(x, [a[other] for a in k], v, 1 / 16)[0]):
+            assert (np.abs(wrong - o) > tol).mean() > 0.5
+        assert (np.abs(got - o) <= tol).all(), (np.abs(got - o) / tol).max()
+        got_w = g.download(dw, sums.shape, np.float32).reshape(9, 2, 8, -1)
+        assert (np.abs(got_w[8, 1, :, :300] - w) <= (fw + 2.0 ** -20) * w).all()
+        got_w[8, 1, :, :300] = 0
+        assert (got_w == 0).all() and p.status()[0] == 0
+    finally:
+        for h in held:
+            g.free(h)
+        p.close()
