@@ -588,7 +588,7 @@ int mhip_attention_shared(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages
  * Rows into the cache, as mhip_pages_write takes them, of `type` (MHIP_F32,
  * MHIP_F16 or MHIP_BF16): m is the least of 32 values rounded to fp16, s a
  * fifteenth of what the greatest is above m (0 if it is not), rounded to fp32 and then to
- * fp16, and c the nearest code (halves up). Values are kept within +-2^15, NaN as 0, with error
+ * fp16, and c the nearest code (halves up, by x - m in 64 bits). Values are kept within +-2^15, NaN as 0, with error
  * bit MHIP_PAGES_NOT_FINITE. d_weights (NULL: none): the tokens' accumulated weights
  * of this layer (below) become 0. */
 int mhip_pages_write_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p, int layer,

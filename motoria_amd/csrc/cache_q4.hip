@@ -5,8 +5,9 @@
 // s = fp16((hi - m) / 15) with an fp32 difference and quotient, and
 //   c = how many k of 0 .. 14 have x - m >= (k + 1/2) s   (0 where s is 0).
 // The nearest code is estimated in fp32; where the estimate is within 2^-16 of a border
-// (its own error is below 2^-17) the comparison is made in 64 bits, in which x - m and
-// (k + 1/2) s are exact, so a code does not depend on how it was found.
+// (its own error is below 2^-17) the comparison is made in 64 bits, in which (k + 1/2) s is exact
+// and x - m is rounded once (exact unless x and m are more than 2^29 apart in size). That difference is the
+// definition's, so a code does not depend on how it was found.
 //
 // A thread has eight values of a token, or of four tokens that lie in a word of values' codes
 // (whose bytes are four tokens', and s and m the same): with a byte and two a store, prompts of
