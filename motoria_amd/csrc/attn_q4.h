@@ -55,9 +55,10 @@ struct Cut {
 };
 
 
-// Tiles of 16 rows of a workgroup that has more than one: two share a tile's codes and s. Heads of more
-// than 128 elements leave no registers for them (a chunk of 500 tokens over 6000, heads of 256: 79 us
-// with one, 84 with two; heads of 128 in fp32 193 with two, 200 with one).
+// Tiles of 16 rows of a workgroup that has more than one: two share a tile's codes and s (a chunk of 500
+// tokens over 6000, 32 heads over 4 of 128: bf16 152 us with two, 182 with one, fp32 159 and 192). With heads
+// of more than 128 elements two take more registers than half of a SIMD's, and half as many workgroups: 8 heads over 2
+// of 256 98 us with one, 102 with two; with more of them two would be faster (16 heads 153, with one 191).
 constexpr int wide_tiles(int groups) { return groups > 4 ? 1 : 2; }
 
 int launch_f32(mhip_ctx *c, const Job &a, const Cut &k);

@@ -19,16 +19,16 @@ int up(long long n, int to) { return (int)((n + to - 1) / to * to); }
 // How a call is cut. Up to 512 positions a workgroup takes an item whole, which saves the join
 // (5 us with its launch). Longer ones are cut into parts for all workgroups to be on their CUs at
 // once, with some to spare, as an item's last part is shorter (two on a CU, one with heads of more than
-// 192 elements, whose stages are large): 32 slots of up to 8000 positions 34.6 us with 448 parts in
-// all, 37.5 with 640, and 40 to 46 where some had to wait for others to end; 16 slots of up to 2900
-// 18.2, 19.2 with 640.
+// 192 elements, whose stages are large): 32 slots of up to 8000 positions 41.4 us with 448 parts in
+// all, 44 with 640 and 47 with 896, where some have to wait for others to end; 16 slots of up to 2900
+// 19.4, 20.5 with 640 and 20.9 with 896.
 constexpr int WHOLE = 512, PARTS = 448, PARTS_LARGE = 224, LEAST = 2;
 
 // Weights are added up from kept scores where a slot and head have one tile of up to 16 rows, some
 // 2048 workgroups of 256 positions at least (memory is what they wait for). Else they are from
 // new scores, by wavefronts that share positions where there are enough rows for them, with more
-// positions for each once 256 workgroups have some (a chunk of 500 tokens over 6000: 283 us with its
-// attention, 295 with 512 workgroups; 8 drafted tokens of 8 slots of up to 1000, fp32: 34 both).
+// positions for each once 256 workgroups have some (a chunk of 500 tokens over 6000: 299 us with its
+// attention, 315 with 512 workgroups; 8 drafted tokens of 8 slots of up to 1000, fp32: 32 both).
 constexpr int SUM_WGS = 256;
 bool kept(const Cut &k) { return k.nq == 1 && k.tiles == 1; }
 
@@ -40,7 +40,7 @@ Cut cut_of(const mhip_page_dims *s, int n_heads, int n, int mc, int max_len) {
     const long long items = (long long)n * k.tiles;
     const int parts = s->head_dim > 192 ? PARTS_LARGE : PARTS;
     // (a chunk at a slot's end: all items are about as long and none would be cut; 500 tokens over 6000
-    // 108 us so, 113 with a join that finds nothing to do)
+    // 152 us so, 160 with a join that finds nothing to do)
     const bool alike = n == 1 && mc <= max_len / 2 && items * s->n_kv_heads >= parts;
     const bool cut = items <= mhip_q4::ITEMS_MAX && max_len > WHOLE && items * s->n_kv_heads < 4 * parts && !alike;
     k.wgs = cut ? (parts + s->n_kv_heads - 1) / s->n_kv_heads : 0;
