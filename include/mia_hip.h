@@ -608,7 +608,7 @@ int mhip_pages_read_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p
  * largest of their row, 16-bit ones whole, but for what is below 2^-34 of that.
  * Scores, softmax and sums are fp32; a weight enters the sums over the values and over the weights
  * within 2^-22 of its size or 2^-34 of the row's largest; its product with s within 2^-21 of its
- * size, or the products of a row and 32 values are, all together, within 2^-20 (16-bit rows 2^-16) of
+ * size, or the products of a row and 32 values are, all together, within 2^-18 (16-bit rows 2^-15) of
  * the sum of weight x 15 s over the tokens that the row sees. (Values whose sizes are so far apart that
  * the fast way would be off by more are worked on twice.) Sums over an m below 2^-14 are within
  * 2^-14 of their size.
