@@ -610,8 +610,8 @@ int mhip_pages_read_q4(mhip_ctx *c, const mhip_page_dims *s, const mhip_pages *p
  * within 2^-22 of its size or 2^-34 of the row's largest; its product with s within 2^-21 of its
  * size, or the products of a row and 32 values are, all together, within 2^-18 (16-bit rows 2^-15) of
  * the sum of weight x 15 s over the tokens that the row sees. (Values whose sizes are so far apart that
- * the fast way would be off by more are worked on twice.) Sums over an m below 2^-14 are within
- * 2^-14 of their size.
+ * the fast way would be off by more are worked on twice.) The product of an m below 2^-14 is
+ * cut at 2^-37 of the row's largest weight (of keys: of the largest sum of a query's 32 values).
  *
  * d_weights (NULL: not added up): [n_layers][max_seqs][n_kv_heads][max_blocks *
  * page] floats, mhip_weights_bytes() in all, 16-byte aligned: for each token of a slot

@@ -422,3 +422,33 @@ def test_a_wavefront_on_its_own_goes_twice(g, t, heads, count, n, parts):
         check(c, t, heads, q.reshape(len(q), -1), seqs, counts, count, n, 1.0, n // 128 + 1, 1, weights=True)
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("t", [M.MHIP_F32, M.MHIP_BF16])
+@pytest.mark.parametrize("size", [2.0 ** -13, 2.0 ** -17, 2.0 ** -21])
+def test_the_smallest_values(g, t, size):
+    """Keys and values whose m (and s) are below fp16's normal range: products with such an m are cut at 2^-37 of the
+    largest weight, or of the largest of the query's sums over a group (three pieces of it for each group)."""
+    print("test_the_smallest_values", t, size, flush=True)
+    n, heads, hd = 200, 4, 64
+    c = CacheQ4(g, n_layers=1, n_kv_heads=1, head_dim=hd, page=16, n_pages=20, max_blocks=13, max_seqs=1)
+    rng = np.random.default_rng(15)
+    scale = 0.25 / size
+    try:
+        c.extend([0], [n])
+        k, v = (rng.standard_normal((n, hd)) * size for _ in (0, 1))
+        c.write_q4(0, M.MHIP_F32, [0], [n], k, v, n)
+        q = rng.standard_normal((1, heads, hd)) * 0.5
+        got = call(c, 0, t, heads, q.reshape(1, -1), [0], None, 1, n, scale, weights=False)
+        x = c.rows_of(q.reshape(1, -1), 0, t)[1].astype(np.float64).reshape(heads, hd)
+        k, v = c.parts(0, 0, 0), c.parts(1, 0, 0)
+        o, w, err = rows_of(x, k, v, scale)
+        off, _ = bound(t, w, v, err, 2)
+        cut = scale * 6 * 2.0 ** -37 * np.abs(x.reshape(heads, 2, 32).sum(-1)).max(-1)
+        off = off + 2 * cut[:, None] * np.einsum("ht,thd->hd", w, np.repeat((v[0] + np.abs(v[1])), heads, 1))
+        off = off + n * 2.0 ** -37 * w.max(1)[:, None]
+        assert off.max() < size / 16
+        tol = off + half_step(t, np.abs(o) + off)
+        assert (np.abs(got[0] - o) <= tol).all(), (np.abs(got[0] - o) / tol).max()
+    finally:
+        c.close()
